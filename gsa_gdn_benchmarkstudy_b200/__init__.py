@@ -11,6 +11,7 @@ nirmalpratheep/GSA_GDN_BenchmarkStudy:
 The compute runs in ``libgsa_b200.so`` (built by ``python -m
 gsa_gdn_benchmarkstudy_b200.build``); there is no CPU fallback.
 """
+from .delta import gated_delta_rule, gated_delta_step  # noqa: F401
 from .gsa import (  # noqa: F401
     AdaptiveTopKSelector,
     GatedLightningIndexer,
@@ -22,10 +23,12 @@ from .gsa import (  # noqa: F401
     ValueGate,
     apply_rotary_pos_emb,
 )
+from .norm import rms_norm, rms_norm_fp8  # noqa: F401
 from .ops import fused_gated_indexer, fused_sparse_attention, sparse_attention_ref  # noqa: F401
 
 __all__ = [
     "GatedSparseAttention", "GraphedForward", "GraphedForwardHost", "GatedLightningIndexer",
     "AdaptiveTopKSelector", "ValueGate", "OutputGate", "RotaryEmbedding", "apply_rotary_pos_emb", "fused_gated_indexer",
-    "fused_sparse_attention", "sparse_attention_ref",
+    "fused_sparse_attention", "sparse_attention_ref", "gated_delta_rule", "gated_delta_step",
+    "rms_norm", "rms_norm_fp8",
 ]

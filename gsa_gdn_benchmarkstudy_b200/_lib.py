@@ -18,11 +18,28 @@ GSA_DTYPE_BF16 = 0
 GSA_DTYPE_F32 = 1
 GSA_FUSED_AUTO, GSA_FUSED_ALWAYS, GSA_FUSED_NEVER = 0, 1, 2
 
+GSA_DELTA_INFERENCE, GSA_DELTA_TRAINING, GSA_DELTA_BACKWARD = 0, 1, 2
+
+
+class DeltaArgs(ctypes.Structure):
+    """gsa_delta_t of include/gsa_b200.h."""
+
+    _fields_ = (
+        [(n, ctypes.c_void_p) for n in ("q", "k", "v", "g", "beta")]
+        + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+        + [(n, ctypes.c_int64 * 2) for n in ("g_stride", "beta_stride")]
+        + [(n, ctypes.c_void_p) for n in ("cu_seqlens", "initial_state")]
+        + [("dtype", ctypes.c_int), ("gate_dtype", ctypes.c_int), ("scale", ctypes.c_float)]
+        + [(n, ctypes.c_int) for n in ("B", "T", "Hk", "Hv", "dk", "dv", "N")]
+    )
+
+
 # Every exported symbol of include/gsa_b200.h with (restype, argtypes).
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_dp = ctypes.POINTER(DeltaArgs)
 SIGNATURES: dict[str, tuple] = {
     "gsa_version": (_i32, []),
     "gsa_set_fused_selection": (_i32, [_i32]),
@@ -91,6 +108,28 @@ SIGNATURES: dict[str, tuple] = {
     "gsa_fused_projection_pack": (
         _i32,
         [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp],
+    ),
+    "gsa_delta_rule_workspace_size": (_i64, [_dp, _i32]),
+    "gsa_delta_rule_forward": (_i32, [_dp, _vp, _vp, _i32, _vp, _i64, _vp]),
+    "gsa_delta_rule_backward": (
+        _i32,
+        [_dp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "gsa_delta_step": (_i32, [_dp, _vp, _i64, _vp, _vp, _vp]),
+    "gsa_rms_norm": (
+        _i32,
+        [_vp, _i64, _vp, _i64, _vp, _i32, _f32, _i32, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _vp],
+    ),
+    "gsa_rms_norm_fp8": (
+        _i32,
+        [_vp, _i64, _vp, _i64, _vp, _i32, _f32, _i32, _i64, _i32, _vp, _i64, _vp, _i32, _vp, _i64,
+         _vp],
+    ),
+    "gsa_rms_norm_backward_workspace_size": (_i64, [_i64, _i32]),
+    "gsa_rms_norm_backward": (
+        _i32,
+        [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _i32, _i64, _i32, _vp, _i64, _vp, _vp,
+         _i64, _vp],
     ),
 }
 

@@ -914,4 +914,230 @@ int gsa_fused_projection(const void* x, int64_t x_stride, const void* w_packed,
                                       static_cast<cudaStream_t>(stream)));
 }
 
+namespace {
+int check_delta(const gsa_delta_t* p) {
+  if (!p) return set_error(GSA_ERR_INVALID_ARG, "NULL arguments");
+  if (p->B < 0 || p->T < 0 || p->N < 0 || p->Hk <= 0 || p->Hv <= 0 || p->dk <= 0 || p->dv <= 0)
+    return set_error(GSA_ERR_INVALID_ARG, "bad sizes");
+  if (p->Hv % p->Hk) return set_error(GSA_ERR_INVALID_ARG, "Hv must be a multiple of Hk");
+  if ((p->dtype != GSA_DTYPE_BF16 && p->dtype != GSA_DTYPE_F32) ||
+      (p->gate_dtype != GSA_DTYPE_BF16 && p->gate_dtype != GSA_DTYPE_F32))
+    return set_error(GSA_ERR_UNSUPPORTED, "dtype and gate_dtype must be bf16 or f32");
+  if (p->dk % 8 || p->dv % 8 || p->dk > gsa::kDeltaMaxDk || p->dv > gsa::kDeltaMaxDv)
+    return set_error(GSA_ERR_UNSUPPORTED, "dk and dv must be multiples of 8, dk <= 128, dv <= 256");
+  if (p->Hv > 65535) return set_error(GSA_ERR_UNSUPPORTED, "more than 65535 heads");
+  return GSA_OK;
+}
+
+bool delta_rows_aligned(const void* q, const int64_t* stride) {
+  return aligned16(q) && stride[0] % 8 == 0 && stride[1] % 8 == 0 && stride[2] % 8 == 0;
+}
+
+int check_delta_inputs(const gsa_delta_t* p) {
+  if (static_cast<int64_t>(p->B) * p->T == 0) return GSA_OK;
+  if (!p->q || !p->k || !p->v || !p->g || !p->beta)
+    return set_error(GSA_ERR_INVALID_ARG, "q / k / v / g / beta is NULL");
+  if (p->dtype == GSA_DTYPE_BF16 &&
+      !(delta_rows_aligned(p->q, p->q_stride) && delta_rows_aligned(p->k, p->k_stride) &&
+        delta_rows_aligned(p->v, p->v_stride)))
+    return set_error(GSA_ERR_ALIGNMENT, "bf16 q, k, v rows must be 16-byte aligned");
+  return GSA_OK;
+}
+
+// What holds for whole sequences on top of check_delta.
+int check_delta_rule(const gsa_delta_t* p) {
+  int rc = check_delta(p);
+  if (rc) return rc;
+  if (p->cu_seqlens) {
+    if (p->B != 1) return set_error(GSA_ERR_INVALID_ARG, "cu_seqlens needs B == 1");
+    if (p->N < 1) return set_error(GSA_ERR_INVALID_ARG, "cu_seqlens needs N >= 1");
+  } else if (p->N != p->B) {
+    return set_error(GSA_ERR_INVALID_ARG, "N must equal B without cu_seqlens");
+  }
+  // the kernels count tokens and chunks in 32 bits
+  if (static_cast<int64_t>(p->T) + p->N > INT32_MAX - 256 ||
+      static_cast<int64_t>(p->B) * (p->T / 64 + 1) > INT32_MAX - 256)
+    return set_error(GSA_ERR_UNSUPPORTED, "too many tokens");
+  return GSA_OK;
+}
+}  // namespace
+
+int64_t gsa_delta_rule_workspace_size(const gsa_delta_t* p, int use) {
+  if (check_delta_rule(p)) return -1;
+  switch (use) {
+    case GSA_DELTA_INFERENCE: return gsa::delta::simt_saved_bytes(*p, false);
+    case GSA_DELTA_TRAINING: return gsa::delta::simt_saved_bytes(*p, true);
+    case GSA_DELTA_BACKWARD: return gsa::delta::simt_scratch_bytes(*p);
+    default: set_error(GSA_ERR_INVALID_ARG, "unknown use"); return -1;
+  }
+}
+
+int gsa_delta_rule_forward(const gsa_delta_t* p, void* o, float* final_state, int use,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  int rc = check_delta_rule(p);
+  if (rc) return rc;
+  if (use != GSA_DELTA_INFERENCE && use != GSA_DELTA_TRAINING)
+    return set_error(GSA_ERR_INVALID_ARG, "use must be inference or training");
+  if (p->B == 0 || p->N == 0) return GSA_OK;
+  if ((rc = check_delta_inputs(p))) return rc;
+  if (!o && p->T > 0) return set_error(GSA_ERR_INVALID_ARG, "o is NULL");
+  if (p->dtype == GSA_DTYPE_BF16 && !aligned16(o))
+    return set_error(GSA_ERR_ALIGNMENT, "o must be 16-byte aligned");
+  const int64_t need = gsa_delta_rule_workspace_size(p, use);
+  if (need > 0 && !workspace) return set_error(GSA_ERR_INVALID_ARG, "workspace is NULL");
+  if (workspace_bytes < need)
+    return set_error(GSA_ERR_INVALID_ARG, "workspace smaller than gsa_delta_rule_workspace_size");
+  if (!aligned16(workspace)) return set_error(GSA_ERR_ALIGNMENT, "workspace not 16-byte aligned");
+  DeviceState* st = nullptr;
+  if ((rc = device_state(&st))) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = gsa::delta::launch_table(*p, workspace, st->err, s);
+  if (e == cudaSuccess)
+    e = gsa::delta::simt_forward(*p, o, final_state, use == GSA_DELTA_TRAINING, workspace, s);
+  return finish(e);
+}
+
+int gsa_delta_rule_backward(const gsa_delta_t* p, const void* dout, const float* dfinal,
+                            const void* saved, int64_t saved_bytes, void* scratch,
+                            int64_t scratch_bytes, void* dq, void* dk, void* dv, void* dg,
+                            void* dbeta, float* dinitial, void* stream) {
+  int rc = check_delta_rule(p);
+  if (rc) return rc;
+  if (p->B == 0 || p->N == 0) return GSA_OK;
+  if ((rc = check_delta_inputs(p))) return rc;
+  if (p->T > 0 && (!dq || !dk || !dv || !dg || !dbeta))
+    return set_error(GSA_ERR_INVALID_ARG, "dq / dk / dv / dg / dbeta is NULL");
+  if (p->dtype == GSA_DTYPE_BF16 &&
+      (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)))
+    return set_error(GSA_ERR_ALIGNMENT, "bf16 gradients must be 16-byte aligned");
+  const int64_t need = gsa_delta_rule_workspace_size(p, GSA_DELTA_TRAINING);
+  const int64_t need_scratch = gsa_delta_rule_workspace_size(p, GSA_DELTA_BACKWARD);
+  if ((need > 0 && !saved) || (need_scratch > 0 && !scratch))
+    return set_error(GSA_ERR_INVALID_ARG, "saved / scratch is NULL");
+  if (saved_bytes < need || scratch_bytes < need_scratch)
+    return set_error(GSA_ERR_INVALID_ARG,
+                     "saved / scratch smaller than gsa_delta_rule_workspace_size");
+  if (!aligned16(saved) || !aligned16(scratch))
+    return set_error(GSA_ERR_ALIGNMENT, "saved / scratch not 16-byte aligned");
+  DeviceState* st = nullptr;
+  if ((rc = device_state(&st))) return rc;
+  const gsa::DeltaGrads g = {dout, dfinal, dq, dk, dv, dg, dbeta, dinitial};
+  return finish(gsa::delta::simt_backward(*p, g, const_cast<void*>(saved), scratch,
+                                          static_cast<cudaStream_t>(stream)));
+}
+
+int gsa_delta_step(const gsa_delta_t* p, float* state, int64_t slots, const int32_t* indices,
+                   void* o, void* stream) {
+  int rc = check_delta(p);
+  if (rc) return rc;
+  if (slots < 0) return set_error(GSA_ERR_INVALID_ARG, "slots < 0");
+  if (!indices && slots < p->B)
+    return set_error(GSA_ERR_INVALID_ARG, "fewer state slots than rows, and no indices");
+  if (p->B == 0 || p->T == 0) return GSA_OK;
+  if ((rc = check_delta_inputs(p))) return rc;
+  if (!o || (!state && slots > 0)) return set_error(GSA_ERR_INVALID_ARG, "o / state is NULL");
+  if (!aligned16(state)) return set_error(GSA_ERR_ALIGNMENT, "state must be 16-byte aligned");
+  DeviceState* st = nullptr;
+  if ((rc = device_state(&st))) return rc;
+  return finish(gsa::launch_delta_step(*p, state, slots, indices, o, st->err,
+                                       static_cast<cudaStream_t>(stream)));
+}
+
+namespace {
+int check_norm(int dtype, int weight_dtype, int64_t rows, int width) {
+  if (rows < 0 || width <= 0) return set_error(GSA_ERR_INVALID_ARG, "bad sizes");
+  if ((dtype != GSA_DTYPE_BF16 && dtype != GSA_DTYPE_F32) ||
+      (weight_dtype != GSA_DTYPE_BF16 && weight_dtype != GSA_DTYPE_F32))
+    return set_error(GSA_ERR_UNSUPPORTED, "dtype and weight_dtype must be bf16 or f32");
+  if (width > gsa::kRmsNormMaxWidth)
+    return set_error(GSA_ERR_UNSUPPORTED, "width > 32768");
+  if (rows > INT32_MAX) return set_error(GSA_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
+  return GSA_OK;
+}
+
+int rms_norm_impl(gsa::RmsNormArgs a, int dtype, int weight_dtype, void* stream) {
+  int rc = check_norm(dtype, weight_dtype, a.rows, a.width);
+  if (rc) return rc;
+  if (a.rows == 0) return GSA_OK;
+  if (!a.x || !a.weight || !a.y) return set_error(GSA_ERR_INVALID_ARG, "x / weight / y is NULL");
+  if (a.residual && !a.h) return set_error(GSA_ERR_INVALID_ARG, "a residual needs h");
+  if (a.x_stride < 0 || a.y_stride < a.width || (a.residual && a.residual_stride < 0) ||
+      (a.residual && a.h_stride < a.width))
+    return set_error(GSA_ERR_INVALID_ARG, "bad row stride");
+  a.weight_f32 = weight_dtype == GSA_DTYPE_F32;
+  DeviceState* st = nullptr;
+  if ((rc = device_state(&st))) return rc;
+  const cudaError_t e = gsa::launch_rms_norm(a, dtype, static_cast<cudaStream_t>(stream));
+  if (e == cudaErrorMisalignedAddress)
+    return set_error(GSA_ERR_ALIGNMENT, "group scales need 16-byte aligned rows");
+  return finish(e);
+}
+}  // namespace
+
+int gsa_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                 const void* weight, int weight_dtype, float eps, int dtype, int64_t rows,
+                 int width, void* y, int64_t y_stride, void* h, int64_t h_stride, float* rstd,
+                 void* stream) {
+  const gsa::RmsNormArgs a = {x,    x_stride, residual, residual_stride, weight, false, eps, rows,
+                              width, y,       y_stride, h, h_stride, rstd, nullptr, 0};
+  return rms_norm_impl(a, dtype, weight_dtype, stream);
+}
+
+int gsa_rms_norm_fp8(const void* x, int64_t x_stride, const void* residual,
+                     int64_t residual_stride, const void* weight, int weight_dtype, float eps,
+                     int dtype, int64_t rows, int width, void* y, int64_t y_stride, float* scale,
+                     int group, void* h, int64_t h_stride, void* stream) {
+  if (group != 0 && (group != 128 || width % 128))
+    return set_error(GSA_ERR_UNSUPPORTED, "group must be 0, or 128 with width a multiple of 128");
+  if (rows > 0 && !scale) return set_error(GSA_ERR_INVALID_ARG, "scale is NULL");
+  const gsa::RmsNormArgs a = {x,    x_stride, residual, residual_stride, weight, false, eps, rows,
+                              width, y,       y_stride, h, h_stride, nullptr, scale, group};
+  return rms_norm_impl(a, dtype, weight_dtype, stream);
+}
+
+int64_t gsa_rms_norm_backward_workspace_size(int64_t rows, int width) {
+  if (rows <= 0 || width <= 0 || width > gsa::kRmsNormMaxWidth) return 0;
+  return static_cast<int64_t>(gsa::rms_norm_backward_blocks(rows, width)) * width * 4;
+}
+
+int gsa_rms_norm_backward(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride,
+                          const void* h, int64_t h_stride, const void* weight, int weight_dtype,
+                          const float* rstd, int dtype, int64_t rows, int width, void* dx,
+                          int64_t dx_stride, void* dweight, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  int rc = check_norm(dtype, weight_dtype, rows, width);
+  if (rc) return rc;
+  if (rows == 0 && !dweight) return GSA_OK;
+  if (rows > 0 && (!dy || !h || !weight || !rstd || !dx))
+    return set_error(GSA_ERR_INVALID_ARG, "dy / h / weight / rstd / dx is NULL");
+  if (rows > 0 && (dy_stride < 0 || h_stride < 0 || (dh && dh_stride < 0) || dx_stride < width))
+    return set_error(GSA_ERR_INVALID_ARG, "bad row stride");
+  const int64_t need = dweight ? gsa_rms_norm_backward_workspace_size(rows, width) : 0;
+  if (need > 0 && !workspace) return set_error(GSA_ERR_INVALID_ARG, "workspace is NULL");
+  if (workspace_bytes < need)
+    return set_error(GSA_ERR_INVALID_ARG,
+                     "workspace smaller than gsa_rms_norm_backward_workspace_size");
+  if (reinterpret_cast<uintptr_t>(workspace) % 4)
+    return set_error(GSA_ERR_ALIGNMENT, "workspace must be 4-byte aligned");
+  DeviceState* st = nullptr;
+  if ((rc = device_state(&st))) return rc;
+  gsa::RmsNormBackwardArgs a = {};
+  a.dy = dy;
+  a.dy_stride = dy_stride;
+  a.dh = dh;
+  a.dh_stride = dh_stride;
+  a.h = h;
+  a.h_stride = h_stride;
+  a.weight = weight;
+  a.weight_f32 = weight_dtype == GSA_DTYPE_F32;
+  a.rstd = rstd;
+  a.rows = rows;
+  a.width = width;
+  a.dx = dx;
+  a.dx_stride = dx_stride;
+  a.partial = dweight ? static_cast<float*>(workspace) : nullptr;
+  a.dweight = dweight;
+  return finish(gsa::launch_rms_norm_backward(a, dtype, static_cast<cudaStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -193,6 +193,73 @@ cudaError_t launch_proj_gemm(const CUtensorMap& xmap, const CUtensorMap& wmap,
                              const CUtensorMap& vmap, const CUtensorMap& rmap,
                              const ProjGemmArgs& a, int clusters, cudaStream_t stream);
 
+// RMS norm (norm.cu).  Strides in elements between rows.
+constexpr int kRmsNormMaxWidth = 32768;  // 1024 threads x 4 vectors of 8 values hold a row
+struct RmsNormArgs {
+  const void* x;
+  int64_t x_stride;
+  const void* residual;  // nullptr: h is x
+  int64_t residual_stride;
+  const void* weight;    // [width]
+  bool weight_f32;       // else bf16
+  float eps;
+  int64_t rows;
+  int width;
+  void* y;               // the inputs' type, or e4m3 bytes when scale is set
+  int64_t y_stride;
+  void* h;               // x + residual, set with residual
+  int64_t h_stride;
+  float* rstd;           // optional [rows]
+  float* scale;          // e4m3: [rows] (group 0) or [rows, width / 128] (group 128)
+  int group;
+};
+cudaError_t launch_rms_norm(const RmsNormArgs& a, int dtype, cudaStream_t stream);
+
+struct RmsNormBackwardArgs {
+  const void* dy;
+  int64_t dy_stride;
+  const void* dh;        // optional gradient of h
+  int64_t dh_stride;
+  const void* h;
+  int64_t h_stride;
+  const void* weight;
+  bool weight_f32;
+  const float* rstd;     // [rows], from the forward pass
+  int64_t rows;
+  int width;
+  void* dx;
+  int64_t dx_stride;
+  float* partial;        // [rms_norm_backward_blocks, width]; nullptr: no dweight
+  void* dweight;         // [width], weight's type
+};
+int rms_norm_backward_blocks(int64_t rows, int width);
+cudaError_t launch_rms_norm_backward(const RmsNormBackwardArgs& a, int dtype, cudaStream_t stream);
+
+// Gated delta rule (delta_*.cu).
+constexpr int kDeltaMaxDk = 128;
+constexpr int kDeltaMaxDv = 256;
+// Upstream gradients (each may be nullptr) and where the gradients go
+// (contiguous; dinitial may be nullptr).
+struct DeltaGrads {
+  const void* dout;
+  const float* dfinal;
+  void *dq, *dk, *dv, *dg, *dbeta;
+  float* dinitial;
+};
+cudaError_t launch_delta_step(const gsa_delta_t& p, float* state, int64_t slots,
+                              const int32_t* indices, void* o, int* err, cudaStream_t stream);
+namespace delta {
+// The chunk table of a packed batch, at the start of the forward's workspace.
+cudaError_t launch_table(const gsa_delta_t& p, void* workspace, int* err, cudaStream_t stream);
+// fp32 inputs.  save: the workspace keeps what the backward pass reads.
+int64_t simt_saved_bytes(const gsa_delta_t& p, bool save);
+int64_t simt_scratch_bytes(const gsa_delta_t& p);
+cudaError_t simt_forward(const gsa_delta_t& p, void* o, float* final_state, bool save, void* ws,
+                         cudaStream_t stream);
+cudaError_t simt_backward(const gsa_delta_t& p, const DeltaGrads& g, void* saved, void* scratch,
+                          cudaStream_t stream);
+}  // namespace delta
+
 cudaError_t launch_gather_attention(const void* q, int64_t q_stride, const void* k,
                                     int64_t k_stride, const void* v, int64_t v_stride,
                                     const int32_t* indices, const uint8_t* mask, int k_sel,

@@ -1,0 +1,235 @@
+"""The gated delta rule: whole sequences with gradients, and decoding steps.
+
+The token mixer that the benchmark study sets beside gated sparse attention
+(the reference's benchmark_models.ipynb:187-225 states it token by token).  Per
+sequence and value head, with a state S [dk, dv]:
+
+    S_t = exp(g_t) S_{t-1} + k_t u_t^T
+    u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t)
+    o_t = scale S_t^T q_t
+
+``gated_delta_rule`` computes it chunk by chunk for training and prompts,
+``gated_delta_step`` token by token against a pool of states for decoding.
+Both run on the tensors' device and its current stream; there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _cuda, _dtype_code, _ptr
+
+
+def _strides(t: torch.Tensor, n: int) -> list:
+    """The first n strides, 0 for a dimension of one element (never stepped over)."""
+    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(n)]
+
+
+def _rows_ok(t: torch.Tensor) -> torch.Tensor:
+    """t [B, T, H, d] as the kernels read it: unit inner stride, rows on 16 bytes in bf16;
+    copied where it is not."""
+    bf16 = t.dtype == torch.bfloat16
+    if t.numel() and (
+            (t.shape[3] > 1 and t.stride(3) != 1)
+            or (bf16 and (t.data_ptr() % 16 or any(s % 8 for s in _strides(t, 3))))):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _gates_ok(t: torch.Tensor) -> torch.Tensor:
+    if t.numel() and t.shape[2] > 1 and t.stride(2) != 1:
+        return t.contiguous()
+    return t
+
+
+def _check(q, k, v, g, beta, *others) -> None:
+    _cuda(q, k, v, g, beta, *others)
+    for name, t, dims in (("q", q, 4), ("k", k, 4), ("v", v, 4), ("g", g, 3), ("beta", beta, 3)):
+        if t.dim() != dims:
+            raise ValueError(f"{name}: expected {dims} dims, got {tuple(t.shape)}")
+    _dtype_code(q), _dtype_code(g)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must share a dtype")
+    if beta.dtype != g.dtype:
+        raise ValueError("g and beta must share a dtype")
+    B, T, Hk, dk = q.shape
+    if k.shape != q.shape:
+        raise ValueError(f"k must be [{B}, {T}, {Hk}, {dk}], got {tuple(k.shape)}")
+    Hv, dv = v.shape[2], v.shape[3]
+    if v.shape[:2] != (B, T) or Hk == 0 or Hv == 0 or Hv % Hk:
+        raise ValueError(f"v must be [{B}, {T}, Hv, dv] with Hv a multiple of {Hk}, got "
+                         f"{tuple(v.shape)}")
+    for name, t in (("g", g), ("beta", beta)):
+        if t.shape != (B, T, Hv):
+            raise ValueError(f"{name} must be [{B}, {T}, {Hv}], got {tuple(t.shape)}")
+    if dk % 8 or dv % 8 or not 0 < dk <= 128 or not 0 < dv <= 256:
+        raise ValueError(f"dk and dv must be multiples of 8, dk <= 128 and dv <= 256, got "
+                         f"{dk} and {dv}")
+    for t in (k, v, g, beta) + others:
+        if t is not None and t.device != q.device:
+            raise ValueError("all tensors must be on one device")
+
+
+def _args(q, k, v, g, beta, scale, N, cu, initial) -> _lib.DeltaArgs:
+    B, T, Hk, dk = q.shape
+    a = _lib.DeltaArgs()
+    for name, t, n in (("q", q, 3), ("k", k, 3), ("v", v, 3), ("g", g, 2), ("beta", beta, 2)):
+        setattr(a, name, t.data_ptr())
+        getattr(a, name + "_stride")[:] = _strides(t, n)
+    a.cu_seqlens, a.initial_state = _ptr(cu), _ptr(initial)
+    a.dtype, a.gate_dtype, a.scale = _dtype_code(q), _dtype_code(g), float(scale)
+    a.B, a.T, a.Hk, a.Hv, a.dk, a.dv, a.N = B, T, Hk, v.shape[2], dk, v.shape[3], N
+    return a
+
+
+def _workspace(a: _lib.DeltaArgs, use: int, device) -> torch.Tensor:
+    need = int(_lib.load().gsa_delta_rule_workspace_size(ctypes.byref(a), use))
+    if need < 0:
+        raise RuntimeError(f"gsa_delta_rule_workspace_size failed: {_lib.last_error()}")
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def _forward(q, k, v, g, beta, initial, cu, scale, N, want_final, use):
+    B, T, _, dk = q.shape
+    Hv, dv = v.shape[2], v.shape[3]
+    a = _args(q, k, v, g, beta, scale, N, cu, initial)
+    ws = _workspace(a, use, q.device)
+    o = torch.empty(B, T, Hv, dv, dtype=q.dtype, device=q.device)
+    final = (torch.empty(N, Hv, dk, dv, dtype=torch.float32, device=q.device) if want_final
+             else None)
+    rc = _lib.load().gsa_delta_rule_forward(
+        ctypes.byref(a), o.data_ptr(), _ptr(final), use, ws.data_ptr(), ws.numel(),
+        torch.cuda.current_stream().cuda_stream)
+    _lib.check(rc, "gsa_delta_rule_forward")
+    return o, final, ws
+
+
+class _GatedDeltaRule(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, initial, cu, scale, N, want_final):
+        with torch.cuda.device(q.device):
+            o, final, ws = _forward(q, k, v, g, beta, initial, cu, scale, N, want_final,
+                                    _lib.GSA_DELTA_TRAINING)
+        ctx.save_for_backward(q, k, v, g, beta, cu, ws)
+        ctx.scale, ctx.N, ctx.has_initial = scale, N, initial is not None
+        ctx.set_materialize_grads(False)
+        return o, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, dfinal):
+        q, k, v, g, beta, cu, ws = ctx.saved_tensors
+        B, T, Hk, dk = q.shape
+        Hv, dv_ = v.shape[2], v.shape[3]
+        if do is not None:
+            do = do.to(q.dtype).contiguous()
+            if do.data_ptr() % 16:
+                do = do.clone()
+        if dfinal is not None:
+            dfinal = dfinal.float().contiguous()
+        with torch.cuda.device(q.device):
+            a = _args(q, k, v, g, beta, ctx.scale, ctx.N, cu, None)
+            scratch = _workspace(a, _lib.GSA_DELTA_BACKWARD, q.device)
+            dq = torch.empty(B, T, Hk, dk, dtype=q.dtype, device=q.device)
+            dk_ = torch.empty_like(dq)
+            dv = torch.empty(B, T, Hv, dv_, dtype=q.dtype, device=q.device)
+            dg = torch.empty(B, T, Hv, dtype=g.dtype, device=q.device)
+            dbeta = torch.empty_like(dg)
+            dinitial = (torch.empty(ctx.N, Hv, dk, dv_, dtype=torch.float32, device=q.device)
+                        if ctx.has_initial and ctx.needs_input_grad[5] else None)
+            rc = _lib.load().gsa_delta_rule_backward(
+                ctypes.byref(a), _ptr(do), _ptr(dfinal), ws.data_ptr(), ws.numel(),
+                scratch.data_ptr(), scratch.numel(), dq.data_ptr(), dk_.data_ptr(), dv.data_ptr(),
+                dg.data_ptr(), dbeta.data_ptr(), _ptr(dinitial),
+                torch.cuda.current_stream().cuda_stream)
+        _lib.check(rc, "gsa_delta_rule_backward")
+        return dq, dk_, dv, dg, dbeta, dinitial, None, None, None, None
+
+
+def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                     beta: torch.Tensor, scale: float | None = None,
+                     initial_state: torch.Tensor | None = None,
+                     cu_seqlens: torch.Tensor | None = None, output_final_state: bool = False):
+    """The gated delta rule over whole sequences, with gradients.
+
+    q, k [B, T, Hk, dk] and v [B, T, Hv, dv] (bf16 or fp32), Hv a multiple of Hk
+    (value head h reads key head h // (Hv // Hk)), dk <= 128 and dv <= 256,
+    multiples of 8; g (log decay, at most 0) and beta [B, T, Hv], both bf16 or
+    both fp32; scale defaults to dk ** -0.5.  ``initial_state`` [N, Hv, dk, dv]
+    fp32 (default zeros).  With ``cu_seqlens`` (int32 [N + 1] on the device, as
+    ``[0, n_0, n_0 + n_1, ...]``) B is 1 and the N sequences lie one behind the
+    other; rows of no sequence come out, and in the gradients, as zeros.
+
+    Returns (o [B, T, Hv, dv] in q's dtype, final state [N, Hv, dk, dv] fp32 or
+    None).  Differentiable once in q, k, v, g, beta and the initial state; the
+    gradients have the inputs' dtypes and add up in a fixed order.  States, decays
+    and sums are fp32; bf16 gradients are formed from factors rounded to bf16.
+    Keys are expected near unit length (``rms_norm`` with weight dk ** -0.5 makes
+    them), values finite."""
+    _check(q, k, v, g, beta, initial_state, cu_seqlens)
+    B, T, _, dk = q.shape
+    Hv, dv = v.shape[2], v.shape[3]
+    N = B
+    if cu_seqlens is not None:
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype not in (
+                torch.int32, torch.int64):
+            raise ValueError("cu_seqlens must be int32 or int64 [N + 1] with N >= 1")
+        if B != 1:
+            raise ValueError("cu_seqlens needs a batch of 1")
+        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+        N = cu_seqlens.numel() - 1
+    if initial_state is not None:
+        if initial_state.shape != (N, Hv, dk, dv) or initial_state.dtype != torch.float32:
+            raise ValueError(f"initial_state must be float32 [{N}, {Hv}, {dk}, {dv}]")
+        initial_state = initial_state.contiguous()
+    scale = dk ** -0.5 if scale is None else float(scale)
+    q, k, v, g, beta = _rows_ok(q), _rows_ok(k), _rows_ok(v), _gates_ok(g), _gates_ok(beta)
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
+        return _GatedDeltaRule.apply(q, k, v, g, beta, initial_state, cu_seqlens, scale, N,
+                                     output_final_state)
+    with torch.cuda.device(q.device):
+        return _forward(q, k, v, g, beta, initial_state, cu_seqlens, scale, N,
+                        output_final_state, _lib.GSA_DELTA_INFERENCE)[:2]
+
+
+def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,
+                     beta: torch.Tensor, state: torch.Tensor, scale: float | None = None,
+                     state_indices: torch.Tensor | None = None) -> torch.Tensor:
+    """One or a few tokens of each of B sequences, against states updated in place.
+
+    Inputs as ``gated_delta_rule`` with T the tokens of the step (usually 1).
+    ``state`` [slots, Hv, dk, dv] fp32, contiguous: sequence b has the slot
+    ``state_indices[b]`` (int32 [B] on the device; default b); -1 marks an empty
+    row of the batch, whose output is zero.  An index outside [-1, slots) or one
+    that an earlier row has already is refused on the device: that row comes out
+    as NaN, no state changes for it, and ``_lib.device_error()`` reports it.
+    Returns o [B, T, Hv, dv].  No gradients."""
+    _check(q, k, v, g, beta, state, state_indices)
+    B, T, _, dk = q.shape
+    Hv, dv = v.shape[2], v.shape[3]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
+        raise RuntimeError("gated_delta_step has no gradients; use gated_delta_rule")
+    if (state.dim() != 4 or state.shape[1:] != (Hv, dk, dv) or state.dtype != torch.float32
+            or not state.is_contiguous() or state.data_ptr() % 16):
+        raise ValueError(f"state must be contiguous float32 [slots, {Hv}, {dk}, {dv}], 16-byte "
+                         "aligned")
+    if state_indices is not None:
+        if state_indices.shape != (B,) or state_indices.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"state_indices must be int32 or int64 [{B}]")
+        state_indices = state_indices.to(torch.int32).contiguous()
+    elif state.shape[0] < B:
+        raise ValueError(f"{B} rows need as many states, got {state.shape[0]}")
+    scale = dk ** -0.5 if scale is None else float(scale)
+    q, k, v, g, beta = _rows_ok(q), _rows_ok(k), _rows_ok(v), _gates_ok(g), _gates_ok(beta)
+    with torch.cuda.device(q.device):
+        a = _args(q, k, v, g, beta, scale, B, None, None)
+        o = torch.empty(B, T, Hv, dv, dtype=q.dtype, device=q.device)
+        rc = _lib.load().gsa_delta_step(
+            ctypes.byref(a), state.data_ptr(), state.shape[0], _ptr(state_indices), o.data_ptr(),
+            torch.cuda.current_stream().cuda_stream)
+    _lib.check(rc, "gsa_delta_step")
+    return o

@@ -1,0 +1,163 @@
+"""Root-mean-square norm with the residual's addition, in the inputs' type (with
+gradients) or with an output in 8 bits.
+
+    h = x + residual              (rounded to the inputs' type; x without a residual)
+    y = h / sqrt(mean(h^2) + eps) * weight
+
+Both functions run on the tensors' device and its current stream; there is no
+CPU path.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _cuda, _dtype_code, _ptr
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """t as rows [R, D] with unit inner stride (a copy only where the layout needs one)."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _check(x, weight, residual) -> None:
+    _cuda(x, weight, residual)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must have a last dim of at least 1, got {tuple(x.shape)}")
+    _dtype_code(x), _dtype_code(weight)
+    if x.shape[-1] > 32768:
+        raise ValueError(f"rows of at most 32768 values, got {x.shape[-1]}")
+    if weight.shape != (x.shape[-1],):
+        raise ValueError(f"weight must be [{x.shape[-1]}], got {tuple(weight.shape)}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("residual must match x in shape and dtype")
+    if weight.device != x.device or (residual is not None and residual.device != x.device):
+        raise ValueError("all tensors must be on one device")
+
+
+def _forward(x, weight, residual, eps, want_rstd):
+    rows, width = x.shape
+    y = torch.empty(rows, width, dtype=x.dtype, device=x.device)
+    h = torch.empty_like(y) if residual is not None else None
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
+    with torch.cuda.device(x.device):
+        rc = _lib.load().gsa_rms_norm(
+            x.data_ptr(), _row_stride(x), _ptr(residual),
+            _row_stride(residual) if residual is not None else 0, weight.data_ptr(),
+            _dtype_code(weight), float(eps), _dtype_code(x), rows, width, y.data_ptr(), width,
+            _ptr(h), width, _ptr(rstd), torch.cuda.current_stream().cuda_stream)
+    _lib.check(rc, "gsa_rms_norm")
+    return y, h, rstd
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        x2, r2 = _flat(x), _flat(residual) if residual is not None else None
+        y, h, rstd = _forward(x2, weight, r2, eps, True)
+        y = y.view(x.shape)
+        if residual is None:
+            ctx.save_for_backward(x, weight, rstd)
+            ctx.set_materialize_grads(False)
+            return y
+        h = h.view(x.shape)
+        ctx.save_for_backward(h, weight, rstd)
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        if dy is None:  # only the sum h was used
+            return dh, None, dh, None
+        width = h.shape[-1]
+        h2, dy2 = _flat(h), _flat(dy.to(h.dtype))
+        dh2 = _flat(dh.to(h.dtype)) if dh is not None else None
+        rows = h2.shape[0]
+        dx = torch.empty(rows, width, dtype=h.dtype, device=h.device)
+        dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+        with torch.cuda.device(h.device):
+            lib = _lib.load()
+            need = int(lib.gsa_rms_norm_backward_workspace_size(rows, width)) if dw is not None \
+                else 0
+            ws = torch.empty(need, dtype=torch.uint8, device=h.device)
+            rc = lib.gsa_rms_norm_backward(
+                dy2.data_ptr(), _row_stride(dy2), _ptr(dh2),
+                _row_stride(dh2) if dh2 is not None else 0, h2.data_ptr(), _row_stride(h2),
+                weight.data_ptr(), _dtype_code(weight), rstd.data_ptr(), _dtype_code(h2), rows,
+                width, dx.data_ptr(), width, _ptr(dw), ws.data_ptr(), need,
+                torch.cuda.current_stream().cuda_stream)
+        _lib.check(rc, "gsa_rms_norm_backward")
+        dx = dx.view(h.shape)
+        return dx, dw, dx if ctx.needs_input_grad[2] else None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+             residual: torch.Tensor | None = None):
+    """RMS norm over the last dim (at most 32768 values), with an optional residual.
+
+    x [..., D] (bf16 or fp32), weight [D] (bf16 or fp32).  Returns y in x's dtype, or
+    (y, h) with ``residual`` (x's shape and dtype): h = x + residual rounded to
+    that dtype, which is what the norm reads and the next residual is.
+    Differentiable once in x, weight and the residual; the weight's gradient
+    adds the rows up in a fixed order."""
+    _check(x, weight, residual)
+    weight = weight.contiguous()
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, weight, residual)):
+        return _RmsNorm.apply(x, weight, residual, float(eps))
+    y, h, _ = _forward(_flat(x), weight, _flat(residual) if residual is not None else None, eps,
+                       False)
+    return y.view(x.shape) if h is None else (y.view(x.shape), h.view(x.shape))
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                 residual: torch.Tensor | None = None, group_size: int | None = None):
+    """``rms_norm`` with its output in 8 bits (torch.float8_e4m3fn) and fp32 scales.
+
+    y8 * scale stands for the norm's values: the scale is the largest magnitude
+    of a row, or of each ``group_size`` = 128 values of it (D a multiple of 128),
+    over 448, the type's largest number; the values are rounded once, from fp32.
+    Returns (y8 [..., D], scale [..., 1] or [..., D / 128]) and, with a residual, h.
+    No gradients."""
+    _check(x, weight, residual)
+    if group_size not in (None, 128):
+        raise ValueError(f"group_size must be None or 128, got {group_size}")
+    width = x.shape[-1]
+    if group_size and width % 128:
+        raise ValueError(f"group scales need a last dim that is a multiple of 128, got {width}")
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, weight, residual)):
+        raise RuntimeError("rms_norm_fp8 has no gradients; use rms_norm")
+
+    def usable(t):
+        """Group scales move 16 bytes at a time: rows that are not on 16 bytes are copied."""
+        es = t.element_size()
+        if group_size and (t.data_ptr() % 16 or _row_stride(t) * es % 16):
+            return t.clone(memory_format=torch.contiguous_format)
+        return t
+
+    x2, r2 = usable(_flat(x)), usable(_flat(residual)) if residual is not None else None
+    weight = weight.contiguous()
+    if group_size and weight.data_ptr() % 16:
+        weight = weight.clone()
+    rows, groups = x2.shape[0], width // group_size if group_size else 1
+    y = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(rows, groups, dtype=torch.float32, device=x.device)
+    h = torch.empty(rows, width, dtype=x.dtype, device=x.device) if r2 is not None else None
+    with torch.cuda.device(x.device):
+        rc = _lib.load().gsa_rms_norm_fp8(
+            x2.data_ptr(), _row_stride(x2), _ptr(r2), _row_stride(r2) if r2 is not None else 0,
+            weight.data_ptr(), _dtype_code(weight), float(eps), _dtype_code(x2), rows, width,
+            y.data_ptr(), width, scale.data_ptr(), group_size or 0, _ptr(h), width,
+            torch.cuda.current_stream().cuda_stream)
+    _lib.check(rc, "gsa_rms_norm_fp8")
+    y, scale = y.view(x.shape), scale.view(x.shape[:-1] + (groups,))
+    return (y, scale) if h is None else (y, scale, h.view(x.shape))

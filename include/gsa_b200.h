@@ -404,6 +404,127 @@ GSA_API int gsa_fused_projection_pack(const void* w_q, const void* w_k,
                          int D, int H_I, int d_I,
                          void* w_packed, float* b_packed, void* stream);
 
+/*
+ * The gated delta rule, the token mixer of the gated-delta layers that the
+ * benchmark study sets beside gated sparse attention.  Per sequence and value
+ * head, with a state S [dk, dv]:
+ *   S_t = e^{g_t} S_{t-1} + k_t u_t^T
+ *   u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t)
+ *   o_t = scale S_t^T q_t
+ * Value head h reads key head h / (Hv / Hk).  g is the logarithm of the decay
+ * (at most 0; -inf wipes the state); keys are expected near unit length.
+ * q, k, v must be finite up to the end of a sequence: a value that is not makes
+ * the outputs of its 64-token chunk and of what follows it unspecified.
+ *
+ *   q, k [B, T, Hk, dk], v [B, T, Hv, dv] (dtype), unit inner stride;
+ *   g, beta [B, T, Hv] (gate_dtype), unit inner stride;
+ *   strides in elements: {batch, token, head}, for the gates {batch, token}.
+ *   dk, dv multiples of 8, dk <= 128, dv <= 256; Hv a multiple of Hk.
+ *   N sequences.  Without cu_seqlens N == B and every sequence has T tokens.
+ *   With cu_seqlens (int32 [N + 1] on the device) B == 1, and sequence n is the
+ *   rows [cu_seqlens[n], cu_seqlens[n + 1]); rows of no sequence get zeros.
+ *   Sequences that overlap or leave [0, T] are cut to their order and to T,
+ *   and the device error word (gsa_device_error) is set.
+ *   initial_state float32 [N, Hv, dk, dv] contiguous, or NULL for zeros.
+ * bf16: tensor cores with 16-bit pairs for the state, so the state keeps
+ * about fp32's accuracy; 16-byte aligned rows.  f32: CUDA cores.
+ */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* g;
+  const void* beta;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t g_stride[2];
+  int64_t beta_stride[2];
+  const int32_t* cu_seqlens;
+  const float* initial_state;
+  int dtype;
+  int gate_dtype;
+  float scale;
+  int B, T, Hk, Hv, dk, dv, N;
+} gsa_delta_t;
+
+/* What a workspace is for. */
+typedef enum {
+  GSA_DELTA_INFERENCE = 0, /* gsa_delta_rule_forward, nothing kept */
+  GSA_DELTA_TRAINING = 1,  /* gsa_delta_rule_forward, kept for the backward */
+  GSA_DELTA_BACKWARD = 2   /* gsa_delta_rule_backward's own scratch */
+} gsa_delta_use_t;
+
+/* Bytes of caller-owned workspace (256-byte aligned); -1 for arguments that
+ * the calls would refuse.  Only sizes, types and whether cu_seqlens is NULL
+ * matter. */
+GSA_API int64_t gsa_delta_rule_workspace_size(const gsa_delta_t* p, int use);
+
+/* o [B, T, Hv, dv] contiguous (dtype); final_state float32 [N, Hv, dk, dv] or
+ * NULL.  use: GSA_DELTA_INFERENCE or GSA_DELTA_TRAINING. */
+GSA_API int gsa_delta_rule_forward(const gsa_delta_t* p, void* o, float* final_state,
+                                   int use, void* workspace, int64_t workspace_bytes,
+                                   void* stream);
+
+/* Gradients, from the workspace that a GSA_DELTA_TRAINING forward of the same
+ * arguments filled.  dout [B, T, Hv, dv] contiguous (dtype) and dfinal
+ * [N, Hv, dk, dv] may each be NULL (zero).  dq, dk [B, T, Hk, dk], dv
+ * [B, T, Hv, dv] (dtype), dg, dbeta [B, T, Hv] (gate_dtype), dinitial
+ * [N, Hv, dk, dv] float32 (may be NULL): contiguous. */
+GSA_API int gsa_delta_rule_backward(const gsa_delta_t* p, const void* dout,
+                                    const float* dfinal, const void* saved,
+                                    int64_t saved_bytes, void* scratch,
+                                    int64_t scratch_bytes, void* dq, void* dk, void* dv,
+                                    void* dg, void* dbeta, float* dinitial, void* stream);
+
+/* The same rule for T (usually 1) tokens of each of B sequences, decoding:
+ * sequence b's state is slot indices[b] (slot b with indices NULL) of `state`,
+ * float32 [slots, Hv, dk, dv] contiguous, updated in place.  indices[b] == -1
+ * is an empty row: its o is zero.  An index outside [-1, slots), or one that an
+ * earlier row of the call has, is refused on the device: its o is NaN, no state
+ * changes, and the device error word is set.  initial_state, cu_seqlens and N
+ * of *p are not used.  o [B, T, Hv, dv] contiguous (dtype). */
+GSA_API int gsa_delta_step(const gsa_delta_t* p, float* state, int64_t slots,
+                           const int32_t* indices, void* o, void* stream);
+
+/*
+ * Root-mean-square norm with the residual's addition:
+ *   h = dtype(x + residual)   (h = x where residual is NULL)
+ *   y = dtype(h * weight / sqrt(mean(h^2) + eps))
+ * Rows of `width` values (1 .. 32768), unit inner stride, row strides in
+ * elements.  weight [width] in weight_dtype.  h and rstd (float32 [rows], the
+ * reciprocal root, kept for the backward) may be NULL; h is written only with a
+ * residual, which then needs it.  Sums are float32.
+ */
+GSA_API int gsa_rms_norm(const void* x, int64_t x_stride, const void* residual,
+                         int64_t residual_stride, const void* weight, int weight_dtype,
+                         float eps, int dtype, int64_t rows, int width, void* y,
+                         int64_t y_stride, void* h, int64_t h_stride, float* rstd,
+                         void* stream);
+
+/* The same with y in 8 bits (e4m3): y = e4m3(f * (448 / m)), scale = m / 448,
+ * f the fp32 value above and m = max(|f|, 1e-12) over the row (group 0: scale
+ * [rows]) or over each 128 values (group 128: scale [rows, width / 128], width
+ * a multiple of 128 and rows 16-byte aligned). */
+GSA_API int gsa_rms_norm_fp8(const void* x, int64_t x_stride, const void* residual,
+                             int64_t residual_stride, const void* weight, int weight_dtype,
+                             float eps, int dtype, int64_t rows, int width, void* y,
+                             int64_t y_stride, float* scale, int group, void* h,
+                             int64_t h_stride, void* stream);
+
+/* Bytes of workspace that gsa_rms_norm_backward needs for dweight. */
+GSA_API int64_t gsa_rms_norm_backward_workspace_size(int64_t rows, int width);
+
+/* dx (also the residual's gradient) and dweight (weight_dtype; may be NULL) from
+ * dy, dh (the gradient of h; may be NULL), h and rstd.  dweight sums the rows
+ * in a fixed order, in float32. */
+GSA_API int gsa_rms_norm_backward(const void* dy, int64_t dy_stride, const void* dh,
+                                  int64_t dh_stride, const void* h, int64_t h_stride,
+                                  const void* weight, int weight_dtype, const float* rstd,
+                                  int dtype, int64_t rows, int width, void* dx,
+                                  int64_t dx_stride, void* dweight, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
