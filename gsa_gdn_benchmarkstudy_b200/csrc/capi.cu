@@ -965,9 +965,14 @@ int check_delta_rule(const gsa_delta_t* p) {
 int64_t gsa_delta_rule_workspace_size(const gsa_delta_t* p, int use) {
   if (check_delta_rule(p)) return -1;
   switch (use) {
-    case GSA_DELTA_INFERENCE: return gsa::delta::simt_saved_bytes(*p, false);
-    case GSA_DELTA_TRAINING: return gsa::delta::simt_saved_bytes(*p, true);
-    case GSA_DELTA_BACKWARD: return gsa::delta::simt_scratch_bytes(*p);
+    case GSA_DELTA_INFERENCE:
+    case GSA_DELTA_TRAINING:
+      return p->dtype == GSA_DTYPE_BF16
+                 ? gsa::delta::mma_saved_bytes(*p, use == GSA_DELTA_TRAINING)
+                 : gsa::delta::simt_saved_bytes(*p, use == GSA_DELTA_TRAINING);
+    case GSA_DELTA_BACKWARD:
+      return p->dtype == GSA_DTYPE_BF16 ? gsa::delta::mma_scratch_bytes(*p)
+                                        : gsa::delta::simt_scratch_bytes(*p);
     default: set_error(GSA_ERR_INVALID_ARG, "unknown use"); return -1;
   }
 }
@@ -993,7 +998,10 @@ int gsa_delta_rule_forward(const gsa_delta_t* p, void* o, float* final_state, in
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = gsa::delta::launch_table(*p, workspace, st->err, s);
   if (e == cudaSuccess)
-    e = gsa::delta::simt_forward(*p, o, final_state, use == GSA_DELTA_TRAINING, workspace, s);
+    e = p->dtype == GSA_DTYPE_BF16
+            ? gsa::delta::mma_forward(*p, o, final_state, use == GSA_DELTA_TRAINING, workspace,
+                                      st->err, s)
+            : gsa::delta::simt_forward(*p, o, final_state, use == GSA_DELTA_TRAINING, workspace, s);
   return finish(e);
 }
 
@@ -1022,8 +1030,11 @@ int gsa_delta_rule_backward(const gsa_delta_t* p, const void* dout, const float*
   DeviceState* st = nullptr;
   if ((rc = device_state(&st))) return rc;
   const gsa::DeltaGrads g = {dout, dfinal, dq, dk, dv, dg, dbeta, dinitial};
-  return finish(gsa::delta::simt_backward(*p, g, const_cast<void*>(saved), scratch,
-                                          static_cast<cudaStream_t>(stream)));
+  void* kept = const_cast<void*>(saved);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return finish(p->dtype == GSA_DTYPE_BF16
+                    ? gsa::delta::mma_backward(*p, g, kept, scratch, st->err, s)
+                    : gsa::delta::simt_backward(*p, g, kept, scratch, s));
 }
 
 int gsa_delta_step(const gsa_delta_t* p, float* state, int64_t slots, const int32_t* indices,

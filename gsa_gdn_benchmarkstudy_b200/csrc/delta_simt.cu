@@ -627,13 +627,11 @@ int64_t simt_scratch_bytes(const gsa_delta_t& p) {
 
 cudaError_t simt_forward(const gsa_delta_t& p, void* o, float* final_state, bool save, void* ws,
                          cudaStream_t stream) {
-  return p.dtype == GSA_DTYPE_BF16 ? forward<__nv_bfloat16>(p, o, final_state, save, ws, stream)
-                                   : forward<float>(p, o, final_state, save, ws, stream);
+  return forward<float>(p, o, final_state, save, ws, stream);
 }
 cudaError_t simt_backward(const gsa_delta_t& p, const DeltaGrads& g, void* saved, void* scratch,
                           cudaStream_t stream) {
-  return p.dtype == GSA_DTYPE_BF16 ? backward<__nv_bfloat16>(p, g, saved, scratch, stream)
-                                   : backward<float>(p, g, saved, scratch, stream);
+  return backward<float>(p, g, saved, scratch, stream);
 }
 
 }  // namespace delta

@@ -258,6 +258,13 @@ cudaError_t simt_forward(const gsa_delta_t& p, void* o, float* final_state, bool
                          cudaStream_t stream);
 cudaError_t simt_backward(const gsa_delta_t& p, const DeltaGrads& g, void* saved, void* scratch,
                           cudaStream_t stream);
+// bf16 inputs.
+int64_t mma_saved_bytes(const gsa_delta_t& p, bool save);
+int64_t mma_scratch_bytes(const gsa_delta_t& p);
+cudaError_t mma_forward(const gsa_delta_t& p, void* o, float* final_state, bool save, void* ws,
+                        int* err, cudaStream_t stream);
+cudaError_t mma_backward(const gsa_delta_t& p, const DeltaGrads& g, void* saved, void* scratch,
+                         int* err, cudaStream_t stream);
 }  // namespace delta
 
 cudaError_t launch_gather_attention(const void* q, int64_t q_stride, const void* k,
