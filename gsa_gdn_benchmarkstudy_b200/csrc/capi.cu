@@ -929,8 +929,14 @@ int check_delta(const gsa_delta_t* p) {
   return GSA_OK;
 }
 
-bool delta_rows_aligned(const void* q, const int64_t* stride) {
-  return aligned16(q) && stride[0] % 8 == 0 && stride[1] % 8 == 0 && stride[2] % 8 == 0;
+// Whether TMA can read [B, T, heads, channels] rows: base and strides on 16
+// bytes, strides positive (that of a dimension of one element does not matter).
+bool delta_rows_ok(const void* q, const int64_t* stride, const gsa_delta_t& p, int heads) {
+  const int64_t size[3] = {p.B, p.T, heads};
+  for (int i = 0; i < 3; ++i)
+    if (size[i] > 1 && (stride[i] <= 0 || stride[i] % 8 || stride[i] >= (int64_t{1} << 39)))
+      return false;
+  return aligned16(q);
 }
 
 int check_delta_inputs(const gsa_delta_t* p) {
@@ -938,10 +944,49 @@ int check_delta_inputs(const gsa_delta_t* p) {
   if (!p->q || !p->k || !p->v || !p->g || !p->beta)
     return set_error(GSA_ERR_INVALID_ARG, "q / k / v / g / beta is NULL");
   if (p->dtype == GSA_DTYPE_BF16 &&
-      !(delta_rows_aligned(p->q, p->q_stride) && delta_rows_aligned(p->k, p->k_stride) &&
-        delta_rows_aligned(p->v, p->v_stride)))
-    return set_error(GSA_ERR_ALIGNMENT, "bf16 q, k, v rows must be 16-byte aligned");
+      !(delta_rows_ok(p->q, p->q_stride, *p, p->Hk) && delta_rows_ok(p->k, p->k_stride, *p, p->Hk) &&
+        delta_rows_ok(p->v, p->v_stride, *p, p->Hv)))
+    return set_error(GSA_ERR_ALIGNMENT,
+                     "bf16 q, k, v rows must be 16-byte aligned, their strides positive");
   return GSA_OK;
+}
+
+// Map over [batch][token][head][channel] rows of bf16 with strides in elements
+// (that of a dimension of one element does not matter); zero fill out of bounds.
+int make_map_delta(CUtensorMap* map, const void* base, const gsa_delta_t& p, int width, int heads,
+                   const int64_t* stride, bool swizzled) {
+  PFN_encodeTiled_t fn = encode_fn();
+  if (!fn) return set_error(GSA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(p.T), static_cast<cuuint64_t>(p.B)};
+  const int64_t steps[3] = {stride[2], stride[1], stride[0]};  // head, token, batch
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i)
+    strides[i] = dims[i + 1] > 1 ? static_cast<cuuint64_t>(steps[i]) * 2
+                                 : static_cast<cuuint64_t>(width) * 2;
+  const cuuint32_t box[4] = {swizzled ? 64u : 16u, 1, 64, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+         CU_TENSOR_MAP_INTERLEAVE_NONE,
+         swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    std::snprintf(g_last_error, sizeof(g_last_error), "cuTensorMapEncodeTiled failed (%d)",
+                  static_cast<int>(r));
+    return GSA_ERR_CUDA;
+  }
+  return GSA_OK;
+}
+
+// The maps of the bf16 kernels; `values` [B, T, Hv, dv] may be NULL.
+int make_delta_maps(gsa::delta::DeltaMaps* m, const gsa_delta_t& p, const void* values,
+                    const int64_t* stride) {
+  if (p.T == 0) return GSA_OK;
+  int rc = make_map_delta(&m->q, p.q, p, p.dk, p.Hk, p.q_stride, true);
+  if (!rc) rc = make_map_delta(&m->k, p.k, p, p.dk, p.Hk, p.k_stride, true);
+  if (!rc && values) rc = make_map_delta(&m->v, values, p, p.dv, p.Hv, stride, false);
+  return rc;
 }
 
 // What holds for whole sequences on top of check_delta.
@@ -996,10 +1041,13 @@ int gsa_delta_rule_forward(const gsa_delta_t* p, void* o, float* final_state, in
   DeviceState* st = nullptr;
   if ((rc = device_state(&st))) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf16 = p->dtype == GSA_DTYPE_BF16;
+  gsa::delta::DeltaMaps maps = {};
+  if (bf16 && (rc = make_delta_maps(&maps, *p, p->v, p->v_stride))) return rc;
   cudaError_t e = gsa::delta::launch_table(*p, workspace, st->err, s);
   if (e == cudaSuccess)
-    e = p->dtype == GSA_DTYPE_BF16
-            ? gsa::delta::mma_forward(*p, o, final_state, use == GSA_DELTA_TRAINING, workspace,
+    e = bf16
+            ? gsa::delta::mma_forward(*p, maps, o, final_state, use == GSA_DELTA_TRAINING, workspace,
                                       st->err, s)
             : gsa::delta::simt_forward(*p, o, final_state, use == GSA_DELTA_TRAINING, workspace, s);
   return finish(e);
@@ -1032,8 +1080,13 @@ int gsa_delta_rule_backward(const gsa_delta_t* p, const void* dout, const float*
   const gsa::DeltaGrads g = {dout, dfinal, dq, dk, dv, dg, dbeta, dinitial};
   void* kept = const_cast<void*>(saved);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return finish(p->dtype == GSA_DTYPE_BF16
-                    ? gsa::delta::mma_backward(*p, g, kept, scratch, st->err, s)
+  const bool bf16 = p->dtype == GSA_DTYPE_BF16;
+  gsa::delta::DeltaMaps maps = {};
+  const int64_t step = static_cast<int64_t>(p->Hv) * p->dv;
+  const int64_t stride[3] = {step * p->T, step, p->dv};
+  if (bf16 && (rc = make_delta_maps(&maps, *p, dout, stride))) return rc;
+  return finish(bf16
+                    ? gsa::delta::mma_backward(*p, maps, g, kept, scratch, st->err, s)
                     : gsa::delta::simt_backward(*p, g, kept, scratch, s));
 }
 

@@ -7,8 +7,9 @@
 // `chain`  one warp a sequence, value head and 16 columns of the state: S^T
 //          [16, dk] stays in the warp's accumulators over the whole sequence.
 //          Every product has S^T, Y^T or N^T on its left, whose accumulator
-//          layout is the left operand's layout of mma.sync, so nothing of the
-//          sequential path goes through shared memory or meets another warp.
+//          layout is the left operand's layout of mma.sync, so the sequential
+//          path stays in registers.  What is not on that path (the outputs, or
+//          backwards dO's own terms) is a second warp's, beside it.
 // `rev`    the same backwards, with the state's gradient.
 // `grad`   one block a chunk and key head: the gradients that contract over dv.
 //
@@ -33,14 +34,12 @@ namespace {
 __device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void stsm(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                      uint32_t d) {
@@ -56,7 +55,7 @@ __device__ __forceinline__ void stsm_t(uint32_t addr, uint32_t a, uint32_t b, ui
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                     uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -113,15 +112,21 @@ __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
 }
 
 // ---------------------------------------------------------------- workspace
-// For each chunk and value head: T and P as pairs, and three rows of decays.
+// For each chunk and value head, T and P as pairs of swizzled tiles with the
+// decays that go with them: the first half is the sequential warp's, the second
+// the other's.
 struct __align__(16) Block {
-  unsigned char t_hi[kTile], t_lo[kTile], p_hi[kTile], p_lo[kTile];
+  unsigned char t_hi[kTile], t_lo[kTile];
   float grown[kChunk];  // e^{c_i}
   float beta[kChunk];
   float left[kChunk];   // e^{c_64 - c_i}
-  float pad[kChunk];
+  float pad0[kChunk];
+  unsigned char p_hi[kTile], p_lo[kTile];
+  float grown_p[kChunk];
+  float pad1[3 * kChunk];
 };
-static_assert(sizeof(Block) == 4 * kTile + 1024, "block");
+constexpr int kHalf = 2 * static_cast<int>(kTile) + 1024;
+static_assert(sizeof(Block) == 2 * kHalf, "block");
 
 __host__ __device__ inline int blocks16(int dv) { return (dv + 15) / 16; }
 __host__ __device__ inline int padded_dk(int dk) { return dk <= 64 ? 64 : 128; }
@@ -177,13 +182,97 @@ __device__ __forceinline__ void copy_rows(uint32_t dst, const bf16* src, int64_t
 // ---------------------------------------------------------------- prep
 constexpr int kPrepThreads = 128;
 constexpr int kLdL = kChunk + 4;
+constexpr int kLdX = 36;
+
+// K and Q, whose place the block's image takes once their products are in
+// registers; L, which becomes T in place; a 32 x 32 product.
+template <int DK>
+constexpr int prep_smem() {
+  return (2 * (DK / 64) * static_cast<int>(kTile) > static_cast<int>(sizeof(Block))
+              ? 2 * (DK / 64) * static_cast<int>(kTile)
+              : static_cast<int>(sizeof(Block))) +
+         (kChunk * kLdL + 32 * kLdX) * 4 + 1024;
+}
+
+// out[r][c] = sign sum_k a[r][k] b[k][c] for a 32 x 32 block, 2 x 4 a thread.
+__device__ __forceinline__ void block32(const float* a, int lda, const float* b, int ldb,
+                                        float* out, int ldo, float sign) {
+  const int r = (threadIdx.x >> 3) * 2, c = (threadIdx.x & 7) * 4;
+  float x[2][4] = {};
+#pragma unroll 8
+  for (int k = 0; k < 32; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(b + k * ldb + c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float u = a[(r + i) * lda + k];
+      x[i][0] = fmaf(u, v.x, x[i][0]);
+      x[i][1] = fmaf(u, v.y, x[i][1]);
+      x[i][2] = fmaf(u, v.z, x[i][2]);
+      x[i][3] = fmaf(u, v.w, x[i][3]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    *reinterpret_cast<float4*>(out + (r + i) * ldo + c) =
+        make_float4(sign * x[i][0], sign * x[i][1], sign * x[i][2], sign * x[i][3]);
+}
+// The same for the two 16 x 16 blocks of a level, 64 threads and 1 x 4 each.
+__device__ __forceinline__ void block16(const float* a, int lda, const float* b, int ldb,
+                                        float* out, int ldo, float sign) {
+  const int t = threadIdx.x & 63, r = t >> 2, c = (t & 3) * 4;
+  float x[4] = {};
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(b + k * ldb + c);
+    const float u = a[r * lda + k];
+    x[0] = fmaf(u, v.x, x[0]);
+    x[1] = fmaf(u, v.y, x[1]);
+    x[2] = fmaf(u, v.z, x[2]);
+    x[3] = fmaf(u, v.w, x[3]);
+  }
+  *reinterpret_cast<float4*>(out + r * ldo + c) =
+      make_float4(sign * x[0], sign * x[1], sign * x[2], sign * x[3]);
+}
+
+// L (strictly lower, 64 x 64) becomes T = (I + L)^-1 in place, in fp32: the four
+// 16 x 16 diagonal blocks by substitution, then T21 = -T22 L21 T11 twice over.
+// A column a thread over all 64 rows took 2.5 times as long: half the threads
+// idle, 64 values of a column in registers.
+__device__ __forceinline__ void invert(float* L, float* X) {
+  const int tid = threadIdx.x;
+  {
+    const int b = (tid & 63) >> 4, j = tid & 15;
+    float* D = L + 16 * b * kLdL + 16 * b;
+    float col[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == j ? 1.f : 0.f;
+#pragma unroll
+      for (int m = 0; m < i; ++m) s = fmaf(-D[i * kLdL + m], col[m], s);
+      col[i] = s;
+    }
+    __syncthreads();
+    if (tid < 64)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) D[i * kLdL + j] = col[i];
+  }
+  __syncthreads();
+  const int b = (tid >> 6) * 32;
+  float* D = L + b * kLdL + b;
+  float* Y = X + (tid >> 6) * 16 * kLdX;
+  block16(D + 16 * kLdL, kLdL, D, kLdL, Y, kLdX, 1.f);
+  __syncthreads();
+  block16(D + 16 * kLdL + 16, kLdL, Y, kLdX, D + 16 * kLdL, kLdL, -1.f);
+  __syncthreads();
+  block32(L + 32 * kLdL, kLdL, L, kLdL, X, kLdX, 1.f);
+  __syncthreads();
+  block32(L + 32 * kLdL + 32, kLdL, X, kLdX, L + 32 * kLdL, kLdL, -1.f);
+  __syncthreads();
+}
 
 template <int DK>
-constexpr int prep_smem() { return 2 * (DK / 64) * kTile + kChunk * kLdL * 4 + 1024; }
-
-template <int DK>
-__global__ void __launch_bounds__(kPrepThreads) prep_kernel(const gsa_delta_t p, Table table,
-                                                            Block* blocks) {
+__global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t p, Table table,
+                                                               Block* blocks) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~1023ull);
@@ -193,12 +282,15 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const gsa_delta_t p,
   const Chunk c = chunk_at(p, table, blockIdx.x);
   if (!c.valid || c.gap) return;
   const uint32_t K = smem_u32(smem), Q = K + (DK / 64) * kTile;
-  float* L = reinterpret_cast<float*>(smem + 2 * (DK / 64) * kTile);
+  Block* img = reinterpret_cast<Block*>(smem);
+  float* L = reinterpret_cast<float*>(smem + prep_smem<DK>() - 1024) - kChunk * kLdL - 32 * kLdX;
+  float* X = L + kChunk * kLdL;
   copy_rows(K, rows_at(p.k, p.k_stride, c.b, c.begin, hk), p.k_stride[1], c.len, DK, p.dk, tid,
             kPrepThreads);
   copy_rows(Q, rows_at(p.q, p.q_stride, c.b, c.begin, hk), p.q_stride[1], c.len, DK, p.dk, tid,
             kPrepThreads);
   asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+  if (tid < 32) chunk_decays(p, c, hk * group, d);
   __syncthreads();
   float kk[8][4] = {}, qk[8][4] = {};
 #pragma unroll
@@ -217,76 +309,81 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(const gsa_delta_t p,
     }
   }
   for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
-    __syncthreads();  // d and L are the last head's until here
-    if (tid < 32) chunk_decays(p, c, hv, d);
-    __syncthreads();
-    Block* blk = blocks + static_cast<int64_t>(blockIdx.x) * p.Hv + hv;
+    __syncthreads();  // K and Q, or the last head's image, are read
+    if (hv > hk * group) {
+      if (tid < 32) chunk_decays(p, c, hv, d);
+      __syncthreads();
+    }
     if (tid < kChunk) {
-      blk->grown[tid] = decay_from_start(d, tid);
-      blk->beta[tid] = d.beta[tid];
-      blk->left[tid] = decay_between(d, kChunk - 1, tid);
+      img->grown[tid] = img->grown_p[tid] = decay_from_start(d, tid);
+      img->beta[tid] = d.beta[tid];
+      img->left[tid] = decay_between(d, kChunk - 1, tid);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = m0 + gid + 8 * e, cc = 8 * j + 2 * tig;
-        float l[2], x[2];
+        float l[2] = {0.f, 0.f}, x[2] = {0.f, 0.f};
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const float w = r >= cc + f ? decay_between(d, r, cc + f) : 0.f;
-          l[f] = r > cc + f ? d.beta[r] * w * kk[j][2 * e + f] : 0.f;
-          x[f] = p.scale * w * qk[j][2 * e + f];
-          if (r < cc + f) x[f] = 0.f;
-        }
+        for (int f = 0; f < 2; ++f)
+          if (r >= cc + f) {
+            const float w = decay_between(d, r, cc + f);
+            if (r > cc + f) l[f] = d.beta[r] * w * kk[j][2 * e + f];
+            x[f] = p.scale * w * qk[j][2 * e + f];
+          }
         *reinterpret_cast<float2*>(L + r * kLdL + cc) = make_float2(l[0], l[1]);
         uint32_t hi, lo;
         split(x[0], x[1], hi, lo);
         const uint32_t at = sw128_offset(r, j) + 4 * tig;
-        *reinterpret_cast<uint32_t*>(blk->p_hi + at) = hi;
-        *reinterpret_cast<uint32_t*>(blk->p_lo + at) = lo;
+        *reinterpret_cast<uint32_t*>(img->p_hi + at) = hi;
+        *reinterpret_cast<uint32_t*>(img->p_lo + at) = lo;
       }
     __syncthreads();
-    // forward substitution, a column of T a thread
-    if (tid < kChunk) {
-      float col[kChunk];
+    invert(L, X);
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) {
-        float s[4] = {i == tid ? 1.f : 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int m = 0; m < i; m += 4) {
-          const float4 l = *reinterpret_cast<const float4*>(L + i * kLdL + m);
-          s[0] = fmaf(-l.x, col[m], s[0]);
-          if (m + 1 < i) s[1] = fmaf(-l.y, col[m + 1], s[1]);
-          if (m + 2 < i) s[2] = fmaf(-l.z, col[m + 2], s[2]);
-          if (m + 3 < i) s[3] = fmaf(-l.w, col[m + 3], s[3]);
-        }
-        col[i] = (s[0] + s[1]) + (s[2] + s[3]);
-        const __nv_bfloat16 hi = __float2bfloat16_rn(col[i]);
-        const uint32_t at = sw128_offset(i, tid >> 3) + 2 * (tid & 7);
-        *reinterpret_cast<__nv_bfloat16*>(blk->t_hi + at) = hi;
-        *reinterpret_cast<__nv_bfloat16*>(blk->t_lo + at) =
-            __float2bfloat16_rn(col[i] - __bfloat162float(hi));
-      }
+    for (int i = 0; i < kChunk * 8 / kPrepThreads; ++i) {
+      const int x = tid + i * kPrepThreads, r = x >> 3, piece = x & 7;
+      const float4 u = *reinterpret_cast<const float4*>(L + r * kLdL + piece * 8);
+      const float4 v = *reinterpret_cast<const float4*>(L + r * kLdL + piece * 8 + 4);
+      uint4 hi, lo;
+      split(u.x, u.y, hi.x, lo.x);
+      split(u.z, u.w, hi.y, lo.y);
+      split(v.x, v.y, hi.z, lo.z);
+      split(v.z, v.w, hi.w, lo.w);
+      *reinterpret_cast<uint4*>(img->t_hi + sw128_offset(r, piece)) = hi;
+      *reinterpret_cast<uint4*>(img->t_lo + sw128_offset(r, piece)) = lo;
     }
+    __syncthreads();
+    uint4* dst = reinterpret_cast<uint4*>(blocks + static_cast<int64_t>(blockIdx.x) * p.Hv + hv);
+    const uint4* src = reinterpret_cast<const uint4*>(img);
+    for (int i = tid; i < static_cast<int>(sizeof(Block) / 16); i += kPrepThreads) dst[i] = src[i];
   }
 }
 
 // ---------------------------------------------------------------- chain and rev
-// Shared memory of a block of W warps: kStages stages of K, Q, the T / P block
-// and 64 x 16 values (v or dO) for each warp, then a staging area a warp.
+// A block has W pairs of warps and one warp that copies.  Of a pair, the first
+// warp walks the state, the second has what is off that path.  Two queues of
+// kStages stages: A for the first warps (K, T and decays), B for the second (Q, P
+// and decays); 64 x 16 values for each pair go with A (v) or with B (dO).
 constexpr int kStages = 2;
 template <int DK>
-constexpr int tile_bytes() { return (DK / 64) * static_cast<int>(kTile); }
+__host__ __device__ constexpr int tile_bytes() { return (DK / 64) * static_cast<int>(kTile); }
 template <int DK>
-__host__ __device__ constexpr int stage_bytes(int W) {
-  return 2 * (DK / 64) * static_cast<int>(kTile) + static_cast<int>(sizeof(Block)) + W * 2048;
-}
+__host__ __device__ constexpr int queue_bytes() { return tile_bytes<DK>() + kHalf; }
+// What a pair shares: S^T and N^T as operands (forwards), or the second warp's
+// part of dN^T and of dS^T (backwards); and the second (backwards: first) warp's
+// staging area for rows that leave.
+template <int DK>
+__host__ __device__ constexpr int state_share() { return DK * 64; }
+template <int DK>
+__host__ __device__ constexpr int pair_bytes() { return state_share<DK>() + 4096; }
 template <int DK>
 __host__ __device__ constexpr int staging_bytes() { return 16 * (DK * 2 + 16); }
 template <int DK>
-constexpr int seq_smem(int W) {
-  return kStages * stage_bytes<DK>(W) + W * staging_bytes<DK>() + 1024;
+__host__ __device__ constexpr int seq_smem(int W) {
+  return kStages * (2 * queue_bytes<DK>() + W * 2048) +
+         W * (pair_bytes<DK>() + staging_bytes<DK>()) + 1024;
 }
 
 struct SeqArgs {
@@ -303,55 +400,103 @@ struct SeqArgs {
   int* err;
 };
 
-// The copies of a sequence's chunks, by one warp.
+struct SeqBars {
+  uint64_t full_a[kStages], empty_a[kStages], full_b[kStages], empty_b[kStages];
+  uint64_t s_full[8], s_free[8], n_full[8], n_free[8];  // by pair
+  int abort;
+};
+
+template <int DK>
+struct SeqSmem {
+  unsigned char* base;
+  int W;
+  __device__ unsigned char* a(int st) const { return base + st * queue_bytes<DK>(); }
+  __device__ unsigned char* b(int st) const { return base + (kStages + st) * queue_bytes<DK>(); }
+  __device__ unsigned char* v(int st, int pair) const {
+    return base + 2 * kStages * queue_bytes<DK>() + (st * W + pair) * 2048;
+  }
+  __device__ unsigned char* pair(int i) const {
+    return v(kStages, 0) + i * (pair_bytes<DK>() + staging_bytes<DK>());
+  }
+};
+
+__device__ __forceinline__ void tma_load_rows(void* dst, const CUtensorMap* map, int x, int h,
+                                              int t, int b, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(t), "r"(b), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// The copies of a sequence's chunks, by one warp.  Rows past the tensor's end
+// come out of TMA as zeros; a chunk that ends before its 64th row inside a packed
+// batch, where another sequence follows, takes its rows one by one.
 template <int DK, bool REV>
-__device__ __forceinline__ void produce(const gsa_delta_t& p, const SeqArgs& a, const Seq& s,
-                                        int hv, int col0, int W, unsigned char* smem,
-                                        uint64_t* full, uint64_t* empty, volatile int* abort) {
+__device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& maps,
+                                        const SeqArgs& a, const Seq& s, int hv, int col0, int W,
+                                        const SeqSmem<DK>& sm, SeqBars& bars) {
   const int lane = threadIdx.x & 31, hk = hv / (p.Hv / p.Hk);
   const int chunks = (s.len + kChunk - 1) / kChunk;
   const bool have = !REV || a.in != nullptr;
-  int n = 0;
-  for (; n < chunks; ++n) {
-    const int st = n % kStages;
-    if (!mbar_wait_warp(&empty[st], ((n / kStages) & 1) ^ 1, a.err, abort)) break;
+  int na = 0, nb = 0;  // chunks begun of each queue
+  for (int n = 0; n < chunks; ++n) {
+    const int st = n % kStages, parity = ((n / kStages) & 1) ^ 1;
     const int at = REV ? chunks - 1 - n : n;
-    const int begin = s.begin + at * kChunk, left = s.len - at * kChunk;
-    const int len = left < kChunk ? left : kChunk;
-    unsigned char* stage = smem + st * stage_bytes<DK>(W);
-    const uint32_t K = smem_u32(stage), Q = K + tile_bytes<DK>();
-    unsigned char* blk = stage + 2 * tile_bytes<DK>();
-    const uint32_t V = smem_u32(blk) + sizeof(Block);
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&full[st], sizeof(Block));
-      bulk_load(blk, a.blocks + static_cast<int64_t>(s.chunk0 + at) * p.Hv + hv, sizeof(Block),
-                &full[st]);
+    const int begin = s.begin + at * kChunk, rest = s.len - at * kChunk;
+    const int len = rest < kChunk ? rest : kChunk;
+    const bool whole = len == kChunk || !p.cu_seqlens;
+    const Block* blk = a.blocks + static_cast<int64_t>(s.chunk0 + at) * p.Hv + hv;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint64_t* full = q ? &bars.full_b[st] : &bars.full_a[st];
+      if (!mbar_wait_warp(q ? &bars.empty_b[st] : &bars.empty_a[st], parity, a.err, &bars.abort))
+        goto done;
+      unsigned char* dst = q ? sm.b(st) : sm.a(st);
+      const bool values = (q == 1) == REV;
+      const bool tma_values = values && whole && have;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(full, kHalf + (whole ? tile_bytes<DK>() : 0) +
+                                        (tma_values ? W * 2048 : 0));
+        bulk_load(dst + tile_bytes<DK>(), reinterpret_cast<const unsigned char*>(blk) + q * kHalf,
+                  kHalf, full);
+        if (whole)
+          for (int i = 0; i < DK / 64; ++i)
+            tma_load_rows(dst + i * kTile, q ? &maps.q : &maps.k, 64 * i, hk, begin, s.b, full);
+        if (tma_values)
+          for (int i = 0; i < W; ++i)
+            tma_load_rows(sm.v(st, i), &maps.v, col0 + 16 * i, hv, begin, s.b, full);
+      }
+      if (!whole)
+        copy_rows(smem_u32(dst),
+                  q ? rows_at(p.q, p.q_stride, s.b, begin, hk)
+                    : rows_at(p.k, p.k_stride, s.b, begin, hk),
+                  q ? p.q_stride[1] : p.k_stride[1], len, DK, p.dk, lane, 32);
+      if (values && !tma_values) {
+        const int64_t stride = REV ? static_cast<int64_t>(p.Hv) * p.dv : p.v_stride[1];
+        const bf16* v = REV ? static_cast<const bf16*>(a.in) +
+                                  (have ? (static_cast<int64_t>(s.b) * p.T + begin) * stride +
+                                              hv * p.dv
+                                        : 0)
+                            : rows_at(p.v, p.v_stride, s.b, begin, hv);
+        for (int i = lane; i < kChunk * 2 * W; i += 32) {
+          const int r = i / (2 * W), c = i % (2 * W), col = col0 + c * 8;
+          const bool real = have && r < len && col < p.dv;
+          cp16(smem_u32(sm.v(st, c >> 1)) + r * 32 + (c & 1) * 16,
+               real ? v + r * stride + col : static_cast<const bf16*>(p.k), real);
+        }
+      }
+      cp_arrive(full);
+      if (q) ++nb; else ++na;
     }
-    copy_rows(K, rows_at(p.k, p.k_stride, s.b, begin, hk), p.k_stride[1], len, DK, p.dk, lane, 32);
-    copy_rows(Q, rows_at(p.q, p.q_stride, s.b, begin, hk), p.q_stride[1], len, DK, p.dk, lane, 32);
-    const bf16* v;
-    int64_t stride;
-    if constexpr (REV) {
-      stride = static_cast<int64_t>(p.Hv) * p.dv;
-      v = static_cast<const bf16*>(a.in) +
-          (have ? (static_cast<int64_t>(s.b) * p.T + begin) * stride + hv * p.dv : 0);
-    } else {
-      stride = p.v_stride[1];
-      v = rows_at(p.v, p.v_stride, s.b, begin, hv);
-    }
-    // a warp's 64 rows of 32 bytes; neighbouring lanes take a row's pieces
-    for (int i = lane; i < kChunk * 2 * W; i += 32) {
-      const int r = i / (2 * W), c = i % (2 * W), col = col0 + c * 8;
-      const bool real = have && r < len && col < p.dv;
-      cp16(V + (c >> 1) * 2048 + r * 32 + (c & 1) * 16,
-           real ? v + r * stride + col : static_cast<const bf16*>(p.k), real);
-    }
-    cp_arrive(&full[st]);
   }
-  if (n < chunks) {  // gave up: no copy of ours may outlive the block
+done:
+  if (nb < chunks) {  // gave up: no copy of ours may outlive the block
     asm volatile("cp.async.wait_all;" ::: "memory");
-    for (int i = n > kStages ? n - kStages : 0; i < n; ++i)
-      mbar_wait_drain(&full[i % kStages], (i / kStages) & 1, kWaitLimitCycles);
+    for (int i = na > kStages ? na - kStages : 0; i < na; ++i)
+      mbar_wait_drain(&bars.full_a[i % kStages], (i / kStages) & 1, kWaitLimitCycles);
+    for (int i = nb > kStages ? nb - kStages : 0; i < nb; ++i)
+      mbar_wait_drain(&bars.full_b[i % kStages], (i / kStages) & 1, kWaitLimitCycles);
   }
 }
 
@@ -397,27 +542,26 @@ __device__ __forceinline__ void put_block(const unsigned char* staging, bf16* ds
     reinterpret_cast<uint4*>(dst)[lane + 32 * i] =
         reinterpret_cast<const uint4*>(staging)[lane + 32 * i];
 }
-// S^T [16, DK] rounded to bf16, to dst [16][DK].
+// S^T [16, DK] in bf16 by way of the staging area, to dst [16][DK]: columns
+// 16 ks .. 16 ks + 15, as a left operand.
 template <int DK>
-__device__ __forceinline__ void put_state(const float (&S)[DK / 8][4], unsigned char* staging,
-                                          bf16* dst) {
+__device__ __forceinline__ void stage_state(const uint32_t (&r)[4], int ks, uint32_t staging) {
   const int lane = threadIdx.x & 31, m = lane >> 3;
-  constexpr int kRow = DK * 2 + 16;
-  const uint32_t base = smem_u32(staging);
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < DK / 8; j += 2)
-    stsm(base + (8 * (m & 1) + (lane & 7)) * kRow + (j + (m >> 1)) * 16,
-         pack_bf16x2(S[j][0], S[j][1]), pack_bf16x2(S[j][2], S[j][3]),
-         pack_bf16x2(S[j + 1][0], S[j + 1][1]), pack_bf16x2(S[j + 1][2], S[j + 1][3]));
-  __syncwarp();
+  stsm(staging + (8 * (m & 1) + (lane & 7)) * (DK * 2 + 16) + (2 * ks + (m >> 1)) * 16, r[0], r[1],
+       r[2], r[3]);
+}
+template <int DK>
+__device__ __forceinline__ void put_state(const unsigned char* staging, bf16* dst) {
+  const int lane = threadIdx.x & 31;
   constexpr int kPieces = DK / 8;
+  __syncwarp();
 #pragma unroll
   for (int i = 0; i < 16 * kPieces / 32; ++i) {
     const int x = lane + 32 * i, r = x / kPieces, c = x % kPieces;
     *reinterpret_cast<uint4*>(dst + r * DK + c * 8) =
-        *reinterpret_cast<const uint4*>(staging + r * kRow + c * 16);
+        *reinterpret_cast<const uint4*>(staging + r * (DK * 2 + 16) + c * 16);
   }
+  __syncwarp();
 }
 // S^T from / to a state [dk, dv] in fp32.
 template <int DK, bool STORE, typename P>
@@ -438,18 +582,22 @@ __device__ __forceinline__ void move_state(float (&S)[DK / 8][4], P* state, int 
     }
 }
 
-// acc [16, 64 tokens] += S^T [16, DK] X^T, X a [64][DK] tile.
+// acc [16, 64 tokens] += S^T [16, DK] X^T, X a [64][DK] tile: columns 16 ks on.
 template <int DK>
 __device__ __forceinline__ void times_rows(float (&acc)[8][4], const uint32_t (&hi)[4],
                                            const uint32_t (&lo)[4], uint32_t X, int ks) {
+  uint32_t b[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) ldsm(b[j], at_nk(X, 16 * j, 2 * ks));
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t b[4];
-    ldsm(b, at_nk(X, 16 * j, 2 * ks));
-    mma(acc[2 * j], hi, b[0], b[1]);
-    mma(acc[2 * j + 1], hi, b[2], b[3]);
-    mma(acc[2 * j], lo, b[0], b[1]);
-    mma(acc[2 * j + 1], lo, b[2], b[3]);
+    mma(acc[2 * j], hi, b[j][0], b[j][1]);
+    mma(acc[2 * j + 1], hi, b[j][2], b[j][3]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    mma(acc[2 * j], lo, b[j][0], b[j][1]);
+    mma(acc[2 * j + 1], lo, b[j][2], b[j][3]);
   }
 }
 // S^T [16, DK] += X^T [16, tokens 16 ks ..] Y, Y a [64][DK] tile.
@@ -457,52 +605,95 @@ template <int DK>
 __device__ __forceinline__ void add_outer(float (&S)[DK / 8][4], const uint32_t (&hi)[4],
                                           const uint32_t (&lo)[4], uint32_t Y, int ks) {
 #pragma unroll
-  for (int j = 0; j < DK / 16; ++j) {
-    uint32_t b[4];
-    ldsm_t(b, at_kn(Y, 16 * ks, 2 * j));
-    mma(S[2 * j], hi, b[0], b[1]);
-    mma(S[2 * j + 1], hi, b[2], b[3]);
-    mma(S[2 * j], lo, b[0], b[1]);
-    mma(S[2 * j + 1], lo, b[2], b[3]);
+  for (int j0 = 0; j0 < DK / 16; j0 += 4) {
+    uint32_t b[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ldsm_t(b[j], at_kn(Y, 16 * ks, 2 * (j0 + j)));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mma(S[2 * (j0 + j)], hi, b[j][0], b[j][1]);
+      mma(S[2 * (j0 + j) + 1], hi, b[j][2], b[j][3]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mma(S[2 * (j0 + j)], lo, b[j][0], b[j][1]);
+      mma(S[2 * (j0 + j) + 1], lo, b[j][2], b[j][3]);
+    }
+  }
+}
+// acc [16, 64 tokens] += X^T [16, 64] M^T (COLUMNS: X^T M), M a lower triangle
+// [64][64] held as a pair, X a pair (PAIR) or exact.  The left operands of the
+// outer loop are independent of one another, the accumulators of the inner one.
+template <bool COLUMNS, bool PAIR>
+__device__ __forceinline__ void times_triangle(float (&acc)[8][4], const uint32_t (&hi)[4][4],
+                                               const uint32_t (&lo)[4][4], uint32_t M) {
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    // rows: token tiles j >= ks meet the tokens of ks; columns: j <= ks
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (COLUMNS ? j > ks : j < ks) continue;
+      uint32_t b[4], c[4];
+      if constexpr (COLUMNS) {
+        ldsm_t(b, at_kn(M, 16 * ks, 2 * j));
+        ldsm_t(c, at_kn(M + kTile, 16 * ks, 2 * j));
+      } else {
+        ldsm(b, at_nk(M, 16 * j, 2 * ks));
+        ldsm(c, at_nk(M + kTile, 16 * j, 2 * ks));
+      }
+      mma(acc[2 * j], hi[ks], b[0], b[1]);
+      mma(acc[2 * j + 1], hi[ks], b[2], b[3]);
+      if constexpr (PAIR) {
+        mma(acc[2 * j], lo[ks], b[0], b[1]);
+        mma(acc[2 * j + 1], lo[ks], b[2], b[3]);
+      }
+      mma(acc[2 * j], hi[ks], c[0], c[1]);
+      mma(acc[2 * j + 1], hi[ks], c[2], c[3]);
+    }
   }
 }
 
 struct Place {
-  int warp, col;  // this warp's first column of the value head
+  int pair, col;  // the pair's first column of the value head
+  unsigned char* share;
   unsigned char* staging;
 };
+__device__ __forceinline__ void signal(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 
-// Chunks in order: N = T diag(beta) (V - diag(e^c) K S), O = scale diag(e^c) Q S + P N,
+// Chunks in order, the state's warp: N = T diag(beta) (V - diag(e^c) K S),
 // S <- e^{c_64} S + K^T diag(e^{c_64 - c}) N, all transposed.
 template <int DK>
-__device__ __forceinline__ void chain_warp(const gsa_delta_t& p, const SeqArgs& a, const Seq& s,
-                                           int hv, const Place& w, int W, unsigned char* smem,
-                                           uint64_t* full, uint64_t* empty, volatile int* abort) {
+__device__ __forceinline__ void chain_state(const gsa_delta_t& p, const SeqArgs& a, const Seq& s,
+                                            int hv, const Place& w, const SeqSmem<DK>& sm,
+                                            SeqBars& bars) {
   const int lane = threadIdx.x & 31, tig = lane & 3;
   const int chunks = (s.len + kChunk - 1) / kChunk;
   const int64_t head = static_cast<int64_t>(blockIdx.x) * p.Hv + hv;
+  uint4* s_share = reinterpret_cast<uint4*>(w.share);
+  uint4* n_share = reinterpret_cast<uint4*>(w.share + state_share<DK>());
   float S[DK / 8][4] = {};
   if (a.state0) move_state<DK, false>(S, a.state0 + head * p.dk * p.dv, p.dk, p.dv, w.col);
   for (int n = 0; n < chunks; ++n) {
     const int st = n % kStages;
-    const int64_t slot = static_cast<int64_t>(s.chunk0 + n) * p.Hv + hv;
-    if (a.states)
-      put_state<DK>(S, w.staging, a.states + (slot * blocks16(p.dv) + w.col / 16) * 16 * DK);
-    if (!mbar_wait_warp(&full[st], (n / kStages) & 1, a.err, abort)) return;
-    unsigned char* stage = smem + st * stage_bytes<DK>(W);
-    const uint32_t K = smem_u32(stage), Q = K + tile_bytes<DK>();
-    const Block* blk = reinterpret_cast<const Block*>(stage + 2 * tile_bytes<DK>());
-    const uint32_t T = smem_u32(blk->t_hi), P = smem_u32(blk->p_hi);
-    const uint32_t V = smem_u32(blk) + sizeof(Block) + w.warp * 2048;
+    if (!mbar_wait_warp(&bars.full_a[st], (n / kStages) & 1, a.err, &bars.abort)) return;
+    if (!mbar_wait_warp(&bars.s_free[w.pair], (n & 1) ^ 1, a.err, &bars.abort)) return;
+    const uint32_t K = smem_u32(sm.a(st));
+    const Block* blk = reinterpret_cast<const Block*>(sm.a(st) + tile_bytes<DK>());
+    const uint32_t T = smem_u32(blk->t_hi), V = smem_u32(sm.v(st, w.pair));
 
-    float R[8][4] = {}, O[8][4] = {};
+    float R[8][4] = {};
 #pragma unroll
     for (int ks = 0; ks < DK / 16; ++ks) {
       uint32_t hi[4], lo[4];
       left(S[2 * ks], S[2 * ks + 1], hi, lo);
+      s_share[(2 * ks) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      s_share[(2 * ks + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       times_rows<DK>(R, hi, lo, K, ks);
-      times_rows<DK>(O, hi, lo, Q, ks);
     }
+    signal(&bars.s_full[w.pair]);
     uint32_t yh[4][4], yl[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -514,49 +705,16 @@ __device__ __forceinline__ void chain_warp(const gsa_delta_t& p, const SeqArgs& 
         const float2 g = *reinterpret_cast<const float2*>(blk->grown + t);
         const float2 b = *reinterpret_cast<const float2*>(blk->beta + t);
         float(&r)[4] = R[2 * j + e];
-        float(&o)[4] = O[2 * j + e];
         r[0] = b.x * (lo_of(v[2 * e]) - g.x * r[0]);
         r[1] = b.y * (hi_of(v[2 * e]) - g.y * r[1]);
         r[2] = b.x * (lo_of(v[2 * e + 1]) - g.x * r[2]);
         r[3] = b.y * (hi_of(v[2 * e + 1]) - g.y * r[3]);
-        o[0] *= p.scale * g.x;
-        o[1] *= p.scale * g.y;
-        o[2] *= p.scale * g.x;
-        o[3] *= p.scale * g.y;
       }
       left(R[2 * j], R[2 * j + 1], yh[j], yl[j]);
     }
     float N[8][4] = {};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int ks = 0; ks <= j; ++ks) {  // T is lower triangular
-        uint32_t b[4], c[4];
-        ldsm(b, at_nk(T, 16 * j, 2 * ks));
-        ldsm(c, at_nk(T + kTile, 16 * j, 2 * ks));
-        mma(N[2 * j], yh[ks], b[0], b[1]);
-        mma(N[2 * j + 1], yh[ks], b[2], b[3]);
-        mma(N[2 * j], yl[ks], b[0], b[1]);
-        mma(N[2 * j + 1], yl[ks], b[2], b[3]);
-        mma(N[2 * j], yh[ks], c[0], c[1]);
-        mma(N[2 * j + 1], yh[ks], c[2], c[3]);
-      }
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) left(N[2 * ks], N[2 * ks + 1], yh[ks], yl[ks]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int ks = 0; ks <= j; ++ks) {
-        uint32_t b[4], c[4];
-        ldsm(b, at_nk(P, 16 * j, 2 * ks));
-        ldsm(c, at_nk(P + kTile, 16 * j, 2 * ks));
-        mma(O[2 * j], yh[ks], b[0], b[1]);
-        mma(O[2 * j + 1], yh[ks], b[2], b[3]);
-        mma(O[2 * j], yl[ks], b[0], b[1]);
-        mma(O[2 * j + 1], yl[ks], b[2], b[3]);
-        mma(O[2 * j], yh[ks], c[0], c[1]);
-        mma(O[2 * j + 1], yh[ks], c[2], c[3]);
-      }
+    times_triangle<false, true>(N, yh, yl, T);
+    if (!mbar_wait_warp(&bars.n_free[w.pair], (n & 1) ^ 1, a.err, &bars.abort)) return;
     const float whole = blk->grown[kChunk - 1];
 #pragma unroll
     for (int j = 0; j < DK / 8; ++j)
@@ -564,55 +722,114 @@ __device__ __forceinline__ void chain_warp(const gsa_delta_t& p, const SeqArgs& 
       for (int e = 0; e < 4; ++e) S[j][e] *= whole;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      float x[2][4];
+      uint32_t hi[4], lo[4];
+      left(N[2 * ks], N[2 * ks + 1], hi, lo);
+      n_share[(2 * ks) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      n_share[(2 * ks + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    signal(&bars.n_full[w.pair]);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float2 g = *reinterpret_cast<const float2*>(blk->left + 16 * ks + 8 * e + 2 * tig);
 #pragma unroll
-        for (int f = 0; f < 4; ++f) x[e][f] = (f & 1 ? g.y : g.x) * N[2 * ks + e][f];
+        for (int f = 0; f < 4; ++f) N[2 * ks + e][f] *= f & 1 ? g.y : g.x;
       }
       uint32_t hi[4], lo[4];
-      left(x[0], x[1], hi, lo);
+      left(N[2 * ks], N[2 * ks + 1], hi, lo);
       add_outer<DK>(S, hi, lo, K, ks);
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[st]);
-    const int len = min(kChunk, s.len - n * kChunk);
-    stage_rows(O, smem_u32(w.staging));
-    put_rows(w.staging,
-             static_cast<bf16*>(a.out) +
-                 ((static_cast<int64_t>(s.b) * p.T + s.begin + n * kChunk) * p.Hv + hv) * p.dv +
-                 w.col,
-             static_cast<int64_t>(p.Hv) * p.dv, len, w.col, p.dv);
-    if (a.rows) {
-      stage_rows(N, smem_u32(w.staging));
-      put_block(w.staging, a.rows + (slot * blocks16(p.dv) + w.col / 16) * kChunk * 16);
-    }
+    signal(&bars.empty_a[st]);
   }
   if (a.state1) move_state<DK, true>(S, a.state1 + head * p.dk * p.dv, p.dk, p.dv, w.col);
 }
 
-// Chunks backwards: dN = P^T dO + diag(e^{c_64 - c}) K dS, dY = T^T dN, dV = beta dY,
-// dS <- e^{c_64} dS - K^T diag(e^c beta) dY + Q^T diag(scale e^c) dO, all transposed.
+// ... and its companion: O = scale diag(e^c) Q S + P N, and what training keeps.
 template <int DK>
-__device__ __forceinline__ void rev_warp(const gsa_delta_t& p, const SeqArgs& a, const Seq& s,
-                                         int hv, const Place& w, int W, unsigned char* smem,
-                                         uint64_t* full, uint64_t* empty, volatile int* abort) {
+__device__ __forceinline__ void chain_output(const gsa_delta_t& p, const SeqArgs& a, const Seq& s,
+                                             int hv, const Place& w, const SeqSmem<DK>& sm,
+                                             SeqBars& bars) {
+  const int lane = threadIdx.x & 31, tig = lane & 3;
+  const int chunks = (s.len + kChunk - 1) / kChunk;
+  const uint4* s_share = reinterpret_cast<const uint4*>(w.share);
+  const uint4* n_share = reinterpret_cast<const uint4*>(w.share + state_share<DK>());
+  const uint32_t staging = smem_u32(w.staging);
+  for (int n = 0; n < chunks; ++n) {
+    const int st = n % kStages;
+    const int64_t slot = static_cast<int64_t>(s.chunk0 + n) * p.Hv + hv;
+    if (!mbar_wait_warp(&bars.full_b[st], (n / kStages) & 1, a.err, &bars.abort)) return;
+    if (!mbar_wait_warp(&bars.s_full[w.pair], n & 1, a.err, &bars.abort)) return;
+    const uint32_t Q = smem_u32(sm.b(st)), P = Q + tile_bytes<DK>();
+    const float* grown = reinterpret_cast<const float*>(sm.b(st) + tile_bytes<DK>() + 2 * kTile);
+    float O[8][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < DK / 16; ++ks) {
+      const uint4 h = s_share[(2 * ks) * 32 + lane], l = s_share[(2 * ks + 1) * 32 + lane];
+      const uint32_t hi[4] = {h.x, h.y, h.z, h.w}, lo[4] = {l.x, l.y, l.z, l.w};
+      times_rows<DK>(O, hi, lo, Q, ks);
+      if (a.states) stage_state<DK>(hi, ks, staging);
+    }
+    signal(&bars.s_free[w.pair]);
+    if (a.states)
+      put_state<DK>(w.staging, a.states + (slot * blocks16(p.dv) + w.col / 16) * 16 * DK);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 g = *reinterpret_cast<const float2*>(grown + 8 * j + 2 * tig);
+#pragma unroll
+      for (int f = 0; f < 4; ++f) O[j][f] *= p.scale * (f & 1 ? g.y : g.x);
+    }
+    if (!mbar_wait_warp(&bars.n_full[w.pair], n & 1, a.err, &bars.abort)) return;
+    uint32_t hi[4][4], lo[4][4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const uint4 h = n_share[(2 * ks) * 32 + lane], l = n_share[(2 * ks + 1) * 32 + lane];
+      hi[ks][0] = h.x; hi[ks][1] = h.y; hi[ks][2] = h.z; hi[ks][3] = h.w;
+      lo[ks][0] = l.x; lo[ks][1] = l.y; lo[ks][2] = l.z; lo[ks][3] = l.w;
+    }
+    signal(&bars.n_free[w.pair]);
+    times_triangle<false, true>(O, hi, lo, P);
+    signal(&bars.empty_b[st]);
+    stage_rows(O, staging);
+    put_rows(w.staging,
+             static_cast<bf16*>(a.out) +
+                 ((static_cast<int64_t>(s.b) * p.T + s.begin + n * kChunk) * p.Hv + hv) * p.dv +
+                 w.col,
+             static_cast<int64_t>(p.Hv) * p.dv, min(kChunk, s.len - n * kChunk), w.col, p.dv);
+    __syncwarp();
+    if (a.rows) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        stsm_t(at_v(staging, 16 * j), hi[j][0], hi[j][1], hi[j][2], hi[j][3]);
+      __syncwarp();
+      put_block(w.staging, a.rows + (slot * blocks16(p.dv) + w.col / 16) * kChunk * 16);
+      __syncwarp();
+    }
+  }
+}
+
+// Chunks backwards, the state's warp: dN = (P^T dO) + diag(e^{c_64 - c}) K dS,
+// dY = T^T dN, dV = beta dY, dS <- e^{c_64} dS - K^T diag(e^c beta) dY + (Q^T
+// diag(scale e^c) dO), all transposed; the terms in brackets are the companion's.
+template <int DK>
+__device__ __forceinline__ void rev_state(const gsa_delta_t& p, const SeqArgs& a, const Seq& s,
+                                          int hv, const Place& w, const SeqSmem<DK>& sm,
+                                          SeqBars& bars) {
   const int lane = threadIdx.x & 31, tig = lane & 3;
   const int chunks = (s.len + kChunk - 1) / kChunk;
   const int64_t head = static_cast<int64_t>(blockIdx.x) * p.Hv + hv;
+  const float4* s_share = reinterpret_cast<const float4*>(w.share);
+  const float4* n_share = reinterpret_cast<const float4*>(w.share + state_share<DK>());
+  const uint32_t staging = smem_u32(w.staging);
   float S[DK / 8][4] = {};
   if (a.state0) move_state<DK, false>(S, a.state0 + head * p.dk * p.dv, p.dk, p.dv, w.col);
   for (int n = 0; n < chunks; ++n) {
     const int st = n % kStages, at = chunks - 1 - n;
     const int64_t slot = static_cast<int64_t>(s.chunk0 + at) * p.Hv + hv;
-    put_state<DK>(S, w.staging, a.states + (slot * blocks16(p.dv) + w.col / 16) * 16 * DK);
-    if (!mbar_wait_warp(&full[st], (n / kStages) & 1, a.err, abort)) return;
-    unsigned char* stage = smem + st * stage_bytes<DK>(W);
-    const uint32_t K = smem_u32(stage), Q = K + tile_bytes<DK>();
-    const Block* blk = reinterpret_cast<const Block*>(stage + 2 * tile_bytes<DK>());
-    const uint32_t T = smem_u32(blk->t_hi), P = smem_u32(blk->p_hi);
-    const uint32_t D = smem_u32(blk) + sizeof(Block) + w.warp * 2048;
+    if (!mbar_wait_warp(&bars.full_a[st], (n / kStages) & 1, a.err, &bars.abort)) return;
+    const uint32_t K = smem_u32(sm.a(st));
+    const Block* blk = reinterpret_cast<const Block*>(sm.a(st) + tile_bytes<DK>());
+    const uint32_t T = smem_u32(blk->t_hi);
 
     float N[8][4] = {};
 #pragma unroll
@@ -620,60 +837,39 @@ __device__ __forceinline__ void rev_warp(const gsa_delta_t& p, const SeqArgs& a,
       uint32_t hi[4], lo[4];
       left(S[2 * ks], S[2 * ks + 1], hi, lo);
       times_rows<DK>(N, hi, lo, K, ks);
+      stage_state<DK>(hi, ks, staging);
     }
-    uint32_t d[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      load_v(d[j], D, 16 * j);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float2 g = *reinterpret_cast<const float2*>(blk->left + 16 * j + 8 * e + 2 * tig);
-#pragma unroll
-        for (int f = 0; f < 4; ++f) N[2 * j + e][f] *= f & 1 ? g.y : g.x;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int ks = j; ks < 4; ++ks) {  // columns 16 j of P start at row 16 j
-        uint32_t b[4], c[4];
-        ldsm_t(b, at_kn(P, 16 * ks, 2 * j));
-        ldsm_t(c, at_kn(P + kTile, 16 * ks, 2 * j));
-        mma(N[2 * j], d[ks], b[0], b[1]);
-        mma(N[2 * j + 1], d[ks], b[2], b[3]);
-        mma(N[2 * j], d[ks], c[0], c[1]);
-        mma(N[2 * j + 1], d[ks], c[2], c[3]);
-      }
+    put_state<DK>(w.staging, a.states + (slot * blocks16(p.dv) + w.col / 16) * 16 * DK);
+    if (!mbar_wait_warp(&bars.n_full[w.pair], n & 1, a.err, &bars.abort)) return;
     uint32_t yh[4][4], yl[4][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 g = *reinterpret_cast<const float2*>(blk->left + 8 * j + 2 * tig);
+      const float4 x = n_share[j * 32 + lane];
+      N[j][0] = fmaf(g.x, N[j][0], x.x);
+      N[j][1] = fmaf(g.y, N[j][1], x.y);
+      N[j][2] = fmaf(g.x, N[j][2], x.z);
+      N[j][3] = fmaf(g.y, N[j][3], x.w);
+    }
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) left(N[2 * ks], N[2 * ks + 1], yh[ks], yl[ks]);
     float Y[8][4] = {};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int ks = j; ks < 4; ++ks) {
-        uint32_t b[4], c[4];
-        ldsm_t(b, at_kn(T, 16 * ks, 2 * j));
-        ldsm_t(c, at_kn(T + kTile, 16 * ks, 2 * j));
-        mma(Y[2 * j], yh[ks], b[0], b[1]);
-        mma(Y[2 * j + 1], yh[ks], b[2], b[3]);
-        mma(Y[2 * j], yl[ks], b[0], b[1]);
-        mma(Y[2 * j + 1], yl[ks], b[2], b[3]);
-        mma(Y[2 * j], yh[ks], c[0], c[1]);
-        mma(Y[2 * j + 1], yh[ks], c[2], c[3]);
-      }
-    const int len = min(kChunk, s.len - at * kChunk);
-    stage_rows(Y, smem_u32(w.staging));
+    times_triangle<true, true>(Y, yh, yl, T);
+    stage_rows(Y, staging);
     put_block(w.staging, a.rows + (slot * blocks16(p.dv) + w.col / 16) * kChunk * 16);
-
     const float whole = blk->grown[kChunk - 1];
 #pragma unroll
-    for (int j = 0; j < DK / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[j][e] *= whole;
+    for (int j = 0; j < DK / 8; ++j) {
+      const float4 x = s_share[j * 32 + lane];
+      S[j][0] = fmaf(whole, S[j][0], x.x);
+      S[j][1] = fmaf(whole, S[j][1], x.y);
+      S[j][2] = fmaf(whole, S[j][2], x.z);
+      S[j][3] = fmaf(whole, S[j][3], x.w);
+    }
+    signal(&bars.n_free[w.pair]);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      float x[2][4], z[2][4];
+      float x[2][4];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int t = 16 * ks + 8 * e + 2 * tig;
@@ -683,36 +879,80 @@ __device__ __forceinline__ void rev_warp(const gsa_delta_t& p, const SeqArgs& a,
         for (int f = 0; f < 4; ++f) {
           Y[2 * ks + e][f] *= f & 1 ? b.y : b.x;  // dV from here on
           x[e][f] = -(f & 1 ? g.y : g.x) * Y[2 * ks + e][f];
-          const uint32_t r = d[ks][2 * e + (f >> 1)];
-          z[e][f] = p.scale * (f & 1 ? g.y : g.x) * (f & 1 ? hi_of(r) : lo_of(r));
         }
       }
       uint32_t hi[4], lo[4];
       left(x[0], x[1], hi, lo);
       add_outer<DK>(S, hi, lo, K, ks);
-      left(z[0], z[1], hi, lo);
-      add_outer<DK>(S, hi, lo, Q, ks);
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[st]);
-    stage_rows(Y, smem_u32(w.staging));
+    signal(&bars.empty_a[st]);
+    stage_rows(Y, staging);
     put_rows(w.staging,
              static_cast<bf16*>(a.out) +
                  ((static_cast<int64_t>(s.b) * p.T + s.begin + at * kChunk) * p.Hv + hv) * p.dv +
                  w.col,
-             static_cast<int64_t>(p.Hv) * p.dv, len, w.col, p.dv);
+             static_cast<int64_t>(p.Hv) * p.dv, min(kChunk, s.len - at * kChunk), w.col, p.dv);
+    __syncwarp();
   }
   if (a.state1) move_state<DK, true>(S, a.state1 + head * p.dk * p.dv, p.dk, p.dv, w.col);
 }
 
-// W computing warps and one that copies; block (sequence, value head, 16 W columns).
+// ... and its companion, a chunk ahead: P^T dO and Q^T diag(scale e^c) dO.
+template <int DK>
+__device__ __forceinline__ void rev_input(const gsa_delta_t& p, const SeqArgs& a, const Seq& s,
+                                          const Place& w, const SeqSmem<DK>& sm, SeqBars& bars) {
+  const int lane = threadIdx.x & 31, tig = lane & 3;
+  const int chunks = (s.len + kChunk - 1) / kChunk;
+  float4* s_share = reinterpret_cast<float4*>(w.share);
+  float4* n_share = reinterpret_cast<float4*>(w.share + state_share<DK>());
+  for (int n = 0; n < chunks; ++n) {
+    const int st = n % kStages;
+    if (!mbar_wait_warp(&bars.full_b[st], (n / kStages) & 1, a.err, &bars.abort)) return;
+    const uint32_t Q = smem_u32(sm.b(st)), P = Q + tile_bytes<DK>();
+    const float* grown = reinterpret_cast<const float*>(sm.b(st) + tile_bytes<DK>() + 2 * kTile);
+    const uint32_t D = smem_u32(sm.v(st, w.pair));
+    uint32_t d[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_v(d[j], D, 16 * j);
+    float N[8][4] = {}, Z[DK / 8][4] = {};
+    times_triangle<true, false>(N, d, d, P);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      float z[2][4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 g = *reinterpret_cast<const float2*>(grown + 16 * ks + 8 * e + 2 * tig);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          const uint32_t r = d[ks][2 * e + (f >> 1)];
+          z[e][f] = p.scale * (f & 1 ? g.y : g.x) * (f & 1 ? hi_of(r) : lo_of(r));
+        }
+      }
+      uint32_t hi[4], lo[4];
+      left(z[0], z[1], hi, lo);
+      add_outer<DK>(Z, hi, lo, Q, ks);
+    }
+    signal(&bars.empty_b[st]);
+    if (!mbar_wait_warp(&bars.n_free[w.pair], (n & 1) ^ 1, a.err, &bars.abort)) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      n_share[j * 32 + lane] = make_float4(N[j][0], N[j][1], N[j][2], N[j][3]);
+#pragma unroll
+    for (int j = 0; j < DK / 8; ++j)
+      s_share[j * 32 + lane] = make_float4(Z[j][0], Z[j][1], Z[j][2], Z[j][3]);
+    signal(&bars.n_full[w.pair]);
+  }
+}
+
+// Block (sequence, value head, 16 W columns).
 template <int DK, bool REV, int W>
-__global__ void __launch_bounds__(32 * (W + 1)) seq_kernel(const gsa_delta_t p, const SeqArgs a) {
+__global__ void __launch_bounds__(32 * (2 * W + 1), 1)
+    seq_kernel(const gsa_delta_t p, const __grid_constant__ DeltaMaps maps, const SeqArgs a) {
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem =
-      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~1023ull);
-  __shared__ uint64_t full[kStages], empty[kStages];
-  __shared__ int abort;
+  const SeqSmem<DK> sm = {
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~1023ull),
+      W};
+  __shared__ SeqBars bars;
   const int hv = blockIdx.y, col0 = blockIdx.z * 16 * W, warp = threadIdx.x >> 5;
   const Seq s = sequence(p, a.table, blockIdx.x);
   if (s.gap) {  // rows of no sequence: zeros
@@ -724,33 +964,50 @@ __global__ void __launch_bounds__(32 * (W + 1)) seq_kernel(const gsa_delta_t p, 
     return;
   }
   if (threadIdx.x == 0) {
-    abort = 0;
+    bars.abort = 0;
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 33);  // 32 copying lanes, and the bulk copy's announcement
-      mbar_init(&empty[i], W);
+      mbar_init(&bars.full_a[i], 33);  // 32 copying lanes, and the bulk copies' announcement
+      mbar_init(&bars.full_b[i], 33);
+      mbar_init(&bars.empty_a[i], W);
+      mbar_init(&bars.empty_b[i], W);
+    }
+    for (int i = 0; i < W; ++i) {
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.s_free[i], 1);
+      mbar_init(&bars.n_full[i], 1);
+      mbar_init(&bars.n_free[i], 1);
     }
     fence_mbar_init();
   }
   __syncthreads();
-  if (warp == W) {
-    produce<DK, REV>(p, a, s, hv, col0, W, smem, full, empty, &abort);
+  if (warp == 2 * W) {
+    produce<DK, REV>(p, maps, a, s, hv, col0, W, sm, bars);
     return;
   }
-  const Place w = {warp, col0 + 16 * warp,
-                   smem + kStages * stage_bytes<DK>(W) + warp * staging_bytes<DK>()};
+  const bool second = warp >= W;
+  const int pair = second ? warp - W : warp;
+  const Place w = {pair, col0 + 16 * pair, sm.pair(pair), sm.pair(pair) + pair_bytes<DK>()};
   if (w.col >= p.dv) {  // columns of no one: keep the stages moving
     const int chunks = (s.len + kChunk - 1) / kChunk;
     for (int n = 0; n < chunks; ++n) {
-      if (!mbar_wait_warp(&full[n % kStages], (n / kStages) & 1, a.err, &abort)) return;
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(&empty[n % kStages]);
+      if (!mbar_wait_warp(second ? &bars.full_b[n % kStages] : &bars.full_a[n % kStages],
+                          (n / kStages) & 1, a.err, &bars.abort))
+        return;
+      signal(second ? &bars.empty_b[n % kStages] : &bars.empty_a[n % kStages]);
     }
     return;
   }
-  if constexpr (REV)
-    rev_warp<DK>(p, a, s, hv, w, W, smem, full, empty, &abort);
-  else
-    chain_warp<DK>(p, a, s, hv, w, W, smem, full, empty, &abort);
+  if constexpr (REV) {
+    if (second)
+      rev_input<DK>(p, a, s, w, sm, bars);
+    else
+      rev_state<DK>(p, a, s, hv, w, sm, bars);
+  } else {
+    if (second)
+      chain_output<DK>(p, a, s, hv, w, sm, bars);
+    else
+      chain_state<DK>(p, a, s, hv, w, sm, bars);
+  }
 }
 
 // ---------------------------------------------------------------- grad
@@ -1105,36 +1362,38 @@ cudaError_t allow(K kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-// Warps of a block of chain / rev: as many as share the copies of K and Q while
-// the blocks still cover the SMs.
-int warps_of(const gsa_delta_t& p) {
+// Pairs of a block of chain / rev: as many as share the copies of K and Q while
+// the blocks still cover the SMs.  Four pairs and the copying warp leave each
+// thread 168 registers, which the state's warp needs.
+int pairs_of(const gsa_delta_t& p) {
   const int64_t all = static_cast<int64_t>(p.N) * p.Hv * blocks16(p.dv);
   int w = 1;
-  while (w < 8 && all / (2 * w) >= 128 && w < blocks16(p.dv)) w *= 2;
+  while (w < 4 && all / (2 * w) >= 128 && w < blocks16(p.dv)) w *= 2;
   return w;
 }
 
 template <int DK, bool REV, int W>
-cudaError_t launch_seq_w(const gsa_delta_t& p, const SeqArgs& a, cudaStream_t stream) {
+cudaError_t launch_seq_w(const gsa_delta_t& p, const DeltaMaps& m, const SeqArgs& a,
+                         cudaStream_t stream) {
   cudaError_t e = allow(seq_kernel<DK, REV, W>, seq_smem<DK>(W));
   if (e != cudaSuccess) return e;
   const int seqs = p.N + (!REV && p.cu_seqlens ? 2 : 0);
-  seq_kernel<DK, REV, W><<<dim3(seqs, p.Hv, (p.dv + 16 * W - 1) / (16 * W)), 32 * (W + 1),
-                           seq_smem<DK>(W), stream>>>(p, a);
+  seq_kernel<DK, REV, W><<<dim3(seqs, p.Hv, (p.dv + 16 * W - 1) / (16 * W)), 32 * (2 * W + 1),
+                           seq_smem<DK>(W), stream>>>(p, m, a);
   return cudaGetLastError();
 }
 template <int DK, bool REV>
-cudaError_t launch_seq(const gsa_delta_t& p, const SeqArgs& a, cudaStream_t stream) {
-  switch (warps_of(p)) {
-    case 1: return launch_seq_w<DK, REV, 1>(p, a, stream);
-    case 2: return launch_seq_w<DK, REV, 2>(p, a, stream);
-    case 4: return launch_seq_w<DK, REV, 4>(p, a, stream);
-    default: return launch_seq_w<DK, REV, 8>(p, a, stream);
+cudaError_t launch_seq(const gsa_delta_t& p, const DeltaMaps& m, const SeqArgs& a,
+                       cudaStream_t stream) {
+  switch (pairs_of(p)) {
+    case 1: return launch_seq_w<DK, REV, 1>(p, m, a, stream);
+    case 2: return launch_seq_w<DK, REV, 2>(p, m, a, stream);
+    default: return launch_seq_w<DK, REV, 4>(p, m, a, stream);
   }
 }
 
 template <int DK>
-cudaError_t forward(const gsa_delta_t& p, void* o, float* final_state, bool save, void* ws,
+cudaError_t forward(const gsa_delta_t& p, const DeltaMaps& m, void* o, float* final_state, bool save, void* ws,
                     int* err, cudaStream_t stream) {
   const Saved s = saved_at(p, ws);
   const Table t = table_at(ws, p.N);
@@ -1147,17 +1406,17 @@ cudaError_t forward(const gsa_delta_t& p, void* o, float* final_state, bool save
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const SeqArgs a = {t,           s.blocks,  nullptr, o, p.initial_state,
                      final_state, save ? s.news : nullptr, save ? s.states : nullptr, err};
-  return launch_seq<DK, false>(p, a, stream);
+  return launch_seq<DK, false>(p, m, a, stream);
 }
 
 template <int DK>
-cudaError_t backward(const gsa_delta_t& p, const DeltaGrads& g, void* saved, void* scratch,
-                     int* err, cudaStream_t stream) {
+cudaError_t backward(const gsa_delta_t& p, const DeltaMaps& m, const DeltaGrads& g, void* saved,
+                     void* scratch, int* err, cudaStream_t stream) {
   const Saved s = saved_at(p, saved);
   const Scratch r = scratch_at(p, scratch);
   const Table t = table_at(saved, p.N);
   const SeqArgs a = {t, s.blocks, g.dout, g.dv, g.dfinal, g.dinitial, r.back, r.states, err};
-  cudaError_t e = launch_seq<DK, true>(p, a, stream);
+  cudaError_t e = launch_seq<DK, true>(p, m, a, stream);
   if (e != cudaSuccess) return e;
   if ((e = allow(grad_kernel<DK>, grad_smem<DK>())) != cudaSuccess) return e;
   const GradArgs ga = {t,      s.blocks, s.news, s.states, r.back, r.states,
@@ -1179,15 +1438,15 @@ int64_t mma_saved_bytes(const gsa_delta_t& p, bool save) {
 int64_t mma_scratch_bytes(const gsa_delta_t& p) {
   return max_chunks(p) * p.Hv * (news_bytes(p) + state_bytes(p));
 }
-cudaError_t mma_forward(const gsa_delta_t& p, void* o, float* final_state, bool save, void* ws,
-                        int* err, cudaStream_t stream) {
-  return p.dk <= 64 ? forward<64>(p, o, final_state, save, ws, err, stream)
-                    : forward<128>(p, o, final_state, save, ws, err, stream);
+cudaError_t mma_forward(const gsa_delta_t& p, const DeltaMaps& m, void* o, float* final_state,
+                        bool save, void* ws, int* err, cudaStream_t stream) {
+  return p.dk <= 64 ? forward<64>(p, m, o, final_state, save, ws, err, stream)
+                    : forward<128>(p, m, o, final_state, save, ws, err, stream);
 }
-cudaError_t mma_backward(const gsa_delta_t& p, const DeltaGrads& g, void* saved, void* scratch,
-                         int* err, cudaStream_t stream) {
-  return p.dk <= 64 ? backward<64>(p, g, saved, scratch, err, stream)
-                    : backward<128>(p, g, saved, scratch, err, stream);
+cudaError_t mma_backward(const gsa_delta_t& p, const DeltaMaps& m, const DeltaGrads& g, void* saved,
+                         void* scratch, int* err, cudaStream_t stream) {
+  return p.dk <= 64 ? backward<64>(p, m, g, saved, scratch, err, stream)
+                    : backward<128>(p, m, g, saved, scratch, err, stream);
 }
 
 }  // namespace delta

@@ -29,12 +29,13 @@ def _strides(t: torch.Tensor, n: int) -> list:
 
 
 def _rows_ok(t: torch.Tensor) -> torch.Tensor:
-    """t [B, T, H, d] as the kernels read it: unit inner stride, rows on 16 bytes in bf16;
-    copied where it is not."""
+    """t [B, T, H, d] as the kernels read it: unit inner stride; in bf16 rows on 16 bytes and no
+    dimension expanded.  Copied where it is not."""
     bf16 = t.dtype == torch.bfloat16
     if t.numel() and (
             (t.shape[3] > 1 and t.stride(3) != 1)
-            or (bf16 and (t.data_ptr() % 16 or any(s % 8 for s in _strides(t, 3))))):
+            or (bf16 and (t.data_ptr() % 16 or any(
+                t.shape[i] > 1 and (t.stride(i) % 8 or t.stride(i) == 0) for i in range(3))))):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 

@@ -427,7 +427,8 @@ GSA_API int gsa_fused_projection_pack(const void* w_q, const void* w_k,
  *   and the device error word (gsa_device_error) is set.
  *   initial_state float32 [N, Hv, dk, dv] contiguous, or NULL for zeros.
  * bf16: tensor cores with 16-bit pairs for the state, so the state keeps
- * about fp32's accuracy; 16-byte aligned rows.  f32: CUDA cores.
+ * about fp32's accuracy; q, k, v rows 16-byte aligned and strides positive
+ * (gsa_delta_rule_*).  f32: CUDA cores.
  */
 typedef struct {
   const void* q;

@@ -57,7 +57,10 @@ def test_delta_null_alignment_and_workspace(lib):
         setattr(a, n, 4096)
     a.q_stride[1] = 4
     assert lib.gsa_delta_rule_forward(ctypes.byref(a), 4096, None, 0, 4096, 1 << 40, None) == 2
-    a.q_stride[1] = 0
+    a.q_stride[1] = 0  # an expanded dimension
+    assert lib.gsa_delta_rule_forward(ctypes.byref(a), 4096, None, 0, 4096, 1 << 40, None) == 2
+    for n in ("q", "k", "v"):
+        getattr(a, n + "_stride")[:] = [1 << 20, 1 << 10, 128]
     a.k = 4098
     assert lib.gsa_delta_rule_forward(ctypes.byref(a), 4096, None, 0, 4096, 1 << 40, None) == 2
     a.k = 4096
