@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -34,12 +35,16 @@ class DeltaArgs(ctypes.Structure):
     )
 
 
+# The same structure as bytes: one call instead of an attribute for each field.
+DELTA_ARGS = struct.Struct("@5Q13q2Q2if7i")
+assert DELTA_ARGS.size == ctypes.sizeof(DeltaArgs)
+
 # Every exported symbol of include/gsa_b200.h with (restype, argtypes).
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
-_dp = ctypes.POINTER(DeltaArgs)
+_dp = ctypes.c_void_p  # gsa_delta_t, as ctypes.byref(DeltaArgs) or packed bytes
 SIGNATURES: dict[str, tuple] = {
     "gsa_version": (_i32, []),
     "gsa_set_fused_selection": (_i32, [_i32]),

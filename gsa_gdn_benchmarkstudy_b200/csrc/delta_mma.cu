@@ -1357,11 +1357,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const gsa_delta_t
 }
 
 // ---------------------------------------------------------------- launches
-template <typename K>
-cudaError_t allow(K kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 // Pairs of a block of chain / rev: as many as share the copies of K and Q while
 // the blocks still cover the SMs.  Four pairs and the copying warp leave each
 // thread 168 registers, which the state's warp needs.
@@ -1375,7 +1370,7 @@ int pairs_of(const gsa_delta_t& p) {
 template <int DK, bool REV, int W>
 cudaError_t launch_seq_w(const gsa_delta_t& p, const DeltaMaps& m, const SeqArgs& a,
                          cudaStream_t stream) {
-  cudaError_t e = allow(seq_kernel<DK, REV, W>, seq_smem<DK>(W));
+  cudaError_t e = allow_smem<seq_kernel<DK, REV, W>>(seq_smem<DK>(W));
   if (e != cudaSuccess) return e;
   const int seqs = p.N + (!REV && p.cu_seqlens ? 2 : 0);
   seq_kernel<DK, REV, W><<<dim3(seqs, p.Hv, (p.dv + 16 * W - 1) / (16 * W)), 32 * (2 * W + 1),
@@ -1398,7 +1393,7 @@ cudaError_t forward(const gsa_delta_t& p, const DeltaMaps& m, void* o, float* fi
   const Saved s = saved_at(p, ws);
   const Table t = table_at(ws, p.N);
   const int64_t chunks = max_chunks(p);
-  cudaError_t e = allow(prep_kernel<DK>, prep_smem<DK>());
+  cudaError_t e = allow_smem<prep_kernel<DK>>(prep_smem<DK>());
   if (e != cudaSuccess) return e;
   if (chunks > 0)
     prep_kernel<DK><<<dim3(static_cast<unsigned>(chunks), p.Hk), kPrepThreads, prep_smem<DK>(),
@@ -1418,7 +1413,7 @@ cudaError_t backward(const gsa_delta_t& p, const DeltaMaps& m, const DeltaGrads&
   const SeqArgs a = {t, s.blocks, g.dout, g.dv, g.dfinal, g.dinitial, r.back, r.states, err};
   cudaError_t e = launch_seq<DK, true>(p, m, a, stream);
   if (e != cudaSuccess) return e;
-  if ((e = allow(grad_kernel<DK>, grad_smem<DK>())) != cudaSuccess) return e;
+  if ((e = allow_smem<grad_kernel<DK>>(grad_smem<DK>())) != cudaSuccess) return e;
   const GradArgs ga = {t,      s.blocks, s.news, s.states, r.back, r.states,
                        g.dout, g.dq,     g.dk,   g.dv,     g.dg,   g.dbeta};
   const int64_t chunks = max_chunks(p);

@@ -566,10 +566,11 @@ int64_t grad_smem(const gsa_delta_t& p) {
   return 4LL * (2 * kChunk * (p.dk + 1) + 2 * p.dk * kLdC + 3 * kChunk * kLdC + 2 * kChunk * kLdM);
 }
 
-template <typename K>
-cudaError_t allow(K kernel, int64_t bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(bytes));
+// The limits are set for the widest head, once.
+gsa_delta_t widest() {
+  gsa_delta_t p = {};
+  p.dk = kDeltaMaxDk;
+  return p;
 }
 
 template <typename E>
@@ -577,8 +578,8 @@ cudaError_t forward(const gsa_delta_t& p, void* o, float* final_state, bool save
                     cudaStream_t stream) {
   const Saved s = saved_at(p, ws);
   const Table t = table_at(ws, p.N);
-  cudaError_t e = allow(prep_kernel<E>, prep_smem(p));
-  if (e == cudaSuccess) e = allow(chain_kernel<E>, chain_smem(p));
+  cudaError_t e = allow_smem<prep_kernel<E>>(static_cast<int>(prep_smem(widest())));
+  if (e == cudaSuccess) e = allow_smem<chain_kernel<E>>(static_cast<int>(chain_smem(widest())));
   if (e != cudaSuccess) return e;
   const int64_t chunks = max_chunks(p);
   if (chunks > 0)
@@ -598,8 +599,8 @@ cudaError_t backward(const gsa_delta_t& p, const DeltaGrads& g, void* saved, voi
   const Saved s = saved_at(p, saved);
   const Scratch r = scratch_at(p, scratch);
   const Table t = table_at(saved, p.N);
-  cudaError_t e = allow(rev_kernel<E>, chain_smem(p));
-  if (e == cudaSuccess) e = allow(grad_kernel<E>, grad_smem(p));
+  cudaError_t e = allow_smem<rev_kernel<E>>(static_cast<int>(chain_smem(widest())));
+  if (e == cudaSuccess) e = allow_smem<grad_kernel<E>>(static_cast<int>(grad_smem(widest())));
   if (e != cudaSuccess) return e;
   const RevArgs ra = {t, s.tiles, g.dout, g.dfinal, r.back, r.states, g.dinitial};
   rev_kernel<E><<<dim3(p.N, p.Hv, (p.dv + kCols - 1) / kCols), kThreads, chain_smem(p), stream>>>(

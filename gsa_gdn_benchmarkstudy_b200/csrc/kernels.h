@@ -11,6 +11,23 @@ namespace gsa {
 // Devices the per-device launch state covers (cudaGetDevice indices).
 constexpr int kMaxDevices = 64;
 
+// Sets a kernel's dynamic shared memory limit once per device (two threads that
+// race here both set the same value).
+template <auto Kernel>
+cudaError_t allow_smem(int bytes) {
+  static std::atomic<bool> done[kMaxDevices];
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < kMaxDevices && done[dev].load(std::memory_order_acquire))
+    return cudaSuccess;
+  const cudaError_t set =
+      cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (set == cudaSuccess && dev >= 0 && dev < kMaxDevices)
+    done[dev].store(true, std::memory_order_release);
+  return set;
+}
+
 cudaError_t launch_rope_gates(const void* q_src, const void* k_src, const void* v_src,
                               const void* vg_src, int64_t src_stride, int dtype, int B, int T,
                               int H, int d, const void* cos_t, const void* sin_t, void* q_out,

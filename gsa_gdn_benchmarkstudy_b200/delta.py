@@ -14,28 +14,25 @@ Both run on the tensors' device and its current stream; there is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _cuda, _dtype_code, _ptr
-
-
-def _strides(t: torch.Tensor, n: int) -> list:
-    """The first n strides, 0 for a dimension of one element (never stepped over)."""
-    return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(n)]
+from .ops import _DTYPES, _cuda, _dtype_code, _on, _ptr, _raw_stream
 
 
 def _rows_ok(t: torch.Tensor) -> torch.Tensor:
     """t [B, T, H, d] as the kernels read it: unit inner stride; in bf16 rows on 16 bytes and no
     dimension expanded.  Copied where it is not."""
-    bf16 = t.dtype == torch.bfloat16
-    if t.numel() and (
-            (t.shape[3] > 1 and t.stride(3) != 1)
-            or (bf16 and (t.data_ptr() % 16 or any(
-                t.shape[i] > 1 and (t.stride(i) % 8 or t.stride(i) == 0) for i in range(3))))):
+    b, r, h, c = t.stride()
+    if t.dtype is torch.bfloat16:
+        if c == 1 and b > 0 and r > 0 and h > 0 and (b | r | h) % 8 == 0 and t.data_ptr() % 16 == 0:
+            return t
+        steps = [x for x, n in zip((b, r, h), t.shape) if n > 1]
+        bad = t.data_ptr() % 16 or any(x % 8 or x <= 0 for x in steps)
+    else:
+        bad = False
+    if t.numel() and (bad or (c != 1 and t.shape[3] > 1)):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -48,46 +45,48 @@ def _gates_ok(t: torch.Tensor) -> torch.Tensor:
 
 def _check(q, k, v, g, beta, *others) -> None:
     _cuda(q, k, v, g, beta, *others)
-    for name, t, dims in (("q", q, 4), ("k", k, 4), ("v", v, 4), ("g", g, 3), ("beta", beta, 3)):
+    for name, t, dims in (("q", q, 4), ("v", v, 4)):
         if t.dim() != dims:
             raise ValueError(f"{name}: expected {dims} dims, got {tuple(t.shape)}")
-    _dtype_code(q), _dtype_code(g)
+    if q.dtype not in _DTYPES or g.dtype not in _DTYPES:
+        _dtype_code(q), _dtype_code(g)
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q, k and v must share a dtype")
     if beta.dtype != g.dtype:
         raise ValueError("g and beta must share a dtype")
     B, T, Hk, dk = q.shape
+    vB, vT, Hv, dv = v.shape
     if k.shape != q.shape:
         raise ValueError(f"k must be [{B}, {T}, {Hk}, {dk}], got {tuple(k.shape)}")
-    Hv, dv = v.shape[2], v.shape[3]
-    if v.shape[:2] != (B, T) or Hk == 0 or Hv == 0 or Hv % Hk:
+    if vB != B or vT != T or Hk == 0 or Hv == 0 or Hv % Hk:
         raise ValueError(f"v must be [{B}, {T}, Hv, dv] with Hv a multiple of {Hk}, got "
                          f"{tuple(v.shape)}")
-    for name, t in (("g", g), ("beta", beta)):
-        if t.shape != (B, T, Hv):
-            raise ValueError(f"{name} must be [{B}, {T}, {Hv}], got {tuple(t.shape)}")
+    gates = (B, T, Hv)
+    if g.shape != gates or beta.shape != gates:
+        raise ValueError(f"g and beta must be [{B}, {T}, {Hv}], got {tuple(g.shape)} and "
+                         f"{tuple(beta.shape)}")
     if dk % 8 or dv % 8 or not 0 < dk <= 128 or not 0 < dv <= 256:
         raise ValueError(f"dk and dv must be multiples of 8, dk <= 128 and dv <= 256, got "
                          f"{dk} and {dv}")
+    device = q.device
     for t in (k, v, g, beta) + others:
-        if t is not None and t.device != q.device:
+        if t is not None and t.device != device:
             raise ValueError("all tensors must be on one device")
 
 
-def _args(q, k, v, g, beta, scale, N, cu, initial) -> _lib.DeltaArgs:
+def _args(q, k, v, g, beta, scale, N, cu, initial) -> bytes:
+    """gsa_delta_t."""
     B, T, Hk, dk = q.shape
-    a = _lib.DeltaArgs()
-    for name, t, n in (("q", q, 3), ("k", k, 3), ("v", v, 3), ("g", g, 2), ("beta", beta, 2)):
-        setattr(a, name, t.data_ptr())
-        getattr(a, name + "_stride")[:] = _strides(t, n)
-    a.cu_seqlens, a.initial_state = _ptr(cu), _ptr(initial)
-    a.dtype, a.gate_dtype, a.scale = _dtype_code(q), _dtype_code(g), float(scale)
-    a.B, a.T, a.Hk, a.Hv, a.dk, a.dv, a.N = B, T, Hk, v.shape[2], dk, v.shape[3], N
-    return a
+    _, _, Hv, dv = v.shape
+    return _lib.DELTA_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride()[:2], *beta.stride()[:2],
+        0 if cu is None else cu.data_ptr(), 0 if initial is None else initial.data_ptr(),
+        _DTYPES[q.dtype], _DTYPES[g.dtype], scale, B, T, Hk, Hv, dk, dv, N)
 
 
-def _workspace(a: _lib.DeltaArgs, use: int, device) -> torch.Tensor:
-    need = int(_lib.load().gsa_delta_rule_workspace_size(ctypes.byref(a), use))
+def _workspace(a: bytes, use: int, device) -> torch.Tensor:
+    need = int(_lib.load().gsa_delta_rule_workspace_size(a, use))
     if need < 0:
         raise RuntimeError(f"gsa_delta_rule_workspace_size failed: {_lib.last_error()}")
     return torch.empty(need, dtype=torch.uint8, device=device)
@@ -102,8 +101,8 @@ def _forward(q, k, v, g, beta, initial, cu, scale, N, want_final, use):
     final = (torch.empty(N, Hv, dk, dv, dtype=torch.float32, device=q.device) if want_final
              else None)
     rc = _lib.load().gsa_delta_rule_forward(
-        ctypes.byref(a), o.data_ptr(), _ptr(final), use, ws.data_ptr(), ws.numel(),
-        torch.cuda.current_stream().cuda_stream)
+        a, o.data_ptr(), _ptr(final), use, ws.data_ptr(), ws.numel(),
+        _raw_stream(q.device.index))
     _lib.check(rc, "gsa_delta_rule_forward")
     return o, final, ws
 
@@ -111,7 +110,7 @@ def _forward(q, k, v, g, beta, initial, cu, scale, N, want_final, use):
 class _GatedDeltaRule(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, initial, cu, scale, N, want_final):
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             o, final, ws = _forward(q, k, v, g, beta, initial, cu, scale, N, want_final,
                                     _lib.GSA_DELTA_TRAINING)
         ctx.save_for_backward(q, k, v, g, beta, cu, ws)
@@ -131,7 +130,7 @@ class _GatedDeltaRule(torch.autograd.Function):
                 do = do.clone()
         if dfinal is not None:
             dfinal = dfinal.float().contiguous()
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             a = _args(q, k, v, g, beta, ctx.scale, ctx.N, cu, None)
             scratch = _workspace(a, _lib.GSA_DELTA_BACKWARD, q.device)
             dq = torch.empty(B, T, Hk, dk, dtype=q.dtype, device=q.device)
@@ -142,10 +141,10 @@ class _GatedDeltaRule(torch.autograd.Function):
             dinitial = (torch.empty(ctx.N, Hv, dk, dv_, dtype=torch.float32, device=q.device)
                         if ctx.has_initial and ctx.needs_input_grad[5] else None)
             rc = _lib.load().gsa_delta_rule_backward(
-                ctypes.byref(a), _ptr(do), _ptr(dfinal), ws.data_ptr(), ws.numel(),
+                a, _ptr(do), _ptr(dfinal), ws.data_ptr(), ws.numel(),
                 scratch.data_ptr(), scratch.numel(), dq.data_ptr(), dk_.data_ptr(), dv.data_ptr(),
                 dg.data_ptr(), dbeta.data_ptr(), _ptr(dinitial),
-                torch.cuda.current_stream().cuda_stream)
+                _raw_stream(q.device.index))
         _lib.check(rc, "gsa_delta_rule_backward")
         return dq, dk_, dv, dg, dbeta, dinitial, None, None, None, None
 
@@ -192,7 +191,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
             t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
         return _GatedDeltaRule.apply(q, k, v, g, beta, initial_state, cu_seqlens, scale, N,
                                      output_final_state)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         return _forward(q, k, v, g, beta, initial_state, cu_seqlens, scale, N,
                         output_final_state, _lib.GSA_DELTA_INFERENCE)[:2]
 
@@ -226,11 +225,11 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         raise ValueError(f"{B} rows need as many states, got {state.shape[0]}")
     scale = dk ** -0.5 if scale is None else float(scale)
     q, k, v, g, beta = _rows_ok(q), _rows_ok(k), _rows_ok(v), _gates_ok(g), _gates_ok(beta)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         a = _args(q, k, v, g, beta, scale, B, None, None)
         o = torch.empty(B, T, Hv, dv, dtype=q.dtype, device=q.device)
         rc = _lib.load().gsa_delta_step(
-            ctypes.byref(a), state.data_ptr(), state.shape[0], _ptr(state_indices), o.data_ptr(),
-            torch.cuda.current_stream().cuda_stream)
+            a, state.data_ptr(), state.shape[0], _ptr(state_indices), o.data_ptr(),
+            _raw_stream(q.device.index))
     _lib.check(rc, "gsa_delta_step")
     return o

@@ -13,12 +13,13 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _cuda, _dtype_code, _ptr
+from .ops import _DTYPES, _cuda, _dtype_code, _on, _ptr, _raw_stream
 
 
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """t as rows [R, D] with unit inner stride (a copy only where the layout needs one)."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -28,31 +29,45 @@ def _row_stride(t: torch.Tensor) -> int:
 
 def _check(x, weight, residual) -> None:
     _cuda(x, weight, residual)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must have a last dim of at least 1, got {tuple(x.shape)}")
-    _dtype_code(x), _dtype_code(weight)
-    if x.shape[-1] > 32768:
-        raise ValueError(f"rows of at most 32768 values, got {x.shape[-1]}")
-    if weight.shape != (x.shape[-1],):
-        raise ValueError(f"weight must be [{x.shape[-1]}], got {tuple(weight.shape)}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError("residual must match x in shape and dtype")
-    if weight.device != x.device or (residual is not None and residual.device != x.device):
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"x must have a last dim of at least 1, got {tuple(shape)}")
+    width = shape[-1]
+    if x.dtype not in _DTYPES or weight.dtype not in _DTYPES:
+        _dtype_code(x), _dtype_code(weight)
+    if width > 32768:
+        raise ValueError(f"rows of at most 32768 values, got {width}")
+    if weight.shape != (width,):
+        raise ValueError(f"weight must be [{width}], got {tuple(weight.shape)}")
+    if weight.device != x.device:
         raise ValueError("all tensors must be on one device")
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != x.dtype:
+            raise ValueError("residual must match x in shape and dtype")
+        if residual.device != x.device:
+            raise ValueError("all tensors must be on one device")
 
 
 def _forward(x, weight, residual, eps, want_rstd):
+    """(y, h, rstd) of x and residual as rows."""
     rows, width = x.shape
-    y = torch.empty(rows, width, dtype=x.dtype, device=x.device)
-    h = torch.empty_like(y) if residual is not None else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
-    with torch.cuda.device(x.device):
+    device = x.device
+    y = torch.empty((rows, width), dtype=x.dtype, device=device)
+    h = rstd = h_ptr = r_ptr = rstd_ptr = None
+    r_stride = 0
+    if residual is not None:
+        h = torch.empty_like(y)
+        h_ptr, r_ptr, r_stride = h.data_ptr(), residual.data_ptr(), _row_stride(residual)
+    if want_rstd:
+        rstd = torch.empty(rows, dtype=torch.float32, device=device)
+        rstd_ptr = rstd.data_ptr()
+    with _on(device):
         rc = _lib.load().gsa_rms_norm(
-            x.data_ptr(), _row_stride(x), _ptr(residual),
-            _row_stride(residual) if residual is not None else 0, weight.data_ptr(),
-            _dtype_code(weight), float(eps), _dtype_code(x), rows, width, y.data_ptr(), width,
-            _ptr(h), width, _ptr(rstd), torch.cuda.current_stream().cuda_stream)
-    _lib.check(rc, "gsa_rms_norm")
+            x.data_ptr(), _row_stride(x), r_ptr, r_stride, weight.data_ptr(),
+            _DTYPES[weight.dtype], eps, _DTYPES[x.dtype], rows, width, y.data_ptr(), width, h_ptr,
+            width, rstd_ptr, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "gsa_rms_norm")
     return y, h, rstd
 
 
@@ -83,7 +98,7 @@ class _RmsNorm(torch.autograd.Function):
         rows = h2.shape[0]
         dx = torch.empty(rows, width, dtype=h.dtype, device=h.device)
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
-        with torch.cuda.device(h.device):
+        with _on(h.device):
             lib = _lib.load()
             need = int(lib.gsa_rms_norm_backward_workspace_size(rows, width)) if dw is not None \
                 else 0
@@ -93,7 +108,7 @@ class _RmsNorm(torch.autograd.Function):
                 _row_stride(dh2) if dh2 is not None else 0, h2.data_ptr(), _row_stride(h2),
                 weight.data_ptr(), _dtype_code(weight), rstd.data_ptr(), _dtype_code(h2), rows,
                 width, dx.data_ptr(), width, _ptr(dw), ws.data_ptr(), need,
-                torch.cuda.current_stream().cuda_stream)
+                _raw_stream(h.device.index))
         _lib.check(rc, "gsa_rms_norm_backward")
         dx = dx.view(h.shape)
         return dx, dw, dx if ctx.needs_input_grad[2] else None, None
@@ -110,12 +125,16 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     adds the rows up in a fixed order."""
     _check(x, weight, residual)
     weight = weight.contiguous()
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, residual)):
-        return _RmsNorm.apply(x, weight, residual, float(eps))
-    y, h, _ = _forward(_flat(x), weight, _flat(residual) if residual is not None else None, eps,
-                       False)
-    return y.view(x.shape) if h is None else (y.view(x.shape), h.view(x.shape))
+    eps = float(eps)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (
+            residual is not None and residual.requires_grad)):
+        return _RmsNorm.apply(x, weight, residual, eps)
+    shape = x.shape
+    y, h, _ = _forward(_flat(x), weight, None if residual is None else _flat(residual), eps, False)
+    if len(shape) != 2:
+        y = y.view(shape)
+        h = h.view(shape) if h is not None else None
+    return y if h is None else (y, h)
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -152,12 +171,12 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     y = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty(rows, groups, dtype=torch.float32, device=x.device)
     h = torch.empty(rows, width, dtype=x.dtype, device=x.device) if r2 is not None else None
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         rc = _lib.load().gsa_rms_norm_fp8(
             x2.data_ptr(), _row_stride(x2), _ptr(r2), _row_stride(r2) if r2 is not None else 0,
             weight.data_ptr(), _dtype_code(weight), float(eps), _dtype_code(x2), rows, width,
             y.data_ptr(), width, scale.data_ptr(), group_size or 0, _ptr(h), width,
-            torch.cuda.current_stream().cuda_stream)
+            _raw_stream(x.device.index))
     _lib.check(rc, "gsa_rms_norm_fp8")
     y, scale = y.view(x.shape), scale.view(x.shape[:-1] + (groups,))
     return (y, scale) if h is None else (y, scale, h.view(x.shape))

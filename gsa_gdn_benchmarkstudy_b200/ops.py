@@ -13,6 +13,8 @@ argument meaning:
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
@@ -29,6 +31,15 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device index
+
+
+def _on(device: torch.device):
+    """Makes ``device`` the current one for a launch, where it is not already."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _cuda(*ts: torch.Tensor) -> None:
