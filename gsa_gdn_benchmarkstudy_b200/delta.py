@@ -68,9 +68,9 @@ def _check(q, k, v, g, beta, *others) -> None:
     if dk % 8 or dv % 8 or not 0 < dk <= 128 or not 0 < dv <= 256:
         raise ValueError(f"dk and dv must be multiples of 8, dk <= 128 and dv <= 256, got "
                          f"{dk} and {dv}")
-    device = q.device
-    for t in (k, v, g, beta) + others:
-        if t is not None and t.device != device:
+    device = q.get_device()
+    for t in (k, v, g, beta, *others):
+        if t is not None and t.get_device() != device:
             raise ValueError("all tensors must be on one device")
 
 
@@ -85,6 +85,12 @@ def _args(q, k, v, g, beta, scale, N, cu, initial) -> bytes:
         _DTYPES[q.dtype], _DTYPES[g.dtype], scale, B, T, Hk, Hv, dk, dv, N)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(
+        t.shape, dtype=t.dtype, device=t.device)
+
+
 def _workspace(a: bytes, use: int, device) -> torch.Tensor:
     need = int(_lib.load().gsa_delta_rule_workspace_size(a, use))
     if need < 0:
@@ -97,7 +103,7 @@ def _forward(q, k, v, g, beta, initial, cu, scale, N, want_final, use):
     Hv, dv = v.shape[2], v.shape[3]
     a = _args(q, k, v, g, beta, scale, N, cu, initial)
     ws = _workspace(a, use, q.device)
-    o = torch.empty(B, T, Hv, dv, dtype=q.dtype, device=q.device)
+    o = _like(v)
     final = (torch.empty(N, Hv, dk, dv, dtype=torch.float32, device=q.device) if want_final
              else None)
     rc = _lib.load().gsa_delta_rule_forward(
@@ -211,25 +217,30 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     _check(q, k, v, g, beta, state, state_indices)
     B, T, _, dk = q.shape
     Hv, dv = v.shape[2], v.shape[3]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or g.requires_grad or beta.requires_grad
+                                    or state.requires_grad):
         raise RuntimeError("gated_delta_step has no gradients; use gated_delta_rule")
-    if (state.dim() != 4 or state.shape[1:] != (Hv, dk, dv) or state.dtype != torch.float32
+    slots = state.shape[0] if state.dim() == 4 else -1
+    if (state.shape != (slots, Hv, dk, dv) or state.dtype is not torch.float32
             or not state.is_contiguous() or state.data_ptr() % 16):
         raise ValueError(f"state must be contiguous float32 [slots, {Hv}, {dk}, {dv}], 16-byte "
                          "aligned")
     if state_indices is not None:
         if state_indices.shape != (B,) or state_indices.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"state_indices must be int32 or int64 [{B}]")
-        state_indices = state_indices.to(torch.int32).contiguous()
-    elif state.shape[0] < B:
-        raise ValueError(f"{B} rows need as many states, got {state.shape[0]}")
+        if state_indices.dtype is not torch.int32 or not state_indices.is_contiguous():
+            state_indices = state_indices.to(torch.int32).contiguous()
+    elif slots < B:
+        raise ValueError(f"{B} rows need as many states, got {slots}")
     scale = dk ** -0.5 if scale is None else float(scale)
     q, k, v, g, beta = _rows_ok(q), _rows_ok(k), _rows_ok(v), _gates_ok(g), _gates_ok(beta)
     with _on(q.device):
         a = _args(q, k, v, g, beta, scale, B, None, None)
-        o = torch.empty(B, T, Hv, dv, dtype=q.dtype, device=q.device)
+        o = _like(v)
         rc = _lib.load().gsa_delta_step(
-            a, state.data_ptr(), state.shape[0], _ptr(state_indices), o.data_ptr(),
+            a, state.data_ptr(), slots, _ptr(state_indices), o.data_ptr(),
             _raw_stream(q.device.index))
-    _lib.check(rc, "gsa_delta_step")
+    if rc:
+        _lib.check(rc, "gsa_delta_step")
     return o

@@ -52,7 +52,8 @@ def _forward(x, weight, residual, eps, want_rstd):
     """(y, h, rstd) of x and residual as rows."""
     rows, width = x.shape
     device = x.device
-    y = torch.empty((rows, width), dtype=x.dtype, device=device)
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(
+        (rows, width), dtype=x.dtype, device=device)
     h = rstd = h_ptr = r_ptr = rstd_ptr = None
     r_stride = 0
     if residual is not None:
@@ -152,8 +153,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     width = x.shape[-1]
     if group_size and width % 128:
         raise ValueError(f"group scales need a last dim that is a multiple of 128, got {width}")
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (
+            residual is not None and residual.requires_grad)):
         raise RuntimeError("rms_norm_fp8 has no gradients; use rms_norm")
 
     def usable(t):
@@ -168,15 +169,24 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     if group_size and weight.data_ptr() % 16:
         weight = weight.clone()
     rows, groups = x2.shape[0], width // group_size if group_size else 1
-    y = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(rows, groups, dtype=torch.float32, device=x.device)
-    h = torch.empty(rows, width, dtype=x.dtype, device=x.device) if r2 is not None else None
-    with _on(x.device):
+    device, dtype = x.device, x.dtype
+    y = torch.empty((rows, width), dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty((rows, groups), dtype=torch.float32, device=device)
+    h = h_ptr = r_ptr = None
+    r_stride = 0
+    if r2 is not None:
+        h = torch.empty_like(x2) if x2.is_contiguous() else torch.empty(
+            (rows, width), dtype=dtype, device=device)
+        h_ptr, r_ptr, r_stride = h.data_ptr(), r2.data_ptr(), _row_stride(r2)
+    with _on(device):
         rc = _lib.load().gsa_rms_norm_fp8(
-            x2.data_ptr(), _row_stride(x2), _ptr(r2), _row_stride(r2) if r2 is not None else 0,
-            weight.data_ptr(), _dtype_code(weight), float(eps), _dtype_code(x2), rows, width,
-            y.data_ptr(), width, scale.data_ptr(), group_size or 0, _ptr(h), width,
-            _raw_stream(x.device.index))
-    _lib.check(rc, "gsa_rms_norm_fp8")
-    y, scale = y.view(x.shape), scale.view(x.shape[:-1] + (groups,))
-    return (y, scale) if h is None else (y, scale, h.view(x.shape))
+            x2.data_ptr(), _row_stride(x2), r_ptr, r_stride, weight.data_ptr(),
+            _DTYPES[weight.dtype], float(eps), _DTYPES[dtype], rows, width, y.data_ptr(), width,
+            scale.data_ptr(), group_size or 0, h_ptr, width, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "gsa_rms_norm_fp8")
+    shape = x.shape
+    if len(shape) != 2:
+        y, scale = y.view(shape), scale.view(shape[:-1] + (groups,))
+        h = h.view(shape) if h is not None else None
+    return (y, scale) if h is None else (y, scale, h)
