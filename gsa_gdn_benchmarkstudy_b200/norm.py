@@ -16,10 +16,8 @@ from . import _lib
 from .ops import _DTYPES, _cuda, _dtype_code, _on, _ptr, _raw_stream
 
 
-def _flat(t: torch.Tensor) -> torch.Tensor:
-    """t as rows [R, D] with unit inner stride (a copy only where the layout needs one)."""
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    """Rows [R, D] with unit inner stride (a copy only where the layout needs one)."""
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -73,46 +71,49 @@ def _forward(x, weight, residual, eps, want_rstd):
 
 
 class _RmsNorm(torch.autograd.Function):
+    """rms_norm of rows [R, D]."""
+
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        x2, r2 = _flat(x), _flat(residual) if residual is not None else None
-        y, h, rstd = _forward(x2, weight, r2, eps, True)
-        y = y.view(x.shape)
-        if residual is None:
-            ctx.save_for_backward(x, weight, rstd)
-            ctx.set_materialize_grads(False)
-            return y
-        h = h.view(x.shape)
-        ctx.save_for_backward(h, weight, rstd)
+        y, h, rstd = _forward(_unit(x), weight, None if residual is None else _unit(residual), eps,
+                              True)
         ctx.set_materialize_grads(False)
+        if h is None:
+            ctx.save_for_backward(x, weight, rstd)
+            return y
+        ctx.save_for_backward(h, weight, rstd)
         return y, h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
+        want_x, want_w, want_r, _ = ctx.needs_input_grad
         if dy is None:  # only the sum h was used
             return dh, None, dh, None
-        width = h.shape[-1]
-        h2, dy2 = _flat(h), _flat(dy.to(h.dtype))
-        dh2 = _flat(dh.to(h.dtype)) if dh is not None else None
-        rows = h2.shape[0]
-        dx = torch.empty(rows, width, dtype=h.dtype, device=h.device)
-        dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
-        with _on(h.device):
-            lib = _lib.load()
-            need = int(lib.gsa_rms_norm_backward_workspace_size(rows, width)) if dw is not None \
-                else 0
-            ws = torch.empty(need, dtype=torch.uint8, device=h.device)
+        h, weight, rstd = ctx.saved_tensors
+        h, dy = _unit(h), _unit(dy)
+        rows, width = h.shape
+        dh_ptr = dw = dw_ptr = ws = ws_ptr = None
+        dh_stride = need = 0
+        if dh is not None:
+            dh = _unit(dh)
+            dh_ptr, dh_stride = dh.data_ptr(), _row_stride(dh)
+        lib, device = _lib.load(), h.device
+        dx = torch.empty_like(h) if h.is_contiguous() else torch.empty(
+            (rows, width), dtype=h.dtype, device=device)
+        if want_w:
+            dw = torch.empty_like(weight)
+            need = lib.gsa_rms_norm_backward_workspace_size(rows, width)
+            ws = torch.empty(need, dtype=torch.uint8, device=device)
+            dw_ptr, ws_ptr = dw.data_ptr(), ws.data_ptr()
+        with _on(device):
             rc = lib.gsa_rms_norm_backward(
-                dy2.data_ptr(), _row_stride(dy2), _ptr(dh2),
-                _row_stride(dh2) if dh2 is not None else 0, h2.data_ptr(), _row_stride(h2),
-                weight.data_ptr(), _dtype_code(weight), rstd.data_ptr(), _dtype_code(h2), rows,
-                width, dx.data_ptr(), width, _ptr(dw), ws.data_ptr(), need,
-                _raw_stream(h.device.index))
-        _lib.check(rc, "gsa_rms_norm_backward")
-        dx = dx.view(h.shape)
-        return dx, dw, dx if ctx.needs_input_grad[2] else None, None
+                dy.data_ptr(), _row_stride(dy), dh_ptr, dh_stride, h.data_ptr(), _row_stride(h),
+                weight.data_ptr(), _DTYPES[weight.dtype], rstd.data_ptr(), _DTYPES[h.dtype], rows,
+                width, dx.data_ptr(), width, dw_ptr, ws_ptr, need, _raw_stream(device.index))
+        if rc:
+            _lib.check(rc, "gsa_rms_norm_backward")
+        return dx, dw, dx if want_r else None, None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -127,12 +128,19 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     _check(x, weight, residual)
     weight = weight.contiguous()
     eps = float(eps)
+    shape = x.shape
+    flat = len(shape) == 2
+    if not flat:
+        x = x.reshape(-1, shape[-1])
+        residual = residual.reshape(-1, shape[-1]) if residual is not None else None
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (
             residual is not None and residual.requires_grad)):
-        return _RmsNorm.apply(x, weight, residual, eps)
-    shape = x.shape
-    y, h, _ = _forward(_flat(x), weight, None if residual is None else _flat(residual), eps, False)
-    if len(shape) != 2:
+        got = _RmsNorm.apply(x, weight, residual, eps)
+        y, h = (got, None) if residual is None else got
+    else:
+        y, h, _ = _forward(_unit(x), weight, None if residual is None else _unit(residual), eps,
+                           False)
+    if not flat:
         y = y.view(shape)
         h = h.view(shape) if h is not None else None
     return y if h is None else (y, h)
@@ -164,7 +172,10 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
             return t.clone(memory_format=torch.contiguous_format)
         return t
 
-    x2, r2 = usable(_flat(x)), usable(_flat(residual)) if residual is not None else None
+    x2 = usable(_unit(x if x.dim() == 2 else x.reshape(-1, width)))
+    r2 = None
+    if residual is not None:
+        r2 = usable(_unit(residual if x.dim() == 2 else residual.reshape(-1, width)))
     weight = weight.contiguous()
     if group_size and weight.data_ptr() % 16:
         weight = weight.clone()
