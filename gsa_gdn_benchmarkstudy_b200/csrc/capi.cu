@@ -954,7 +954,7 @@ int check_delta_inputs(const gsa_delta_t* p) {
 // Map over [batch][token][head][channel] rows of bf16 with strides in elements
 // (that of a dimension of one element does not matter); zero fill out of bounds.
 int make_map_delta(CUtensorMap* map, const void* base, const gsa_delta_t& p, int width, int heads,
-                   const int64_t* stride, bool swizzled) {
+                   const int64_t* stride) {
   PFN_encodeTiled_t fn = encode_fn();
   if (!fn) return set_error(GSA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads),
@@ -964,12 +964,11 @@ int make_map_delta(CUtensorMap* map, const void* base, const gsa_delta_t& p, int
   for (int i = 0; i < 3; ++i)
     strides[i] = dims[i + 1] > 1 ? static_cast<cuuint64_t>(steps[i]) * 2
                                  : static_cast<cuuint64_t>(width) * 2;
-  const cuuint32_t box[4] = {swizzled ? 64u : 16u, 1, 64, 1};
+  const cuuint32_t box[4] = {64, 1, 64, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r =
       fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-         CU_TENSOR_MAP_INTERLEAVE_NONE,
-         swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     std::snprintf(g_last_error, sizeof(g_last_error), "cuTensorMapEncodeTiled failed (%d)",
@@ -979,13 +978,13 @@ int make_map_delta(CUtensorMap* map, const void* base, const gsa_delta_t& p, int
   return GSA_OK;
 }
 
-// The maps of the bf16 kernels; `values` [B, T, Hv, dv] may be NULL.
+// The maps of the bf16 kernels; `values` [B, T, Hv, dv].
 int make_delta_maps(gsa::delta::DeltaMaps* m, const gsa_delta_t& p, const void* values,
                     const int64_t* stride) {
   if (p.T == 0) return GSA_OK;
-  int rc = make_map_delta(&m->q, p.q, p, p.dk, p.Hk, p.q_stride, true);
-  if (!rc) rc = make_map_delta(&m->k, p.k, p, p.dk, p.Hk, p.k_stride, true);
-  if (!rc && values) rc = make_map_delta(&m->v, values, p, p.dv, p.Hv, stride, false);
+  int rc = make_map_delta(&m->q, p.q, p, p.dk, p.Hk, p.q_stride);
+  if (!rc) rc = make_map_delta(&m->k, p.k, p, p.dk, p.Hk, p.k_stride);
+  if (!rc) rc = make_map_delta(&m->v, values, p, p.dv, p.Hv, stride);
   return rc;
 }
 
@@ -1013,10 +1012,10 @@ int64_t gsa_delta_rule_workspace_size(const gsa_delta_t* p, int use) {
     case GSA_DELTA_INFERENCE:
     case GSA_DELTA_TRAINING:
       return p->dtype == GSA_DTYPE_BF16
-                 ? gsa::delta::mma_saved_bytes(*p, use == GSA_DELTA_TRAINING)
+                 ? gsa::delta::bf16_saved_bytes(*p, use == GSA_DELTA_TRAINING)
                  : gsa::delta::simt_saved_bytes(*p, use == GSA_DELTA_TRAINING);
     case GSA_DELTA_BACKWARD:
-      return p->dtype == GSA_DTYPE_BF16 ? gsa::delta::mma_scratch_bytes(*p)
+      return p->dtype == GSA_DTYPE_BF16 ? gsa::delta::bf16_scratch_bytes(*p)
                                         : gsa::delta::simt_scratch_bytes(*p);
     default: set_error(GSA_ERR_INVALID_ARG, "unknown use"); return -1;
   }
@@ -1047,7 +1046,7 @@ int gsa_delta_rule_forward(const gsa_delta_t* p, void* o, float* final_state, in
   cudaError_t e = gsa::delta::launch_table(*p, workspace, st->err, s);
   if (e == cudaSuccess)
     e = bf16
-            ? gsa::delta::mma_forward(*p, maps, o, final_state, use == GSA_DELTA_TRAINING, workspace,
+            ? gsa::delta::bf16_forward(*p, maps, o, final_state, use == GSA_DELTA_TRAINING, workspace,
                                       st->err, s)
             : gsa::delta::simt_forward(*p, o, final_state, use == GSA_DELTA_TRAINING, workspace, s);
   return finish(e);
@@ -1081,12 +1080,15 @@ int gsa_delta_rule_backward(const gsa_delta_t* p, const void* dout, const float*
   void* kept = const_cast<void*>(saved);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = p->dtype == GSA_DTYPE_BF16;
-  gsa::delta::DeltaMaps maps = {};
+  gsa::delta::DeltaMaps maps = {}, more = {};
   const int64_t step = static_cast<int64_t>(p->Hv) * p->dv;
   const int64_t stride[3] = {step * p->T, step, p->dv};
-  if (bf16 && (rc = make_delta_maps(&maps, *p, dout, stride))) return rc;
+  if (bf16 && (rc = make_delta_maps(&maps, *p, p->v, p->v_stride))) return rc;
+  more = maps;
+  if (bf16 && dout && p->T > 0 && (rc = make_map_delta(&more.v, dout, *p, p->dv, p->Hv, stride)))
+    return rc;
   return finish(bf16
-                    ? gsa::delta::mma_backward(*p, maps, g, kept, scratch, st->err, s)
+                    ? gsa::delta::bf16_backward(*p, maps, more, g, kept, scratch, st->err, s)
                     : gsa::delta::simt_backward(*p, g, kept, scratch, s));
 }
 

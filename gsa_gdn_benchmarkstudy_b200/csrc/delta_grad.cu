@@ -1,0 +1,591 @@
+// delta_grad.cu — gradients of the gated delta rule that contract over the
+// state's columns, chunk by chunk, on tcgen05 (bf16 inputs).
+//
+// The two sequential passes left S0, N (forwards) and dS1, dY (backwards) of
+// every chunk.  With A = scale tril(dO N^T) D, M = -strict(dY N^T) beta D and
+// D_ij = e^{c_i - c_j}:
+//   dQ = scale e^c dO S0^T + A K,
+//   dK = -e^c beta dY S0^T + e^{c_64 - c} N dS1^T + A^T Q + (M + M^T) K,
+//   dbeta_i = dY_i.(V_i - e^{c_i} S0^T k_i) - sum_{j<i} (dY N^T)_ij D_ij k_i.k_j,
+//   dg_t = what the decays between tokens before t and from t on carry:
+//          sum_{i>=t} (scale e^c q.(dO S0^T) - e^c beta k.(dY S0^T) + E rows - E columns)_i
+//          + sum_{i<t} e^{c_64 - c_i} k_i.(N dS1^T)_i + e^{c_64} <S0, dS1>,
+//   E = A (q.k) + M (k.k), element by element.
+//
+// A block takes chunks and key heads in turn and the value heads that share the
+// key head one after the other, so that their gradients add up in one order.  All
+// products have 128 rows: channels (dO S0^T and its like, transposed: S0's image is
+// the left operand), or N's and dY's tokens on top of one another.  The factors
+// are bf16, rounded once: the results are bf16 too.  Bound by the bytes: about
+// 210 KB for a chunk and head of 128 x 128, of which the next head's are on their
+// way while this one's elements are worked on.
+#include "delta_tc.cuh"
+
+namespace gsa {
+namespace delta {
+namespace {
+
+constexpr int kComputeWarps = 8;
+constexpr int kThreads = 32 * (kComputeWarps + 2);
+constexpr uint32_t kTmemCols = 512;
+
+// Shared memory.  K, Q and K again, 64 channels at a time, so that [K; Q] and [Q;
+// K] are 128 rows each; images of 128 columns (S0, dS1: channels, N and dY: tokens
+// in groups of 8); dO and V as rows; A^T and M.
+constexpr int kKqkBytes = 3 * static_cast<int>(kTile);  // for 64 channels
+constexpr int kGroup = 128 * 16;                        // 8 channels or tokens of an image
+constexpr int kOffS0 = 2 * kKqkBytes;
+constexpr int kOffS1 = kOffS0 + 16 * kGroup;
+constexpr int kOffN = kOffS1 + 16 * kGroup;
+constexpr int kOffY = kOffN + 8 * kGroup;
+constexpr int kOffD = kOffY + 8 * kGroup;
+constexpr int kOffV = kOffD + 2 * static_cast<int>(kTile);
+constexpr int kOffA = kOffV + 2 * static_cast<int>(kTile);
+constexpr int kOffM = kOffA + static_cast<int>(kTile);
+constexpr int kSmem = kOffM + static_cast<int>(kTile) + 1024;
+
+enum : uint32_t {
+  kTo = 0,     // (dO S0^T)^T [channels][tokens]
+  kTy = 64,    // (dY S0^T)^T
+  kTn = 128,   // (N dS1^T)^T
+  kPd = 192,   // [N; dY] dO^T: rows 0 .. 63 are (dO N^T)^T; then (A K)^T
+  kPn = 256,   // [N; dY] N^T: rows 64 .. 127 are dY N^T; then A^T Q + (M + M^T) K, transposed
+  kPv = 320,   // [N; dY] V^T: rows 64 .. 127 are dY V^T
+  kKq = 384,   // [K; Q] Q^T: rows 0 .. 63 are k_j.q_i
+  kKk = 448,   // [Q; K] K^T: rows 64 .. 127 are k_i.k_j
+};
+
+struct GradArgs {
+  Table table;
+  const bf16* news;
+  const bf16* states;
+  const bf16* back;
+  const bf16* dstates;
+  const void* dout;  // contiguous; may be nullptr
+  void *dq, *dk, *dv, *dg, *dbeta;
+  int64_t items;     // chunks x key heads
+  int* err;
+};
+
+struct Bars {
+  uint64_t full_kq, empty_kq, full_h, empty_h;
+  uint64_t ph1_full, ph2_ready, ph2_full, x_read, drain;
+  uint32_t tmem;
+  int abort;
+};
+
+// Unswizzled image: 16 bytes are 8 neighbours of the outer dimension, the
+// contracted one steps by 16 bytes; 16 of it from 16 ks on.
+__device__ __forceinline__ uint64_t desc_image(uint32_t image, int ks) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>(((image + ks * 256) >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(128 >> 4) << 16;
+  d |= static_cast<uint64_t>(kGroup >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+// [K; Q] (or, from Q on, [Q; K]): 128 rows, channels 16 ks on contracted.
+__device__ __forceinline__ uint64_t desc_kq(uint32_t tile, int ks) {
+  return sdesc_sw128(tile + (ks >> 2) * kKqkBytes + (ks & 3) * 32, 16, 1024);
+}
+// K^T or Q^T: channels are the rows, tokens 16 ks on contracted.
+__device__ __forceinline__ uint64_t desc_kt(uint32_t tile, int ks) {
+  return sdesc_sw128(tile + ks * 2048, kKqkBytes, 1024);
+}
+
+// v[i] summed over the warp's lanes; lane l gets the sum of v[l].
+__device__ __forceinline__ float fold_lanes(float (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int m = 16; m; m >>= 1) {
+    const bool up = lane & m;
+#pragma unroll
+    for (int i = 0; i < m; ++i) {
+      const float give = up ? v[i] : v[i + m], keep = up ? v[i + m] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, m);
+    }
+  }
+  return v[0];
+}
+__device__ __forceinline__ void block_sync() {  // the computing warps
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+
+template <int DK>
+__device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& maps,
+                                        const DeltaMaps& more, const GradArgs& a,
+                                        unsigned char* smem, Bars& bars) {
+  const int lane = threadIdx.x & 31, group = p.Hv / p.Hk, rows = padded_dv(p.dv);
+  int items = 0, loads = 0;
+  bool ok = true;
+  for (int64_t x = blockIdx.x; ok && x < a.items; x += gridDim.x) {
+    const int chunk = static_cast<int>(x / p.Hk), hk = static_cast<int>(x % p.Hk);
+    const Chunk c = chunk_at(p, a.table, chunk);
+    if (!c.valid || c.gap) continue;
+    const bool whole = c.len == kChunk || !p.cu_seqlens;
+    ok = mbar_wait_warp(&bars.empty_kq, (items & 1) ^ 1, a.err, &bars.abort);
+    if (!ok) break;
+    if (!whole) {
+      for (int i = 0; i < DK / 64; ++i) {
+        const uint32_t t = smem_u32(smem) + i * kKqkBytes;
+        const bf16* k = rows_at(p.k, p.k_stride, c.b, c.begin, hk) + 64 * i;
+        copy_rows(t, k, p.k_stride[1], c.len, 64, p.dk - 64 * i, lane, 32);
+        copy_rows(t + 2 * kTile, k, p.k_stride[1], c.len, 64, p.dk - 64 * i, lane, 32);
+        copy_rows(t + kTile, rows_at(p.q, p.q_stride, c.b, c.begin, hk) + 64 * i, p.q_stride[1],
+                  c.len, 64, p.dk - 64 * i, lane, 32);
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.full_kq);
+    } else if (lane == 0) {
+      mbar_arrive_expect_tx(&bars.full_kq, DK / 64 * kKqkBytes);
+      for (int i = 0; i < DK / 64; ++i) {
+        unsigned char* t = smem + i * kKqkBytes;
+        tma_load_rows(t, &maps.k, 64 * i, hk, c.begin, c.b, &bars.full_kq);
+        tma_load_rows(t + kTile, &maps.q, 64 * i, hk, c.begin, c.b, &bars.full_kq);
+        tma_load_rows(t + 2 * kTile, &maps.k, 64 * i, hk, c.begin, c.b, &bars.full_kq);
+      }
+    }
+    ++items;
+    for (int hv = hk * group; ok && hv < (hk + 1) * group; ++hv) {
+      const int64_t slot = static_cast<int64_t>(chunk) * p.Hv + hv;
+      for (int col0 = 0; col0 < p.dv; col0 += 128) {
+        ok = mbar_wait_warp(&bars.empty_h, (loads & 1) ^ 1, a.err, &bars.abort);
+        if (!ok) break;
+        const uint32_t wide = min(128, rows - col0) * 16;
+        const bool tma_d = whole && a.dout != nullptr, tma_v = whole;
+        if (!tma_d || !tma_v) {
+          const int64_t stride = static_cast<int64_t>(p.Hv) * p.dv;
+          if (!tma_d)
+            copy_rows(smem_u32(smem) + kOffD,
+                      a.dout ? static_cast<const bf16*>(a.dout) +
+                                   (static_cast<int64_t>(c.b) * p.T + c.begin) * stride +
+                                   hv * p.dv + col0
+                             : static_cast<const bf16*>(p.k),
+                      stride, a.dout ? c.len : 0, 128, p.dv - col0, lane, 32);
+          if (!tma_v)
+            copy_rows(smem_u32(smem) + kOffV,
+                      rows_at(p.v, p.v_stride, c.b, c.begin, hv) + col0, p.v_stride[1], c.len, 128,
+                      p.dv - col0, lane, 32);
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars.full_h, (2 * (DK / 8) + 16) * wide +
+                                                  (int(tma_d) + int(tma_v)) * 2 * kTile);
+          for (int i = 0; i < 2; ++i) {
+            if (tma_d)
+              tma_load_rows(smem + kOffD + i * kTile, &more.v, col0 + 64 * i, hv, c.begin, c.b,
+                            &bars.full_h);
+            if (tma_v)
+              tma_load_rows(smem + kOffV + i * kTile, &maps.v, col0 + 64 * i, hv, c.begin, c.b,
+                            &bars.full_h);
+          }
+        }
+        __syncwarp();
+        // groups of 8 channels or tokens: a copy each
+        const int64_t step = static_cast<int64_t>(rows) * 8, at = static_cast<int64_t>(col0) * 8;
+        if (lane < DK / 8) {
+          const int64_t from = slot * DK * rows + lane * step + at;
+          bulk_load(smem + kOffS0 + lane * kGroup, a.states + from, wide, &bars.full_h);
+          bulk_load(smem + kOffS1 + lane * kGroup, a.dstates + from, wide, &bars.full_h);
+        }
+        if (lane < 8) {
+          const int64_t from = slot * kChunk * rows + lane * step + at;
+          bulk_load(smem + kOffN + lane * kGroup, a.news + from, wide, &bars.full_h);
+          bulk_load(smem + kOffY + lane * kGroup, a.back + from, wide, &bars.full_h);
+        }
+        ++loads;
+      }
+    }
+  }
+  if (!ok) {  // gave up: no copy of ours may outlive the block
+    if (items) mbar_wait_drain(&bars.full_kq, (items - 1) & 1, kWaitLimitCycles);
+    if (loads) mbar_wait_drain(&bars.full_h, (loads - 1) & 1, kWaitLimitCycles);
+  }
+}
+
+template <int DK>
+__device__ __forceinline__ void issue(const gsa_delta_t& p, const GradArgs& a, uint32_t smem,
+                                      Bars& bars) {
+  const uint32_t tm = bars.tmem, K = smem, Q = smem + kTile;
+  const uint32_t S0 = smem + kOffS0, S1 = smem + kOffS1, N = smem + kOffN, Y = smem + kOffY;
+  const uint32_t D = smem + kOffD, V = smem + kOffV, A = smem + kOffA, M = smem + kOffM;
+  constexpr uint32_t kRR = idesc_bf16_f32(128, 64, 0, 0), kCR = idesc_bf16_f32(128, 64, 1, 0);
+  constexpr uint32_t kCC = idesc_bf16_f32(128, 64, 1, 1);
+  const int group = p.Hv / p.Hk, rows = padded_dv(p.dv);
+  int items = 0, loads = 0, heads = 0;
+  bool ok = true;
+  auto until = [&](uint64_t* bar, int parity) {
+    ok = ok && mbar_wait(bar, parity & 1, a.err, &bars.abort);
+    tc_fence_after();
+    return ok;
+  };
+  for (int64_t x = blockIdx.x; ok && x < a.items; x += gridDim.x) {
+    const Chunk c = chunk_at(p, a.table, static_cast<int>(x / p.Hk));
+    if (!c.valid || c.gap) continue;
+    for (int h = 0; ok && h < group; ++h, ++heads) {
+      if (h == 0) {
+        if (!until(&bars.full_kq, items)) break;
+#pragma unroll
+        for (int ks = 0; ks < DK / 16; ++ks) {
+          tc_mma_ss(tm + kKq, desc_kq(K, ks), desc_kq(Q, ks), kRR, ks > 0);
+          tc_mma_ss(tm + kKk, desc_kq(Q, ks), desc_kq(K, ks), kRR, ks > 0);
+        }
+      }
+      if (heads > 0 && !until(&bars.x_read, heads - 1)) break;
+      for (int col0 = 0; col0 < p.dv; col0 += 128, ++loads) {
+        if (!until(&bars.full_h, loads)) break;
+        const int steps = min(128, rows - col0) / 16;
+        for (int ks = 0; ks < steps; ++ks) {
+          const uint32_t on = col0 > 0 || ks > 0;
+          const uint64_t s0 = desc_image(S0, ks), n = desc_image(N, ks);
+          tc_mma_ss(tm + kTo, s0, desc_rows(D, ks), kCR, on);
+          tc_mma_ss(tm + kTy, s0, desc_image(Y, ks), kCC, on);
+          tc_mma_ss(tm + kTn, desc_image(S1, ks), n, kCC, on);
+          tc_mma_ss(tm + kPd, n, desc_rows(D, ks), kCR, on);
+          tc_mma_ss(tm + kPn, n, n, kCC, on);
+          tc_mma_ss(tm + kPv, n, desc_rows(V, ks), kCR, on);
+        }
+        tc_commit(&bars.empty_h);
+      }
+      if (!ok) break;
+      tc_commit(&bars.ph1_full);
+      if (!until(&bars.ph2_ready, heads)) break;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        tc_mma_ss(tm + kPd, desc_kt(K, ks), desc_cols(A, ks), kCC, ks > 0);
+        tc_mma_ss(tm + kPn, desc_kt(Q, ks), desc_rows(A, ks), kCR, ks > 0);
+        tc_mma_ss(tm + kPn, desc_kt(K, ks), desc_cols(M, ks), kCC, 1);
+        tc_mma_ss(tm + kPn, desc_kt(K, ks), desc_rows(M, ks), kCR, 1);
+      }
+      tc_commit(&bars.ph2_full);
+      if (h == group - 1) tc_commit(&bars.empty_kq);
+    }
+    ++items;
+  }
+  tc_commit(&bars.drain);
+  mbar_wait_drain(&bars.drain, 0, kWaitLimitCycles);
+}
+
+struct Sums {  // per token; by quadrant of lanes where several warps have a part
+  float qo[4][kChunk], ky[4][kChunk], kn[4][kChunk];  // q.tO, k.tY, k.tN
+  float row_x[2][kChunk], col_x[2][kChunk];           // E from A: rows (by quadrant), columns (by half)
+  float row_m[2][kChunk], col_m[2][kChunk];           // E from M: rows (by half), columns (by quadrant)
+  float low[2][kChunk];                               // sum_j l_ij k_i.k_j (by half)
+  float yv[kChunk];                                   // dY_i.V_i
+  float cross[kComputeWarps];
+  float grown[kChunk], left[kChunk];
+  Decays d;
+};
+
+template <int DK>
+__device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
+                                        unsigned char* smem, Bars& bars, Sums& sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = warp & 3, half = warp >> 2;
+  const int row = 32 * quad + lane, tid = threadIdx.x, t0 = 32 * half;
+  const uint32_t tm = bars.tmem + (static_cast<uint32_t>(32 * quad) << 16);
+  const int group = p.Hv / p.Hk, rows = padded_dv(p.dv);
+  const bool gate16 = p.gate_dtype == GSA_DTYPE_BF16;
+  const int64_t qk_step = static_cast<int64_t>(p.Hk) * p.dk;
+  int items = 0, loads = 0, heads = 0;
+  auto until = [&](uint64_t* bar, int parity) {
+    const bool ok = mbar_wait_warp(bar, parity & 1, a.err, &bars.abort);
+    tc_fence_after();
+    return ok;
+  };
+  auto signal = [&](uint64_t* bar) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  for (int64_t x = blockIdx.x; x < a.items; x += gridDim.x) {
+    const int chunk = static_cast<int>(x / p.Hk), hk = static_cast<int>(x % p.Hk);
+    const Chunk c = chunk_at(p, a.table, chunk);
+    if (!c.valid) continue;
+    const int64_t row0 = static_cast<int64_t>(c.b) * p.T + c.begin;
+    bf16* dq_out = static_cast<bf16*>(a.dq) + (row0 * p.Hk + hk) * p.dk;
+    bf16* dk_out = static_cast<bf16*>(a.dk) + (row0 * p.Hk + hk) * p.dk;
+    if (c.gap) {
+      for (int i = tid; i < c.len * p.dk / 8; i += 256) {
+        const int r = i / (p.dk / 8), cc = i % (p.dk / 8) * 8;
+        *reinterpret_cast<uint4*>(dq_out + r * qk_step + cc) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dk_out + r * qk_step + cc) = make_uint4(0, 0, 0, 0);
+      }
+      const int wide = group * p.dv / 8;
+      for (int i = tid; i < c.len * wide; i += 256)
+        *reinterpret_cast<uint4*>(static_cast<bf16*>(a.dv) +
+                                  ((row0 + i / wide) * p.Hv + hk * group) * p.dv + i % wide * 8) =
+            make_uint4(0, 0, 0, 0);
+      for (int i = tid; i < c.len * group; i += 256) {
+        const int64_t at = (row0 + i / group) * p.Hv + hk * group + i % group;
+        store_gate(a.dg, at, gate16, 0.f);
+        store_gate(a.dbeta, at, gate16, 0.f);
+      }
+      continue;
+    }
+    float gq[32], gk[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) gq[i] = gk[i] = 0.f;
+    for (int hv = hk * group; hv < (hk + 1) * group; ++hv, ++heads) {
+      if (warp == 0) {
+        chunk_decays(p, c, hv, sum.d);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          sum.grown[lane + 32 * e] = decay_from_start(sum.d, lane + 32 * e);
+          sum.left[lane + 32 * e] = decay_between(sum.d, kChunk - 1, lane + 32 * e);
+        }
+      }
+      block_sync();
+      // <S0, dS1>
+      float cross = 0.f;
+      for (int col0 = 0; col0 < p.dv; col0 += 128, ++loads) {
+        if (!until(&bars.full_h, loads)) return;
+        const int wide = min(128, rows - col0);
+        for (int i = tid; i < DK / 8 * wide; i += 256) {
+          const int at = (i / wide) * kGroup + (i % wide) * 16;
+          const uint4 u = *reinterpret_cast<const uint4*>(smem + kOffS0 + at);
+          const uint4 w = *reinterpret_cast<const uint4*>(smem + kOffS1 + at);
+          const uint32_t us[4] = {u.x, u.y, u.z, u.w}, ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            cross = fmaf(lo_of(us[e]), lo_of(ws[e]), cross);
+            cross = fmaf(hi_of(us[e]), hi_of(ws[e]), cross);
+          }
+        }
+        signal(&bars.empty_h);
+      }
+#pragma unroll
+      for (int m = 16; m; m >>= 1) cross += __shfl_xor_sync(0xFFFFFFFFu, cross, m);
+      if (lane == 0) sum.cross[warp] = cross;
+
+      if (!until(&bars.ph1_full, heads)) return;
+      // A^T (lanes of tokens j, columns i) and M (lanes of tokens i, columns j)
+      const bool first = quad < 2;
+      const int own = row & 63;  // j, or i
+      uint32_t r[32], u[32];
+      tmem_ld32(tm + (first ? kPd : kPn) + t0, r);
+      tmem_ld32(tm + (first ? kKq : kKk) + t0, u);
+      tc_wait_ld();
+      {
+        float e[32], own_sum = 0.f, low = 0.f;
+        uint32_t packed[16];
+        const float hi0 = sum.d.hi[own], lo0 = sum.d.lo[own], beta0 = sum.d.beta[own];
+#pragma unroll
+        for (int z = 0; z < 32; z += 2) {
+          float y[2];
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            const int other = t0 + z + f;
+            const float dh = sum.d.hi[other] - hi0, dl = sum.d.lo[other] - lo0;
+            // decays run from j to i >= j
+            const bool in = first ? other >= own : other < own;
+            const float w = in ? expf(first ? dh + dl : -(dh + dl)) : 0.f;
+            const float prod = __uint_as_float(r[z + f]), dot = __uint_as_float(u[z + f]);
+            const float l = in ? -prod * w : 0.f;
+            y[f] = first ? -p.scale * l : l * beta0;
+            e[z + f] = in ? y[f] * dot : 0.f;
+            own_sum += e[z + f];
+            low += in ? l * dot : 0.f;
+          }
+          packed[z >> 1] = pack_bf16x2(y[0], y[1]);
+        }
+        unsigned char* tile = smem + (first ? kOffA : kOffM);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(tile + sw128_offset(own, 4 * half + i)) = make_uint4(
+              packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+        const float across = fold_lanes(e);  // lane l: column t0 + l over this warp's rows
+        if (first) {
+          sum.col_x[half][own] = own_sum;
+          sum.row_x[quad][t0 + lane] = across;
+        } else {
+          sum.row_m[half][own] = own_sum;
+          sum.col_m[quad - 2][t0 + lane] = across;
+          sum.low[half][own] = low;
+          tmem_ld32(tm + kPv + t0, r);
+          tc_wait_ld();
+          float diag = 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) diag = own == t0 + i ? __uint_as_float(r[i]) : diag;
+          if ((own >> 5) == half) sum.yv[own] = diag;
+        }
+      }
+      fence_proxy_async_smem();  // A^T and M are read by the products
+      // channels: what S0 and dS1 give, and its products with q and k
+      {
+        const unsigned char* kt = smem + (row >> 6) * kKqkBytes + 2 * (row & 7);
+        const int piece = (row & 63) >> 3;
+        const bool real = row < DK;
+        float e[32];
+        tmem_ld32(tm + kTo + t0, r);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float v = real ? __uint_as_float(r[i]) : 0.f;
+          gq[i] = fmaf(p.scale * sum.grown[t0 + i], v, gq[i]);
+          e[i] = real ? v * __bfloat162float(*reinterpret_cast<const bf16*>(
+                                kt + kTile + sw128_offset(t0 + i, piece)))
+                      : 0.f;
+        }
+        sum.qo[quad][t0 + lane] = fold_lanes(e);
+        tmem_ld32(tm + kTy + t0, r);
+        tmem_ld32(tm + kTn + t0, u);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float v = real ? __uint_as_float(r[i]) : 0.f;
+          const float k = real ? __bfloat162float(*reinterpret_cast<const bf16*>(
+                                     kt + sw128_offset(t0 + i, piece)))
+                               : 0.f;
+          gk[i] = fmaf(-sum.grown[t0 + i] * sum.d.beta[t0 + i], v, gk[i]);
+          e[i] = v * k;
+          r[i] = __float_as_uint(k);
+        }
+        sum.ky[quad][t0 + lane] = fold_lanes(e);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float v = real ? __uint_as_float(u[i]) : 0.f;
+          gk[i] = fmaf(sum.left[t0 + i], v, gk[i]);
+          e[i] = v * __uint_as_float(r[i]);
+        }
+        sum.kn[quad][t0 + lane] = fold_lanes(e);
+      }
+      signal(&bars.ph2_ready);
+      block_sync();
+      if (warp == 0) {  // two neighbouring tokens a lane
+        float rs[2], gs[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int t = 2 * lane + e;
+          const float g = sum.grown[t], beta = sum.d.beta[t];
+          const float qo = (sum.qo[0][t] + sum.qo[1][t]) + (sum.qo[2][t] + sum.qo[3][t]);
+          const float ky = (sum.ky[0][t] + sum.ky[1][t]) + (sum.ky[2][t] + sum.ky[3][t]);
+          const float kn = (sum.kn[0][t] + sum.kn[1][t]) + (sum.kn[2][t] + sum.kn[3][t]);
+          const float er = (sum.row_x[0][t] + sum.row_x[1][t]) + (sum.row_m[0][t] + sum.row_m[1][t]);
+          const float ec = (sum.col_x[0][t] + sum.col_x[1][t]) + (sum.col_m[0][t] + sum.col_m[1][t]);
+          rs[e] = p.scale * g * qo - g * beta * ky + er - ec;
+          gs[e] = sum.left[t] * kn;
+          if (t < c.len)
+            store_gate(a.dbeta, (row0 + t) * p.Hv + hv, gate16,
+                       sum.yv[t] - g * ky + (sum.low[0][t] + sum.low[1][t]));
+        }
+        float suffix = rs[0] + rs[1], prefix = gs[0] + gs[1];
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+          const float o = __shfl_down_sync(0xFFFFFFFFu, suffix, m);
+          if (lane + m < 32) suffix += o;
+          const float q = __shfl_up_sync(0xFFFFFFFFu, prefix, m);
+          if (lane >= m) prefix += q;
+        }
+        float after = __shfl_down_sync(0xFFFFFFFFu, suffix, 1);
+        float before = __shfl_up_sync(0xFFFFFFFFu, prefix, 1);
+        if (lane == 31) after = 0.f;
+        if (lane == 0) before = 0.f;
+        float whole = lane < kComputeWarps ? sum.cross[lane] : 0.f;
+#pragma unroll
+        for (int m = 16; m; m >>= 1) whole += __shfl_xor_sync(0xFFFFFFFFu, whole, m);
+        whole *= sum.grown[kChunk - 1];
+        const float dg0 = whole + before + (rs[0] + (rs[1] + after));
+        const float dg1 = whole + (before + gs[0]) + (rs[1] + after);
+        if (2 * lane < c.len) store_gate(a.dg, (row0 + 2 * lane) * p.Hv + hv, gate16, dg0);
+        if (2 * lane + 1 < c.len)
+          store_gate(a.dg, (row0 + 2 * lane + 1) * p.Hv + hv, gate16, dg1);
+      }
+      if (hv == (hk + 1) * group - 1) signal(&bars.empty_kq);  // q and k are read
+      if (!until(&bars.ph2_full, heads)) return;
+      tmem_ld32(tm + kPd + t0, r);
+      tmem_ld32(tm + kPn + t0, u);
+      tc_wait_ld();
+      signal(&bars.x_read);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        gq[i] += __uint_as_float(r[i]);
+        gk[i] += __uint_as_float(u[i]);
+      }
+    }
+    ++items;
+    if (row < p.dk) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (t0 + i < c.len) {
+          dq_out[(t0 + i) * qk_step + row] = __float2bfloat16_rn(gq[i]);
+          dk_out[(t0 + i) * qk_step + row] = __float2bfloat16_rn(gk[i]);
+        }
+    }
+  }
+}
+
+// maps: q, k and v; more.v: dO.
+template <int DK>
+__global__ void __launch_bounds__(kThreads, 1)
+    grad_kernel(const gsa_delta_t p, const __grid_constant__ DeltaMaps maps,
+                const __grid_constant__ DeltaMaps more, const GradArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~1023ull);
+  __shared__ Bars bars;
+  __shared__ Sums sum;
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    bars.abort = 0;
+    mbar_init(&bars.full_kq, 1);
+    mbar_init(&bars.empty_kq, 1 + kComputeWarps);
+    mbar_init(&bars.full_h, 1);
+    mbar_init(&bars.empty_h, 1 + kComputeWarps);
+    mbar_init(&bars.ph1_full, 1);
+    mbar_init(&bars.ph2_ready, kComputeWarps);
+    mbar_init(&bars.ph2_full, 1);
+    mbar_init(&bars.x_read, kComputeWarps);
+    mbar_init(&bars.drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == kComputeWarps) {
+    tmem_alloc(&bars.tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kComputeWarps + 1)
+    produce<DK>(p, maps, more, a, smem, bars);
+  else if (warp == kComputeWarps) {
+    if ((threadIdx.x & 31) == 0) issue<DK>(p, a, smem_u32(smem), bars);
+  } else {
+    compute<DK>(p, a, smem, bars, sum);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kComputeWarps) {
+    tc_fence_after();
+    tmem_dealloc(bars.tmem, kTmemCols);
+  }
+}
+
+template <int DK>
+cudaError_t launch(const gsa_delta_t& p, const DeltaMaps& maps, const DeltaMaps& more,
+                   const GradArgs& a, cudaStream_t stream) {
+  const cudaError_t e = allow_smem<grad_kernel<DK>>(kSmem);
+  if (e != cudaSuccess) return e;
+  const int blocks = static_cast<int>(a.items < 148 ? a.items : 148);
+  grad_kernel<DK><<<blocks, kThreads, kSmem, stream>>>(p, maps, more, a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_grad(const gsa_delta_t& p, const DeltaMaps& maps, const DeltaMaps& more,
+                        const DeltaGrads& g, const Saved& s, const Scratch& r, const Table& t,
+                        int* err, cudaStream_t stream) {
+  const GradArgs a = {t,     s.news, s.states, r.back,  r.states,
+                      g.dout, g.dq,  g.dk,     g.dv,    g.dg,
+                      g.dbeta, max_chunks(p) * p.Hk, err};
+  if (a.items == 0) return cudaSuccess;
+  return p.dk <= 64 ? launch<64>(p, maps, more, a, stream) : launch<128>(p, maps, more, a, stream);
+}
+
+}  // namespace delta
+}  // namespace gsa

@@ -1,0 +1,272 @@
+// delta_prep.cu — the gated delta rule for bf16 inputs: what a chunk needs apart
+// from any state, T = (I + L)^-1 and P (formulas: delta_common.cuh), for all chunks
+// at once, and the launches of the forward and backward pass.
+//
+// One block a chunk and key head makes T and P of the value heads that share the
+// key head.  Its two products (64 x 64 x dk) are mma.sync: they are small, and
+// their results are wanted in registers, where the decays are applied.  T and P
+// leave as hi + lo pairs of bf16, laid out as the shared-memory tiles that the
+// sequential pass copies whole.  Bound by latency: loads, two products, a
+// triangular inverse and 34 KB of stores one after the other; four blocks an SM
+// overlap theirs.
+#include "delta_tc.cuh"
+
+namespace gsa {
+namespace delta {
+namespace {
+
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                    uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Right operand, stored [n][k]: the pieces of two n-tiles (rows n0 .. n0 + 15)
+// and 16 columns (piece c, c + 1 of the whole row).  r[0], r[1]: first n-tile.
+__device__ __forceinline__ uint32_t at_nk(uint32_t tile, int n0, int c) {
+  const int l = threadIdx.x & 31, m = l >> 3;
+  const int row = n0 + 8 * (m >> 1) + (l & 7), piece = c + (m & 1);
+  return tile + (piece >> 3) * kTile + sw128_offset(row, piece & 7);
+}
+// Left operand, stored [m][k]: rows m0 .. m0 + 15, pieces c, c + 1.
+__device__ __forceinline__ uint32_t at_mk(uint32_t tile, int m0, int c) {
+  const int l = threadIdx.x & 31, m = l >> 3;
+  const int row = m0 + 8 * (m & 1) + (l & 7), piece = c + (m >> 1);
+  return tile + (piece >> 3) * kTile + sw128_offset(row, piece & 7);
+}
+
+// ---------------------------------------------------------------- prep
+constexpr int kPrepThreads = 128;
+constexpr int kLdL = kChunk + 4;
+constexpr int kLdX = 36;
+
+// K and Q, whose place the block's image takes once their products are in
+// registers; L, which becomes T in place; a 32 x 32 product.
+template <int DK>
+constexpr int prep_smem() {
+  return (2 * (DK / 64) * static_cast<int>(kTile) > static_cast<int>(sizeof(Block))
+              ? 2 * (DK / 64) * static_cast<int>(kTile)
+              : static_cast<int>(sizeof(Block))) +
+         (kChunk * kLdL + 32 * kLdX) * 4 + 1024;
+}
+
+// out[r][c] = sign sum_k a[r][k] b[k][c] for a 32 x 32 block, 2 x 4 a thread.
+__device__ __forceinline__ void block32(const float* a, int lda, const float* b, int ldb,
+                                        float* out, int ldo, float sign) {
+  const int r = (threadIdx.x >> 3) * 2, c = (threadIdx.x & 7) * 4;
+  float x[2][4] = {};
+#pragma unroll 8
+  for (int k = 0; k < 32; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(b + k * ldb + c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float u = a[(r + i) * lda + k];
+      x[i][0] = fmaf(u, v.x, x[i][0]);
+      x[i][1] = fmaf(u, v.y, x[i][1]);
+      x[i][2] = fmaf(u, v.z, x[i][2]);
+      x[i][3] = fmaf(u, v.w, x[i][3]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    *reinterpret_cast<float4*>(out + (r + i) * ldo + c) =
+        make_float4(sign * x[i][0], sign * x[i][1], sign * x[i][2], sign * x[i][3]);
+}
+// The same for the two 16 x 16 blocks of a level, 64 threads and 1 x 4 each.
+__device__ __forceinline__ void block16(const float* a, int lda, const float* b, int ldb,
+                                        float* out, int ldo, float sign) {
+  const int t = threadIdx.x & 63, r = t >> 2, c = (t & 3) * 4;
+  float x[4] = {};
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(b + k * ldb + c);
+    const float u = a[r * lda + k];
+    x[0] = fmaf(u, v.x, x[0]);
+    x[1] = fmaf(u, v.y, x[1]);
+    x[2] = fmaf(u, v.z, x[2]);
+    x[3] = fmaf(u, v.w, x[3]);
+  }
+  *reinterpret_cast<float4*>(out + r * ldo + c) =
+      make_float4(sign * x[0], sign * x[1], sign * x[2], sign * x[3]);
+}
+
+// L (strictly lower, 64 x 64) becomes T = (I + L)^-1 in place, in fp32: the four
+// 16 x 16 diagonal blocks by substitution, then T21 = -T22 L21 T11 twice over.
+// A column a thread over all 64 rows took 2.5 times as long: half the threads
+// idle, 64 values of a column in registers.
+__device__ __forceinline__ void invert(float* L, float* X) {
+  const int tid = threadIdx.x;
+  {
+    const int b = (tid & 63) >> 4, j = tid & 15;
+    float* D = L + 16 * b * kLdL + 16 * b;
+    float col[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == j ? 1.f : 0.f;
+#pragma unroll
+      for (int m = 0; m < i; ++m) s = fmaf(-D[i * kLdL + m], col[m], s);
+      col[i] = s;
+    }
+    __syncthreads();
+    if (tid < 64)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) D[i * kLdL + j] = col[i];
+  }
+  __syncthreads();
+  const int b = (tid >> 6) * 32;
+  float* D = L + b * kLdL + b;
+  float* Y = X + (tid >> 6) * 16 * kLdX;
+  block16(D + 16 * kLdL, kLdL, D, kLdL, Y, kLdX, 1.f);
+  __syncthreads();
+  block16(D + 16 * kLdL + 16, kLdL, Y, kLdX, D + 16 * kLdL, kLdL, -1.f);
+  __syncthreads();
+  block32(L + 32 * kLdL, kLdL, L, kLdL, X, kLdX, 1.f);
+  __syncthreads();
+  block32(L + 32 * kLdL + 32, kLdL, X, kLdX, L + 32 * kLdL, kLdL, -1.f);
+  __syncthreads();
+}
+
+template <int DK>
+__global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t p, Table table,
+                                                               Block* blocks) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~1023ull);
+  __shared__ Decays d;
+  const int hk = blockIdx.y, group = p.Hv / p.Hk, tid = threadIdx.x, lane = tid & 31;
+  const int m0 = (tid >> 5) * 16, gid = lane >> 2, tig = lane & 3;
+  const Chunk c = chunk_at(p, table, blockIdx.x);
+  if (!c.valid || c.gap) return;
+  const uint32_t K = smem_u32(smem), Q = K + (DK / 64) * kTile;
+  Block* img = reinterpret_cast<Block*>(smem);
+  float* L = reinterpret_cast<float*>(smem + prep_smem<DK>() - 1024) - kChunk * kLdL - 32 * kLdX;
+  float* X = L + kChunk * kLdL;
+  copy_rows(K, rows_at(p.k, p.k_stride, c.b, c.begin, hk), p.k_stride[1], c.len, DK, p.dk, tid,
+            kPrepThreads);
+  copy_rows(Q, rows_at(p.q, p.q_stride, c.b, c.begin, hk), p.q_stride[1], c.len, DK, p.dk, tid,
+            kPrepThreads);
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+  if (tid < 32) chunk_decays(p, c, hk * group, d);
+  __syncthreads();
+  float kk[8][4] = {}, qk[8][4] = {};
+#pragma unroll
+  for (int ks = 0; ks < DK / 16; ++ks) {
+    uint32_t ka[4], qa[4];
+    ldsm(ka, at_mk(K, m0, 2 * ks));
+    ldsm(qa, at_mk(Q, m0, 2 * ks));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t b[4];
+      ldsm(b, at_nk(K, 16 * j, 2 * ks));
+      mma(kk[2 * j], ka, b[0], b[1]);
+      mma(kk[2 * j + 1], ka, b[2], b[3]);
+      mma(qk[2 * j], qa, b[0], b[1]);
+      mma(qk[2 * j + 1], qa, b[2], b[3]);
+    }
+  }
+  for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
+    __syncthreads();  // K and Q, or the last head's image, are read
+    if (hv > hk * group) {
+      if (tid < 32) chunk_decays(p, c, hv, d);
+      __syncthreads();
+    }
+    if (tid < kChunk) {
+      img->grown[tid] = img->grown_p[tid] = decay_from_start(d, tid);
+      img->beta[tid] = d.beta[tid];
+      img->left[tid] = decay_between(d, kChunk - 1, tid);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = m0 + gid + 8 * e, cc = 8 * j + 2 * tig;
+        float l[2] = {0.f, 0.f}, x[2] = {0.f, 0.f};
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+          if (r >= cc + f) {
+            const float w = decay_between(d, r, cc + f);
+            if (r > cc + f) l[f] = d.beta[r] * w * kk[j][2 * e + f];
+            x[f] = p.scale * w * qk[j][2 * e + f];
+          }
+        *reinterpret_cast<float2*>(L + r * kLdL + cc) = make_float2(l[0], l[1]);
+        uint32_t hi, lo;
+        split(x[0], x[1], hi, lo);
+        const uint32_t at = sw128_offset(r, j) + 4 * tig;
+        *reinterpret_cast<uint32_t*>(img->p_hi + at) = hi;
+        *reinterpret_cast<uint32_t*>(img->p_lo + at) = lo;
+      }
+    __syncthreads();
+    invert(L, X);
+#pragma unroll
+    for (int i = 0; i < kChunk * 8 / kPrepThreads; ++i) {
+      const int x = tid + i * kPrepThreads, r = x >> 3, piece = x & 7;
+      const float4 u = *reinterpret_cast<const float4*>(L + r * kLdL + piece * 8);
+      const float4 v = *reinterpret_cast<const float4*>(L + r * kLdL + piece * 8 + 4);
+      uint4 hi, lo;
+      split(u.x, u.y, hi.x, lo.x);
+      split(u.z, u.w, hi.y, lo.y);
+      split(v.x, v.y, hi.z, lo.z);
+      split(v.z, v.w, hi.w, lo.w);
+      *reinterpret_cast<uint4*>(img->t_hi + sw128_offset(r, piece)) = hi;
+      *reinterpret_cast<uint4*>(img->t_lo + sw128_offset(r, piece)) = lo;
+    }
+    __syncthreads();
+    uint4* dst = reinterpret_cast<uint4*>(blocks + static_cast<int64_t>(blockIdx.x) * p.Hv + hv);
+    const uint4* src = reinterpret_cast<const uint4*>(img);
+    for (int i = tid; i < static_cast<int>(sizeof(Block) / 16); i += kPrepThreads) dst[i] = src[i];
+  }
+}
+
+template <int DK>
+cudaError_t launch_prep(const gsa_delta_t& p, const Table& t, Block* blocks, cudaStream_t stream) {
+  const int64_t chunks = max_chunks(p);
+  if (chunks == 0) return cudaSuccess;
+  const cudaError_t e = allow_smem<prep_kernel<DK>>(prep_smem<DK>());
+  if (e != cudaSuccess) return e;
+  prep_kernel<DK><<<dim3(static_cast<unsigned>(chunks), p.Hk), kPrepThreads, prep_smem<DK>(),
+                    stream>>>(p, t, blocks);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+int64_t bf16_saved_bytes(const gsa_delta_t& p, bool save) {
+  const int64_t n = max_chunks(p) * p.Hv;
+  return table_bytes(p) + n * (static_cast<int64_t>(sizeof(Block)) +
+                               (save ? 2 * (news_elems(p) + state_elems(p)) : 0));
+}
+int64_t bf16_scratch_bytes(const gsa_delta_t& p) {
+  return 2 * max_chunks(p) * p.Hv * (news_elems(p) + state_elems(p));
+}
+cudaError_t bf16_forward(const gsa_delta_t& p, const DeltaMaps& m, void* o, float* final_state,
+                         bool save, void* ws, int* err, cudaStream_t stream) {
+  const Saved s = saved_at(p, ws);
+  const Table t = table_at(ws, p.N);
+  const cudaError_t e = p.dk <= 64 ? launch_prep<64>(p, t, s.blocks, stream)
+                                   : launch_prep<128>(p, t, s.blocks, stream);
+  if (e != cudaSuccess) return e;
+  const SeqArgs a = {t,           s.blocks,  nullptr, o, p.initial_state,
+                     final_state, save ? s.news : nullptr, save ? s.states : nullptr, err};
+  return launch_seq(p, m, a, false, stream);
+}
+cudaError_t bf16_backward(const gsa_delta_t& p, const DeltaMaps& m, const DeltaMaps& more,
+                          const DeltaGrads& g, void* saved, void* scratch, int* err,
+                          cudaStream_t stream) {
+  const Saved s = saved_at(p, saved);
+  const Scratch r = scratch_at(p, scratch);
+  const Table t = table_at(saved, p.N);
+  const SeqArgs a = {t, s.blocks, g.dout, g.dv, g.dfinal, g.dinitial, r.back, r.states, err};
+  const cudaError_t e = launch_seq(p, more, a, true, stream);
+  if (e != cudaSuccess) return e;
+  return launch_grad(p, m, more, g, s, r, t, err, stream);
+}
+
+}  // namespace delta
+}  // namespace gsa

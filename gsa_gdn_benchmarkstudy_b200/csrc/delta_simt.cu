@@ -1,6 +1,6 @@
 // delta_simt.cu — the chunked gated delta rule, forward and backward, on the
 // CUDA cores in fp32: fp32 inputs keep fp32's accuracy in every product, which
-// the tensor cores' 16-bit operands do not give (delta_mma.cu serves bf16).
+// the tensor cores' 16-bit operands do not give (delta_prep.cu, delta_seq.cu and delta_grad.cu serve bf16).
 //
 // Four kernels: `prep` makes T and P of every chunk, `chain` walks the chunks
 // of a sequence forwards, `rev` walks them backwards with the state's gradient,

@@ -275,18 +275,19 @@ cudaError_t simt_forward(const gsa_delta_t& p, void* o, float* final_state, bool
                          cudaStream_t stream);
 cudaError_t simt_backward(const gsa_delta_t& p, const DeltaGrads& g, void* saved, void* scratch,
                           cudaStream_t stream);
-// bf16 inputs.  Tensor maps {channel, head, token, batch}: boxes of 64 channels
-// x 64 tokens with 128-byte swizzle for q and k, 16 x 64 unswizzled for the
-// values (v, or dO in the backward pass; unset when there is no dO).
+// bf16 inputs.  Tensor maps {channel, head, token, batch} of q, k and the values
+// (v, or dO in `more`, whose v is unset when there is no dO): boxes of 64 channels x
+// 64 tokens with 128-byte swizzle.
 struct DeltaMaps {
   CUtensorMap q, k, v;
 };
-int64_t mma_saved_bytes(const gsa_delta_t& p, bool save);
-int64_t mma_scratch_bytes(const gsa_delta_t& p);
-cudaError_t mma_forward(const gsa_delta_t& p, const DeltaMaps& m, void* o, float* final_state,
-                        bool save, void* ws, int* err, cudaStream_t stream);
-cudaError_t mma_backward(const gsa_delta_t& p, const DeltaMaps& m, const DeltaGrads& g, void* saved,
-                         void* scratch, int* err, cudaStream_t stream);
+int64_t bf16_saved_bytes(const gsa_delta_t& p, bool save);
+int64_t bf16_scratch_bytes(const gsa_delta_t& p);
+cudaError_t bf16_forward(const gsa_delta_t& p, const DeltaMaps& m, void* o, float* final_state,
+                         bool save, void* ws, int* err, cudaStream_t stream);
+cudaError_t bf16_backward(const gsa_delta_t& p, const DeltaMaps& m, const DeltaMaps& more,
+                          const DeltaGrads& g, void* saved, void* scratch, int* err,
+                          cudaStream_t stream);
 }  // namespace delta
 
 cudaError_t launch_gather_attention(const void* q, int64_t q_stride, const void* k,
