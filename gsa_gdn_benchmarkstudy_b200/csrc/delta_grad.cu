@@ -70,6 +70,7 @@ struct GradArgs {
 struct Bars {
   uint64_t full_kq, empty_kq, full_h, empty_h;
   uint64_t ph1_full, ph2_ready, ph2_full, x_read, drain;
+  uint64_t meet;  // the computing warps, twice a head
   uint32_t tmem;
   int abort;
 };
@@ -86,11 +87,11 @@ __device__ __forceinline__ uint64_t desc_image(uint32_t image, int ks) {
 }
 // [K; Q] (or, from Q on, [Q; K]): 128 rows, channels 16 ks on contracted.
 __device__ __forceinline__ uint64_t desc_kq(uint32_t tile, int ks) {
-  return sdesc_sw128(tile + (ks >> 2) * kKqkBytes + (ks & 3) * 32, 16, 1024);
+  return desc_rows(tile, ks, kKqkBytes);
 }
 // K^T or Q^T: channels are the rows, tokens 16 ks on contracted.
 __device__ __forceinline__ uint64_t desc_kt(uint32_t tile, int ks) {
-  return sdesc_sw128(tile + ks * 2048, kKqkBytes, 1024);
+  return desc_cols(tile, ks, kKqkBytes);
 }
 
 // v[i] summed over the warp's lanes; lane l gets the sum of v[l].
@@ -106,9 +107,6 @@ __device__ __forceinline__ float fold_lanes(float (&v)[32]) {
     }
   }
   return v[0];
-}
-__device__ __forceinline__ void block_sync() {  // the computing warps
-  asm volatile("bar.sync 1, 256;" ::: "memory");
 }
 
 template <int DK>
@@ -290,7 +288,7 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
   const int group = p.Hv / p.Hk, rows = padded_dv(p.dv);
   const bool gate16 = p.gate_dtype == GSA_DTYPE_BF16;
   const int64_t qk_step = static_cast<int64_t>(p.Hk) * p.dk;
-  int items = 0, loads = 0, heads = 0;
+  int loads = 0, heads = 0;
   auto until = [&](uint64_t* bar, int parity) {
     const bool ok = mbar_wait_warp(bar, parity & 1, a.err, &bars.abort);
     tc_fence_after();
@@ -339,7 +337,8 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
           sum.left[lane + 32 * e] = decay_between(sum.d, kChunk - 1, lane + 32 * e);
         }
       }
-      block_sync();
+      signal(&bars.meet);
+      if (!until(&bars.meet, 2 * heads)) return;
       // <S0, dS1>
       float cross = 0.f;
       for (int col0 = 0; col0 < p.dv; col0 += 128, ++loads) {
@@ -455,7 +454,8 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
         sum.kn[quad][t0 + lane] = fold_lanes(e);
       }
       signal(&bars.ph2_ready);
-      block_sync();
+      signal(&bars.meet);
+      if (!until(&bars.meet, 2 * heads + 1)) return;
       if (warp == 0) {  // two neighbouring tokens a lane
         float rs[2], gs[2];
 #pragma unroll
@@ -507,7 +507,6 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
         gk[i] += __uint_as_float(u[i]);
       }
     }
-    ++items;
     if (row < p.dk) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
@@ -540,6 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars.ph2_ready, kComputeWarps);
     mbar_init(&bars.ph2_full, 1);
     mbar_init(&bars.x_read, kComputeWarps);
+    mbar_init(&bars.meet, kComputeWarps);
     mbar_init(&bars.drain, 1);
     fence_mbar_init();
   }

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t
       __syncthreads();
     }
     if (tid < kChunk) {
-      img->grown[tid] = img->grown_p[tid] = decay_from_start(d, tid);
+      img->grown[tid] = decay_from_start(d, tid);
       img->beta[tid] = d.beta[tid];
       img->left[tid] = decay_between(d, kChunk - 1, tid);
     }

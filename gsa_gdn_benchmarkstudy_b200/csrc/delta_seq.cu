@@ -29,46 +29,50 @@ constexpr int kThreads = 32 * (kComputeWarps + 2);
 constexpr int kCols = 128;  // state columns of a block: the lanes of tensor memory
 constexpr uint32_t kTmemCols = 512;
 
-// Tensor memory, 32-bit columns.
+// Tensor memory, 32-bit columns; b = 0, 1 in turn by chunk.  A product takes about
+// 62 cycles for 16 of the contraction whether its accumulator has 64 columns or
+// 128, so K and Q stand as one right operand of 128 rows (R and O come together),
+// and T_hi and T_lo too (two halves that the threads add).
 enum : uint32_t {
-  kAcc = 0,      // what a chunk adds to S^T [128][dk]
-  kShi = 128,    // S^T as a left operand (two values a column)
-  kSlo = 192,
-  kR = 256,      // R^T, then N^T (backwards dS^T K^T, then dY^T) [128][64]
-  kYhi = 320,    // Y^T, then N^T (backwards dN^T, then -e^c beta dY^T)
-  kYlo = 352,
-  kDhi = 384,    // (e^{c_64 - c} N)^T (backwards (scale e^c dO)^T)
-  kDlo = 416,
-  kO = 448,      // O^T (backwards dO^T P)
+  kAcc = 0,    // what a chunk adds to S^T [128][dk]; before that [Y T_hi | Y T_lo]^T
+  kS = 128,    // left operands, two values a column: S^T hi (64), lo (64); then, once
+               // R is there, Y^T (backwards dN^T, then -e^c beta dY^T) hi, lo (32 each)
+  kD = 192,    // and (e^{c_64 - c} N)^T (backwards (scale e^c dO)^T) hi, lo
+  kRO = 256,   // + 128 b: R^T (64), O^T (64); N^T hi, lo in R's place.  Backwards
+               // dS^T K^T and dO^T P, then [dN T_hi | dN T_lo]^T
 };
 
+constexpr uint32_t kKq = 2 * kTile;  // K and Q: 128 rows of 64 channels
 template <int DK>
-__host__ __device__ constexpr int tile_bytes() { return (DK / 64) * static_cast<int>(kTile); }
-template <int DK>
-__host__ __device__ constexpr int queue_bytes() { return tile_bytes<DK>() + kHalf; }
+__host__ __device__ constexpr int kq_bytes() { return (DK / 64) * static_cast<int>(kKq); }
 constexpr int kValueBytes = 2 * static_cast<int>(kTile);
+// Queue a: K and Q, T with the decays, 64 x 128 values (v, or dO); queue b: P.
+template <int DK>
+__host__ __device__ constexpr int a_bytes() { return kq_bytes<DK>() + kTBytes + kValueBytes; }
+// ... and 64 rows of 128 outputs on their way out.
+constexpr int kRowBytes = 256;
 template <int DK>
 __host__ __device__ constexpr int seq_smem() {
-  return kStages * (2 * queue_bytes<DK>() + kValueBytes) + 1024;
+  // values are swizzled tiles: they come before T, whose decays break the 1024 bytes
+  return kStages * (a_bytes<DK>() + kPBytes) + kChunk * kRowBytes + 1024;
 }
-
-// Queue a holds K, T and decays, queue b Q, P and decays; the 64 x 128 values (v
-// forwards, dO backwards) go with a forwards and with b backwards.
 template <int DK>
 struct Smem {
   unsigned char* base;
-  __device__ unsigned char* a(int st) const { return base + st * queue_bytes<DK>(); }
-  __device__ unsigned char* b(int st) const { return base + (kStages + st) * queue_bytes<DK>(); }
-  __device__ unsigned char* v(int st) const {
-    return base + 2 * kStages * queue_bytes<DK>() + st * kValueBytes;
+  __device__ unsigned char* a(int st) const { return base + st * a_bytes<DK>(); }
+  __device__ unsigned char* v(int st) const { return a(st) + kq_bytes<DK>(); }
+  __device__ unsigned char* t(int st) const { return v(st) + kValueBytes; }
+  __device__ unsigned char* p(int st) const {
+    return base + kStages * a_bytes<DK>() + st * kPBytes;
   }
+  __device__ unsigned char* out() const { return p(kStages); }
 };
 
 // Every barrier but the queues' completes once a chunk.
 struct Bars {
   uint64_t full_a[kStages], empty_a[kStages], full_b[kStages], empty_b[kStages];
-  uint64_t s_ready, r_full, y_ready, n_full, d_ready, upd_full;
-  uint64_t o1_full, o1_read, o_full;  // backwards o1_full: dO^T P
+  uint64_t s_ready, r_full, y_ready, z_ready, n_full, d_ready, upd_full, o_full;
+  uint64_t rows[2];  // a half's four warps have written their columns of the outputs
   uint64_t drain;
   uint32_t tmem;
   int abort;
@@ -105,53 +109,57 @@ __device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& m
     const int len = rest < kChunk ? rest : kChunk;
     const bool whole = len == kChunk || !p.cu_seqlens;
     const Block* blk = a.blocks + static_cast<int64_t>(s.chunk0 + at) * p.Hv + hv;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      uint64_t* full = q ? &bars.full_b[st] : &bars.full_a[st];
-      ok = ok && mbar_wait_warp(q ? &bars.empty_b[st] : &bars.empty_a[st], parity, a.err,
-                                &bars.abort);
-      if (!ok) break;
-      unsigned char* dst = q ? sm.b(st) : sm.a(st);
-      const bool values = (q == 1) == REV;
-      const bool tma_values = values && whole && have;
-      bool by_hand = false;
-      if (!whole) {
-        copy_rows(smem_u32(dst),
-                  q ? rows_at(p.q, p.q_stride, s.b, begin, hk)
-                    : rows_at(p.k, p.k_stride, s.b, begin, hk),
-                  q ? p.q_stride[1] : p.k_stride[1], len, DK, p.dk, lane, 32);
-        by_hand = true;
+    ok = mbar_wait_warp(&bars.empty_a[st], parity, a.err, &bars.abort);
+    if (!ok) break;
+    bool by_hand = false;
+    if (!whole) {
+      for (int i = 0; i < DK / 64; ++i) {
+        const uint32_t to = smem_u32(sm.a(st)) + i * kKq;
+        copy_rows(to, rows_at(p.k, p.k_stride, s.b, begin, hk) + 64 * i, p.k_stride[1], len, 64,
+                  p.dk - 64 * i, lane, 32);
+        copy_rows(to + kTile, rows_at(p.q, p.q_stride, s.b, begin, hk) + 64 * i, p.q_stride[1],
+                  len, 64, p.dk - 64 * i, lane, 32);
       }
-      if (values && !tma_values) {
-        const int64_t stride = REV ? static_cast<int64_t>(p.Hv) * p.dv : p.v_stride[1];
-        const bf16* v = REV ? static_cast<const bf16*>(a.in) +
-                                  (have ? (static_cast<int64_t>(s.b) * p.T + begin) * stride +
-                                              hv * p.dv
-                                        : 0)
-                            : rows_at(p.v, p.v_stride, s.b, begin, hv);
-        copy_rows(smem_u32(sm.v(st)), have ? v + col0 : static_cast<const bf16*>(p.k), stride,
-                  have ? len : 0, kCols, p.dv - col0, lane, 32);
-        by_hand = true;
-      }
-      if (by_hand) {  // the products read through the asynchronous proxy
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      if (lane == 0) {
-        mbar_arrive_expect_tx(full, kHalf + (whole ? tile_bytes<DK>() : 0) +
-                                        (tma_values ? kValueBytes : 0));
-        bulk_load(dst + tile_bytes<DK>(), reinterpret_cast<const unsigned char*>(blk) + q * kHalf,
-                  kHalf, full);
-        if (whole)
-          for (int i = 0; i < DK / 64; ++i)
-            tma_load_rows(dst + i * kTile, q ? &maps.q : &maps.k, 64 * i, hk, begin, s.b, full);
-        if (tma_values)
-          for (int i = 0; i < 2; ++i)
-            tma_load_rows(sm.v(st) + i * kTile, &maps.v, col0 + 64 * i, hv, begin, s.b, full);
-      }
-      ++begun[q];
+      by_hand = true;
     }
+    if (!whole || !have) {
+      const int64_t stride = REV ? static_cast<int64_t>(p.Hv) * p.dv : p.v_stride[1];
+      const bf16* v = REV ? static_cast<const bf16*>(a.in) +
+                                (have ? (static_cast<int64_t>(s.b) * p.T + begin) * stride +
+                                            hv * p.dv
+                                      : 0)
+                          : rows_at(p.v, p.v_stride, s.b, begin, hv);
+      copy_rows(smem_u32(sm.v(st)), have ? v + col0 : static_cast<const bf16*>(p.k), stride,
+                have ? len : 0, kCols, p.dv - col0, lane, 32);
+      by_hand = true;
+    }
+    if (by_hand) {  // the products read through the asynchronous proxy
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
+    if (lane == 0) {
+      uint64_t* full = &bars.full_a[st];
+      mbar_arrive_expect_tx(full, kTBytes + (whole ? kq_bytes<DK>() : 0) +
+                                      (whole && have ? kValueBytes : 0));
+      bulk_load(sm.t(st), blk, kTBytes, full);
+      if (whole)
+        for (int i = 0; i < DK / 64; ++i) {
+          tma_load_rows(sm.a(st) + i * kKq, &maps.k, 64 * i, hk, begin, s.b, full);
+          tma_load_rows(sm.a(st) + i * kKq + kTile, &maps.q, 64 * i, hk, begin, s.b, full);
+        }
+      if (whole && have)
+        for (int i = 0; i < 2; ++i)
+          tma_load_rows(sm.v(st) + i * kTile, &maps.v, col0 + 64 * i, hv, begin, s.b, full);
+    }
+    ++begun[0];
+    ok = mbar_wait_warp(&bars.empty_b[st], parity, a.err, &bars.abort);
+    if (!ok) break;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&bars.full_b[st], kPBytes);
+      bulk_load(sm.p(st), blk->p_hi, kPBytes, &bars.full_b[st]);
+    }
+    ++begun[1];
   }
   if (!ok) {  // gave up: no copy of ours may outlive the block
     for (int i = max(0, begun[0] - kStages); i < begun[0]; ++i)
@@ -161,26 +169,14 @@ __device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& m
   }
 }
 
-// acc (+)= (hi + lo) B over KS steps of 16; COLS: B's rows are contracted.
+// acc (+)= left B over KS steps of 16 of the contraction; COLS: B's rows are contracted.
 template <int KS, bool COLS>
-__device__ __forceinline__ void times(uint32_t acc, uint32_t hi, uint32_t lo, uint32_t tile,
+__device__ __forceinline__ void times(uint32_t acc, uint32_t left, uint32_t tile, uint32_t step,
                                       uint32_t idesc, bool fresh) {
 #pragma unroll
-  for (int half = 0; half < 2; ++half)
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      tc_mma_ts(acc, (half ? lo : hi) + 8 * ks, COLS ? desc_cols(tile, ks) : desc_rows(tile, ks),
-                idesc, !fresh || half || ks);
-}
-// acc (+)= (hi + lo) (M_hi + M_lo) without lo M_lo, M a pair of 64 x 64 tiles.
-template <bool COLS>
-__device__ __forceinline__ void times_pair(uint32_t acc, uint32_t hi, uint32_t lo, uint32_t tile,
-                                           uint32_t idesc, bool fresh) {
-  times<4, COLS>(acc, hi, lo, tile, idesc, fresh);
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks)
-    tc_mma_ts(acc, hi + 8 * ks, COLS ? desc_cols(tile + kTile, ks) : desc_rows(tile + kTile, ks),
-              idesc, 1);
+  for (int ks = 0; ks < KS; ++ks)
+    tc_mma_ts(acc, left + 8 * ks, COLS ? desc_cols(tile, ks, step) : desc_rows(tile, ks, step),
+              idesc, !fresh || ks);
 }
 
 // One thread issues all products.
@@ -189,9 +185,12 @@ __device__ __forceinline__ void issue(const SeqArgs& a, int chunks, const Smem<D
                                       Bars& bars) {
   const uint32_t tm = bars.tmem;
   constexpr uint32_t kRows64 = idesc_bf16_f32(128, 64, 0, 0);
+  constexpr uint32_t kRows128 = idesc_bf16_f32(128, 128, 0, 0);
   constexpr uint32_t kCols64 = idesc_bf16_f32(128, 64, 0, 1);
+  constexpr uint32_t kCols128 = idesc_bf16_f32(128, 128, 0, 1);
   constexpr uint32_t kColsDk = idesc_bf16_f32(128, DK, 0, 1);
   constexpr uint32_t kColsCols = idesc_bf16_f32(128, 64, 1, 1);
+  constexpr uint32_t kLo = DK / 2;  // from S's hi columns to its lo columns
   auto until = [&](uint64_t* bar, int parity) {
     if (!mbar_wait(bar, parity & 1, a.err, &bars.abort)) return false;
     tc_fence_after();
@@ -199,42 +198,52 @@ __device__ __forceinline__ void issue(const SeqArgs& a, int chunks, const Smem<D
   };
   for (int n = 0; n < chunks; ++n) {
     const int st = n % kStages, turn = n / kStages;
-    const uint32_t K = smem_u32(sm.a(st)), T = K + tile_bytes<DK>();
-    const uint32_t Q = smem_u32(sm.b(st)), P = Q + tile_bytes<DK>();
+    const uint32_t K = smem_u32(sm.a(st)), Q = K + kTile;
+    const uint32_t T = smem_u32(sm.t(st)), P = smem_u32(sm.p(st));
+    const uint32_t ro = tm + kRO + 128 * (n & 1);
+    if (!until(&bars.full_a[st], turn)) break;
     if constexpr (REV) {
       if (!until(&bars.full_b[st], turn)) break;
       const uint32_t D = smem_u32(sm.v(st));
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        tc_mma_ss(tm + kO, desc_cols(D, i & 3), desc_cols(P + (i >> 2) * kTile, i & 3), kColsCols,
+        tc_mma_ss(ro + 64, desc_cols(D, i & 3), desc_cols(P + (i >> 2) * kTile, i & 3), kColsCols,
                   i > 0);
-      tc_commit(&bars.o1_full);
-    }
-    if (!until(&bars.full_a[st], turn) || !until(&bars.s_ready, n)) break;
-    times<DK / 16, false>(tm + kR, tm + kShi, tm + kSlo, K, kRows64, true);
-    tc_commit(&bars.r_full);
-    if (!until(&bars.y_ready, n)) break;
-    if constexpr (REV) {
-      times_pair<true>(tm + kR, tm + kYhi, tm + kYlo, T, kCols64, true);
-      tc_commit(&bars.n_full);
-      times<4, true>(tm + kAcc, tm + kDhi, tm + kDlo, Q, kColsDk, true);
       tc_commit(&bars.empty_b[st]);
+      if (!until(&bars.s_ready, n)) break;
+      times<DK / 16, false>(ro, tm + kS, K, kKq, kRows64, true);
+      times<DK / 16, false>(ro, tm + kS + kLo, K, kKq, kRows64, false);
+      tc_commit(&bars.r_full);
+      if (!until(&bars.y_ready, n)) break;
+      times<4, true>(ro, tm + kS, T, kTile, kCols128, true);
+      times<4, true>(ro, tm + kS + 32, T, kTile, kCols64, false);
+      tc_commit(&bars.n_full);
+      if (!until(&bars.z_ready, n)) break;
+      times<4, true>(tm + kAcc, tm + kD, Q, kKq, kColsDk, true);
+      times<4, true>(tm + kAcc, tm + kD + 32, Q, kKq, kColsDk, false);
       if (!until(&bars.d_ready, n)) break;
-      times<4, true>(tm + kAcc, tm + kYhi, tm + kYlo, K, kColsDk, false);
+      times<4, true>(tm + kAcc, tm + kS, K, kKq, kColsDk, false);
+      times<4, true>(tm + kAcc, tm + kS + 32, K, kKq, kColsDk, false);
       tc_commit(&bars.upd_full);
       tc_commit(&bars.empty_a[st]);
     } else {
-      times_pair<false>(tm + kR, tm + kYhi, tm + kYlo, T, kRows64, true);
+      if (!until(&bars.s_ready, n)) break;
+      times<DK / 16, false>(ro, tm + kS, K, kKq, kRows128, true);
+      times<DK / 16, false>(ro, tm + kS + kLo, K, kKq, kRows128, false);
+      tc_commit(&bars.r_full);
+      if (!until(&bars.y_ready, n)) break;
+      times<4, false>(tm + kAcc, tm + kS, T, kTile, kRows128, true);
+      times<4, false>(tm + kAcc, tm + kS + 32, T, kTile, kRows64, false);
       tc_commit(&bars.n_full);
-      if (!until(&bars.full_b[st], turn)) break;
-      times<DK / 16, false>(tm + kO, tm + kShi, tm + kSlo, Q, kRows64, true);
-      tc_commit(&bars.o1_full);
       if (!until(&bars.d_ready, n)) break;
-      times<4, true>(tm + kAcc, tm + kDhi, tm + kDlo, K, kColsDk, true);
+      times<4, true>(tm + kAcc, tm + kD, K, kKq, kColsDk, true);
+      times<4, true>(tm + kAcc, tm + kD + 32, K, kKq, kColsDk, false);
       tc_commit(&bars.upd_full);
       tc_commit(&bars.empty_a[st]);
-      if (!until(&bars.o1_read, n)) break;
-      times_pair<false>(tm + kO, tm + kYhi, tm + kYlo, P, kRows64, false);
+      if (!until(&bars.full_b[st], turn)) break;
+      times<4, false>(ro + 64, ro, P, kTile, kRows64, false);
+      times<4, false>(ro + 64, ro + 32, P, kTile, kRows64, false);
+      times<4, false>(ro + 64, ro, P + kTile, kTile, kRows64, false);
       tc_commit(&bars.o_full);
       tc_commit(&bars.empty_b[st]);
     }
@@ -281,7 +290,12 @@ __device__ __forceinline__ void add_update(float (&S)[DK / 2], float whole, cons
     tmem_ld32(l.tmem + kAcc + l.half * (DK / 2) + 32 * q, r);
     tc_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) S[32 * q + i] = fmaf(whole, S[32 * q + i], __uint_as_float(r[i]));
+    for (int i = 0; i < 32; i += 2) {
+      const uint64_t x = f2_fma(f2_pack(whole, whole), f2_pack(S[32 * q + i], S[32 * q + i + 1]),
+                                f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+      S[32 * q + i] = f2_lo(x);
+      S[32 * q + i + 1] = f2_hi(x);
+    }
   }
 }
 // S as the left operand, and (image != nullptr) its upper half kept in bf16.
@@ -293,8 +307,8 @@ __device__ __forceinline__ void put_operand(const float (&S)[DK / 2], const Lane
     uint32_t hi[16], lo[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) split(S[32 * q + 2 * i], S[32 * q + 2 * i + 1], hi[i], lo[i]);
-    tmem_st16(l.tmem + kShi + l.half * (DK / 4) + 16 * q, hi);
-    tmem_st16(l.tmem + kSlo + l.half * (DK / 4) + 16 * q, lo);
+    tmem_st16(l.tmem + kS + l.half * (DK / 4) + 16 * q, hi);
+    tmem_st16(l.tmem + kS + DK / 2 + l.half * (DK / 4) + 16 * q, lo);
     if (image && l.col < rows)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -303,14 +317,14 @@ __device__ __forceinline__ void put_operand(const float (&S)[DK / 2], const Lane
             make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
   }
 }
-// 32 tokens of a left operand (hi at `at`, lo 32 columns behind).
+// 32 tokens of a left operand (hi at `at`, lo 32 columns behind); hi is handed back.
 __device__ __forceinline__ void put_tokens(const float (&x)[32], uint32_t at, const Lane& l,
                                            uint32_t (&hi)[16]) {
   uint32_t lo[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) split(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-  tmem_st16(l.tmem + at + 16 * l.half, hi);
-  tmem_st16(l.tmem + at + 32 + 16 * l.half, lo);
+  tmem_st16(at + 16 * l.half, hi);
+  tmem_st16(at + 32 + 16 * l.half, lo);
 }
 __device__ __forceinline__ void put_image(const uint32_t (&hi)[16], bf16* image, int rows,
                                           const Lane& l) {
@@ -320,20 +334,43 @@ __device__ __forceinline__ void put_image(const uint32_t (&hi)[16], bf16* image,
       *reinterpret_cast<uint4*>(image + (static_cast<int64_t>(4 * l.half + i) * rows + l.col) * 8) =
           make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
 }
-// This lane's value of token t in a 64 x 128 tile of values.
-__device__ __forceinline__ float value_at(const unsigned char* v, int t, const Lane& l) {
-  const uint32_t at = (l.row >> 6) * kTile + sw128_offset(t, (l.row & 63) >> 3) + 2 * (l.row & 7);
-  return __bfloat162float(*reinterpret_cast<const bf16*>(v + at));
-}
-// 32 tokens of this lane to rows of a contiguous [.., Hv, dv] tensor.
-__device__ __forceinline__ void put_rows(const float (&x)[32], bf16* dst, int64_t stride, int len,
-                                         int dv, const Lane& l) {
-  if (l.col >= dv) return;
+// This lane's values of its 32 tokens from two 64 x 64 tiles, as pairs of tokens.
+__device__ __forceinline__ void load_values(uint32_t (&x)[16], const unsigned char* v,
+                                            const Lane& l) {
+  v += (l.row >> 6) * kTile + 32 * l.half * 128 + 2 * (l.row & 7);
+  const int piece = (l.row & 63) >> 3;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const int t = 32 * l.half + i;
-    if (t < len) dst[t * stride] = __float2bfloat16_rn(x[i]);
+  for (int i = 0; i < 16; ++i)
+    x[i] = *reinterpret_cast<const uint16_t*>(v + sw128_offset(2 * i, piece)) |
+           (static_cast<uint32_t>(
+                *reinterpret_cast<const uint16_t*>(v + sw128_offset(2 * i + 1, piece)))
+            << 16);
+}
+// 32 tokens of this lane, as bf16 pairs of tokens, to rows of a contiguous [.., Hv,
+// dv] tensor (`dst`: first row, column 0 of the block), by way of shared memory: the
+// four warps of a half have whole rows of 128 columns between them.
+__device__ __forceinline__ bool put_rows(const uint32_t (&x)[16], unsigned char* out, bf16* dst,
+                                         int64_t stride, int len, int cols, const Lane& l, int n,
+                                         const SeqArgs& a, Bars& bars) {
+  unsigned char* at = out + 32 * l.half * kRowBytes + 2 * l.row;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    *reinterpret_cast<uint16_t*>(at + 2 * i * kRowBytes) = static_cast<uint16_t>(x[i]);
+    *reinterpret_cast<uint16_t*>(at + (2 * i + 1) * kRowBytes) =
+        static_cast<uint16_t>(x[i] >> 16);
   }
+  signal(&bars.rows[l.half]);
+  if (!wait(&bars.rows[l.half], n, a, bars)) return false;
+  const int piece = (l.row & 15) * 8, first = 32 * l.half + (l.row >> 4);
+  const unsigned char* from = out + first * kRowBytes + 2 * piece;
+  bf16* to = dst + first * stride + piece;
+  if (piece < cols)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (first + 8 * i < len)
+        *reinterpret_cast<uint4*>(to + 8 * i * stride) =
+            *reinterpret_cast<const uint4*>(from + 8 * i * kRowBytes);
+  return true;
 }
 
 template <int DK>
@@ -342,23 +379,25 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
   const int chunks = (s.len + kChunk - 1) / kChunk, rows = padded_dv(p.dv);
   const int64_t head = (static_cast<int64_t>(blockIdx.x) * p.Hv + hv) * p.dk * p.dv;
   const int64_t stride = static_cast<int64_t>(p.Hv) * p.dv;
+  const int col0 = l.col - l.row, cols = p.dv - col0, t0 = 32 * l.half;
   bf16* out = static_cast<bf16*>(a.out) +
-              ((static_cast<int64_t>(s.b) * p.T + s.begin) * p.Hv + hv) * p.dv + l.col;
+              ((static_cast<int64_t>(s.b) * p.T + s.begin) * p.Hv + hv) * p.dv + col0;
   auto finish = [&](int n) {  // O of chunk n
-    uint32_t r[32];
-    tmem_ld32(l.tmem + kO + 32 * l.half, r);
+    uint32_t r[32], x[16];
+    tmem_ld32(l.tmem + kRO + 128 * (n & 1) + 64 + t0, r);
     tc_wait_ld();
-    float x[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
-    put_rows(x, out + static_cast<int64_t>(n) * kChunk * stride, stride, s.len - n * kChunk, p.dv,
-             l);
+    for (int i = 0; i < 16; ++i)
+      x[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    return put_rows(x, sm.out(), out + static_cast<int64_t>(n) * kChunk * stride, stride,
+                    s.len - n * kChunk, cols, l, n, a, bars);
   };
   float S[DK / 2];
   load_state<DK>(S, a.state0 ? a.state0 + head : nullptr, p, l);
   float whole = 1.f;
   for (int n = 0; n < chunks; ++n) {
     const int st = n % kStages, turn = n / kStages;
+    const uint32_t ro = l.tmem + kRO + 128 * (n & 1);
     const int64_t slot = static_cast<int64_t>(s.chunk0 + n) * p.Hv + hv;
     if (n > 0) {
       if (!wait(&bars.upd_full, n - 1, a, bars)) return;
@@ -367,76 +406,72 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
     put_operand<DK>(S, l, a.states ? a.states + slot * DK * rows : nullptr, rows);
     tc_wait_st();
     signal(&bars.s_ready);
-    if (n > 0) {
+    if (n > 0) {  // beside this chunk's first product
       if (!wait(&bars.o_full, n - 1, a, bars)) return;
-      finish(n - 1);
+      if (!finish(n - 1)) return;
     }
     if (!wait(&bars.full_a[st], turn, a, bars)) return;
-    const Block* blk = reinterpret_cast<const Block*>(sm.a(st) + tile_bytes<DK>());
-    const unsigned char* v = sm.v(st);
+    const Block* blk = reinterpret_cast<const Block*>(sm.t(st));
     float y[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) y[i] = value_at(v, 32 * l.half + i, l);
+    uint32_t r[32], u[32], hi[16];
+    load_values(hi, sm.v(st), l);
     if (!wait(&bars.r_full, n, a, bars)) return;
-    uint32_t r[32], hi[16];
-    tmem_ld32(l.tmem + kR + 32 * l.half, r);
+    tmem_ld32(ro + t0, r);
     tc_wait_ld();
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(blk->grown + 32 * l.half + i);
-      const float4 b = *reinterpret_cast<const float4*>(blk->beta + 32 * l.half + i);
-      y[i] = b.x * fmaf(-g.x, __uint_as_float(r[i]), y[i]);
-      y[i + 1] = b.y * fmaf(-g.y, __uint_as_float(r[i + 1]), y[i + 1]);
-      y[i + 2] = b.z * fmaf(-g.z, __uint_as_float(r[i + 2]), y[i + 2]);
-      y[i + 3] = b.w * fmaf(-g.w, __uint_as_float(r[i + 3]), y[i + 3]);
+      const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
+      const float4 b = *reinterpret_cast<const float4*>(blk->beta + t0 + i);
+      const uint32_t v0 = hi[i / 2], v1 = hi[i / 2 + 1];
+      y[i] = b.x * fmaf(-g.x, __uint_as_float(r[i]), lo_of(v0));
+      y[i + 1] = b.y * fmaf(-g.y, __uint_as_float(r[i + 1]), hi_of(v0));
+      y[i + 2] = b.z * fmaf(-g.z, __uint_as_float(r[i + 2]), lo_of(v1));
+      y[i + 3] = b.w * fmaf(-g.w, __uint_as_float(r[i + 3]), hi_of(v1));
     }
-    put_tokens(y, kYhi, l, hi);
+    put_tokens(y, l.tmem + kS, l, hi);
     tc_wait_st();
     signal(&bars.y_ready);
     whole = blk->grown[kChunk - 1];
-    if (!wait(&bars.n_full, n, a, bars)) return;
-    tmem_ld32(l.tmem + kR + 32 * l.half, r);
+    // beside the product with T: O's part from the state gets its decays
+    tmem_ld32(ro + 64 + t0, r);
     tc_wait_ld();
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(blk->left + 32 * l.half + i);
-      y[i] = g.x * __uint_as_float(r[i]);
-      y[i + 1] = g.y * __uint_as_float(r[i + 1]);
-      y[i + 2] = g.z * __uint_as_float(r[i + 2]);
-      y[i + 3] = g.w * __uint_as_float(r[i + 3]);
-    }
-    put_tokens(y, kDhi, l, hi);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(r[i]);
-    put_tokens(y, kYhi, l, hi);
-    tc_wait_st();
-    signal(&bars.d_ready);
-    if (a.rows) put_image(hi, a.rows + slot * kChunk * rows, rows, l);
-    signal(&bars.empty_a[st]);
-    if (!wait(&bars.full_b[st], turn, a, bars)) return;
-    const float* grown =
-        reinterpret_cast<const float*>(sm.b(st) + tile_bytes<DK>() + 2 * kTile) + 32 * l.half;
-    if (!wait(&bars.o1_full, n, a, bars)) return;
-    tmem_ld32(l.tmem + kO + 32 * l.half, r);
-    tc_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(grown + i);
+      const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
       r[i] = __float_as_uint(p.scale * g.x * __uint_as_float(r[i]));
       r[i + 1] = __float_as_uint(p.scale * g.y * __uint_as_float(r[i + 1]));
       r[i + 2] = __float_as_uint(p.scale * g.z * __uint_as_float(r[i + 2]));
       r[i + 3] = __float_as_uint(p.scale * g.w * __uint_as_float(r[i + 3]));
     }
-    tmem_st32(l.tmem + kO + 32 * l.half, r);
+    tmem_st32(ro + 64 + t0, r);
+    if (!wait(&bars.n_full, n, a, bars)) return;
+    tmem_ld32(l.tmem + kAcc + t0, r);
+    tmem_ld32(l.tmem + kAcc + 64 + t0, u);
+    tc_wait_ld();
+    float x[32];
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float4 g = *reinterpret_cast<const float4*>(blk->left + t0 + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[i + e] = __uint_as_float(r[i + e]) + __uint_as_float(u[i + e]);
+      y[i] = g.x * x[i];
+      y[i + 1] = g.y * x[i + 1];
+      y[i + 2] = g.z * x[i + 2];
+      y[i + 3] = g.w * x[i + 3];
+    }
+    put_tokens(y, l.tmem + kD, l, hi);
+    put_tokens(x, ro, l, hi);
     tc_wait_st();
-    signal(&bars.o1_read);
-    signal(&bars.empty_b[st]);
+    signal(&bars.d_ready);
+    signal(&bars.empty_a[st]);
+    if (a.rows) put_image(hi, a.rows + slot * kChunk * rows, rows, l);
   }
   if (chunks > 0) {
     if (!wait(&bars.upd_full, chunks - 1, a, bars)) return;
     add_update<DK>(S, whole, l);
     if (!wait(&bars.o_full, chunks - 1, a, bars)) return;
-    finish(chunks - 1);
+    if (!finish(chunks - 1)) return;
   }
   if (a.state1) store_state<DK>(S, a.state1 + head, p, l);
 }
@@ -449,13 +484,15 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
   const int chunks = (s.len + kChunk - 1) / kChunk, rows = padded_dv(p.dv);
   const int64_t head = (static_cast<int64_t>(blockIdx.x) * p.Hv + hv) * p.dk * p.dv;
   const int64_t stride = static_cast<int64_t>(p.Hv) * p.dv;
+  const int col0 = l.col - l.row, cols = p.dv - col0, t0 = 32 * l.half;
   bf16* out = static_cast<bf16*>(a.out) +
-              ((static_cast<int64_t>(s.b) * p.T + s.begin) * p.Hv + hv) * p.dv + l.col;
+              ((static_cast<int64_t>(s.b) * p.T + s.begin) * p.Hv + hv) * p.dv + col0;
   float S[DK / 2];
   load_state<DK>(S, a.state0 ? a.state0 + head : nullptr, p, l);
   float whole = 1.f;
   for (int n = 0; n < chunks; ++n) {
     const int st = n % kStages, turn = n / kStages, at = chunks - 1 - n;
+    const uint32_t ro = l.tmem + kRO + 128 * (n & 1);
     const int64_t slot = static_cast<int64_t>(s.chunk0 + at) * p.Hv + hv;
     if (n > 0) {
       if (!wait(&bars.upd_full, n - 1, a, bars)) return;
@@ -464,76 +501,70 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
     put_operand<DK>(S, l, a.states + slot * DK * rows, rows);
     tc_wait_st();
     signal(&bars.s_ready);
-    if (!wait(&bars.full_b[st], turn, a, bars)) return;
-    float y[32];
-    uint32_t r[32], hi[16];
-    {
-      const unsigned char* v = sm.v(st);
-      const float* grown =
-          reinterpret_cast<const float*>(sm.b(st) + tile_bytes<DK>() + 2 * kTile) + 32 * l.half;
-#pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        const float4 g = *reinterpret_cast<const float4*>(grown + i);
-        y[i] = p.scale * g.x * value_at(v, 32 * l.half + i, l);
-        y[i + 1] = p.scale * g.y * value_at(v, 32 * l.half + i + 1, l);
-        y[i + 2] = p.scale * g.z * value_at(v, 32 * l.half + i + 2, l);
-        y[i + 3] = p.scale * g.w * value_at(v, 32 * l.half + i + 3, l);
-      }
-      put_tokens(y, kDhi, l, hi);
-      signal(&bars.empty_b[st]);
-    }
     if (!wait(&bars.full_a[st], turn, a, bars)) return;
-    const Block* blk = reinterpret_cast<const Block*>(sm.a(st) + tile_bytes<DK>());
-    if (!wait(&bars.o1_full, n, a, bars)) return;
-    tmem_ld32(l.tmem + kO + 32 * l.half, r);
-    tc_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(r[i]);
+    const Block* blk = reinterpret_cast<const Block*>(sm.t(st));
+    float y[32];
+    uint32_t r[32], u[32], hi[16], d[16];
+    load_values(d, sm.v(st), l);
     if (!wait(&bars.r_full, n, a, bars)) return;
-    tmem_ld32(l.tmem + kR + 32 * l.half, r);
+    tmem_ld32(ro + t0, r);
+    tmem_ld32(ro + 64 + t0, u);
     tc_wait_ld();
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(blk->left + 32 * l.half + i);
-      y[i] = fmaf(g.x, __uint_as_float(r[i]), y[i]);
-      y[i + 1] = fmaf(g.y, __uint_as_float(r[i + 1]), y[i + 1]);
-      y[i + 2] = fmaf(g.z, __uint_as_float(r[i + 2]), y[i + 2]);
-      y[i + 3] = fmaf(g.w, __uint_as_float(r[i + 3]), y[i + 3]);
+      const float4 g = *reinterpret_cast<const float4*>(blk->left + t0 + i);
+      y[i] = fmaf(g.x, __uint_as_float(r[i]), __uint_as_float(u[i]));
+      y[i + 1] = fmaf(g.y, __uint_as_float(r[i + 1]), __uint_as_float(u[i + 1]));
+      y[i + 2] = fmaf(g.z, __uint_as_float(r[i + 2]), __uint_as_float(u[i + 2]));
+      y[i + 3] = fmaf(g.w, __uint_as_float(r[i + 3]), __uint_as_float(u[i + 3]));
     }
-    put_tokens(y, kYhi, l, hi);
+    put_tokens(y, l.tmem + kS, l, hi);
     tc_wait_st();
     signal(&bars.y_ready);
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {  // beside the product with T
+      const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
+      y[i] = p.scale * g.x * lo_of(d[i / 2]);
+      y[i + 1] = p.scale * g.y * hi_of(d[i / 2]);
+      y[i + 2] = p.scale * g.z * lo_of(d[i / 2 + 1]);
+      y[i + 3] = p.scale * g.w * hi_of(d[i / 2 + 1]);
+    }
+    put_tokens(y, l.tmem + kD, l, hi);
+    tc_wait_st();
+    signal(&bars.z_ready);
     whole = blk->grown[kChunk - 1];
     if (!wait(&bars.n_full, n, a, bars)) return;
-    tmem_ld32(l.tmem + kR + 32 * l.half, r);
+    tmem_ld32(ro + t0, r);
+    tmem_ld32(ro + 64 + t0, u);
     tc_wait_ld();
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(blk->grown + 32 * l.half + i);
-      const float4 b = *reinterpret_cast<const float4*>(blk->beta + 32 * l.half + i);
-      y[i] = -g.x * b.x * __uint_as_float(r[i]);
-      y[i + 1] = -g.y * b.y * __uint_as_float(r[i + 1]);
-      y[i + 2] = -g.z * b.z * __uint_as_float(r[i + 2]);
-      y[i + 3] = -g.w * b.w * __uint_as_float(r[i + 3]);
+      const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
+      const float4 b = *reinterpret_cast<const float4*>(blk->beta + t0 + i);
+      const float ge[4] = {g.x, g.y, g.z, g.w}, be[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __uint_as_float(r[i + e]) + __uint_as_float(u[i + e]);
+        const float v = be[e] * x;
+        y[i + e] = -ge[e] * v;
+        r[i + e] = __float_as_uint(x);  // dY
+        u[i + e] = __float_as_uint(v);  // dV
+      }
     }
-    put_tokens(y, kYhi, l, hi);
+    put_tokens(y, l.tmem + kS, l, hi);
     tc_wait_st();
     signal(&bars.d_ready);
+    signal(&bars.empty_a[st]);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       hi[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
     put_image(hi, a.rows + slot * kChunk * rows, rows, l);
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 b = *reinterpret_cast<const float4*>(blk->beta + 32 * l.half + i);
-      y[i] = b.x * __uint_as_float(r[i]);
-      y[i + 1] = b.y * __uint_as_float(r[i + 1]);
-      y[i + 2] = b.z * __uint_as_float(r[i + 2]);
-      y[i + 3] = b.w * __uint_as_float(r[i + 3]);
-    }
-    signal(&bars.empty_a[st]);
-    put_rows(y, out + static_cast<int64_t>(at) * kChunk * stride, stride, s.len - at * kChunk, p.dv,
-             l);
+    for (int i = 0; i < 16; ++i)
+      hi[i] = pack_bf16x2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+    if (!put_rows(hi, sm.out(), out + static_cast<int64_t>(at) * kChunk * stride, stride,
+                  s.len - at * kChunk, cols, l, n, a, bars))
+      return;
   }
   if (chunks > 0) {
     if (!wait(&bars.upd_full, chunks - 1, a, bars)) return;
@@ -566,16 +597,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars.full_a[i], 1);
       mbar_init(&bars.full_b[i], 1);
       mbar_init(&bars.empty_a[i], 1 + kComputeWarps);
-      mbar_init(&bars.empty_b[i], 1 + kComputeWarps);
+      mbar_init(&bars.empty_b[i], 1);
     }
     mbar_init(&bars.s_ready, kComputeWarps);
     mbar_init(&bars.y_ready, kComputeWarps);
+    mbar_init(&bars.z_ready, kComputeWarps);
     mbar_init(&bars.d_ready, kComputeWarps);
-    mbar_init(&bars.o1_read, kComputeWarps);
+    mbar_init(&bars.rows[0], kComputeWarps / 2);
+    mbar_init(&bars.rows[1], kComputeWarps / 2);
     mbar_init(&bars.r_full, 1);
     mbar_init(&bars.n_full, 1);
     mbar_init(&bars.upd_full, 1);
-    mbar_init(&bars.o1_full, 1);
     mbar_init(&bars.o_full, 1);
     mbar_init(&bars.drain, 1);
     fence_mbar_init();

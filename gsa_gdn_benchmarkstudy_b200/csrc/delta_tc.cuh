@@ -34,21 +34,22 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
-// A tile whose rows are the outer dimension (M or N) and whose columns are
-// contracted: columns 16 ks .. 16 ks + 15.
-__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int ks) {
-  return sdesc_sw128(tile + (ks >> 2) * kTile + (ks & 3) * 32, 16, 1024);
+// Tiles of `step` bytes for 64 columns.  Rows are the outer dimension (M or N) and
+// columns contracted: columns 16 ks .. 16 ks + 15.
+__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int ks, uint32_t step = kTile) {
+  return sdesc_sw128(tile + (ks >> 2) * step + (ks & 3) * 32, 16, 1024);
 }
-// A tile whose rows are contracted and whose columns are the outer dimension:
-// rows 16 ks .. 16 ks + 15, all columns of all tiles.
-__device__ __forceinline__ uint64_t desc_cols(uint32_t tile, int ks) {
-  return sdesc_sw128(tile + ks * 2048, kTile, 1024);
+// Rows are contracted and columns are the outer dimension: rows 16 ks .. 16 ks + 15.
+__device__ __forceinline__ uint64_t desc_cols(uint32_t tile, int ks, uint32_t step = kTile) {
+  return sdesc_sw128(tile + ks * 2048, step, 1024);
 }
 
 // x, y as hi + lo pairs of bf16.
 __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = pack_bf16x2(x, y);
-  lo = pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
+  const uint64_t rest = f2_fma((static_cast<uint64_t>(hi & 0xFFFF0000u) << 32) | (hi << 16),
+                               f2_pack(-1.f, -1.f), f2_pack(x, y));
+  lo = pack_bf16x2(f2_lo(rest), f2_hi(rest));
 }
 __device__ __forceinline__ float lo_of(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float hi_of(uint32_t r) { return __uint_as_float(r & 0xFFFF0000u); }
@@ -65,12 +66,13 @@ __device__ __forceinline__ const bf16* rows_at(const void* base, const int64_t (
 // 64 rows of `width` (<= limit real) columns into swizzled tiles, zeros past
 // `len` and `limit`; by `threads` threads from thread `t` on.
 __device__ __forceinline__ void copy_rows(uint32_t dst, const bf16* src, int64_t stride, int len,
-                                          int width, int limit, int t, int threads) {
+                                          int width, int limit, int t, int threads,
+                                          uint32_t step = kTile) {
   const int pieces = width >> 3;
   for (int i = t; i < kChunk * pieces; i += threads) {
     const int r = i / pieces, c = i % pieces;
     const bool real = r < len && c * 8 < limit;
-    cp16(dst + (c >> 3) * kTile + sw128_offset(r, c & 7), real ? src + r * stride + c * 8 : src,
+    cp16(dst + (c >> 3) * step + sw128_offset(r, c & 7), real ? src + r * stride + c * 8 : src,
          real);
   }
 }
@@ -91,13 +93,12 @@ struct __align__(16) Block {
   float grown[kChunk];  // e^{c_i}
   float beta[kChunk];
   float left[kChunk];   // e^{c_64 - c_i}
-  float pad0[kChunk];
+  float pad[kChunk];
   unsigned char p_hi[kTile], p_lo[kTile];
-  float grown_p[kChunk];
-  float pad1[3 * kChunk];
 };
-constexpr int kHalf = 2 * static_cast<int>(kTile) + 1024;
-static_assert(sizeof(Block) == 2 * kHalf, "block");
+constexpr int kTBytes = 2 * static_cast<int>(kTile) + 1024;  // T and the decays
+constexpr int kPBytes = 2 * static_cast<int>(kTile);
+static_assert(sizeof(Block) == kTBytes + kPBytes, "block");
 
 __host__ __device__ inline int padded_dk(int dk) { return dk <= 64 ? 64 : 128; }
 // Rows of the images below: the value columns, rounded up to whole tiles.
