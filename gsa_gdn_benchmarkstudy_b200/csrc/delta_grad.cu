@@ -368,7 +368,7 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
       uint32_t r[32], u[32];
       tmem_ld32(tm + (first ? kPd : kPn) + t0, r);
       tmem_ld32(tm + (first ? kKq : kKk) + t0, u);
-      tc_wait_ld();
+      tc_wait_ld(r, u);
       {
         float e[32], own_sum = 0.f, low = 0.f;
         uint32_t packed[16];
@@ -406,7 +406,7 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
           sum.col_m[quad - 2][t0 + lane] = across;
           sum.low[half][own] = low;
           tmem_ld32(tm + kPv + t0, r);
-          tc_wait_ld();
+          tc_wait_ld(r);
           float diag = 0.f;
 #pragma unroll
           for (int i = 0; i < 32; ++i) diag = own == t0 + i ? __uint_as_float(r[i]) : diag;
@@ -421,7 +421,7 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
         const bool real = row < DK;
         float e[32];
         tmem_ld32(tm + kTo + t0, r);
-        tc_wait_ld();
+        tc_wait_ld(r);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const float v = real ? __uint_as_float(r[i]) : 0.f;
@@ -433,7 +433,7 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
         sum.qo[quad][t0 + lane] = fold_lanes(e);
         tmem_ld32(tm + kTy + t0, r);
         tmem_ld32(tm + kTn + t0, u);
-        tc_wait_ld();
+        tc_wait_ld(r, u);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const float v = real ? __uint_as_float(r[i]) : 0.f;
@@ -499,7 +499,7 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
       if (!until(&bars.ph2_full, heads)) return;
       tmem_ld32(tm + kPd + t0, r);
       tmem_ld32(tm + kPn + t0, u);
-      tc_wait_ld();
+      tc_wait_ld(r, u);
       signal(&bars.x_read);
 #pragma unroll
       for (int i = 0; i < 32; ++i) {

@@ -178,8 +178,10 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t
       __syncthreads();
     }
     if (tid < kChunk) {
-      img->grown[tid] = decay_from_start(d, tid);
+      const float grown = decay_from_start(d, tid);
+      img->grown[tid] = grown;
       img->beta[tid] = d.beta[tid];
+      img->both[tid] = d.beta[tid] * grown;
       img->left[tid] = decay_between(d, kChunk - 1, tid);
     }
 #pragma unroll

@@ -9,7 +9,7 @@
 // stays in fp32 in registers; between two products the threads read an
 // accumulator, do its element-wise part, and store the next left operand back to
 // tensor memory, where the product takes it from: no operand made here passes
-// through shared memory.  K, Q, V, T and P arrive by TMA, two chunks ahead.
+// through shared memory.  Four more warps take the outputs away, off that path.  K, Q, V, T and P arrive by TMA, two chunks ahead.
 //
 // Left operands are pairs hi + lo of bf16 (2^-17 of a value together), q, k, v
 // exact in bf16 and T, P pairs, so the state keeps about fp32's accuracy over
@@ -25,7 +25,13 @@ namespace {
 
 constexpr int kStages = 2;
 constexpr int kComputeWarps = 8;
-constexpr int kThreads = 32 * (kComputeWarps + 2);
+constexpr int kRowWarps = 4;
+constexpr int kIssueWarp = kComputeWarps + kRowWarps;
+constexpr int kCopyWarp = kIssueWarp + 1;
+constexpr int kThreads = 512;  // whole warpgroups: two warps idle
+// Registers: 512 x 128 at launch = 256 x 168 (computing) + 256 x 88 (the others).
+constexpr int kLaunchRegs = 128, kComputeRegs = 168, kOtherRegs = 88;
+static_assert(256 * kComputeRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
 constexpr int kCols = 128;  // state columns of a block: the lanes of tensor memory
 constexpr uint32_t kTmemCols = 512;
 
@@ -71,8 +77,11 @@ struct Smem {
 // Every barrier but the queues' completes once a chunk.
 struct Bars {
   uint64_t full_a[kStages], empty_a[kStages], full_b[kStages], empty_b[kStages];
-  uint64_t s_ready, r_full, y_ready, z_ready, n_full, d_ready, upd_full, o_full;
-  uint64_t rows[2];  // a half's four warps have written their columns of the outputs
+  uint64_t s_ready, r_full, y_ready, n_full, d_ready, upd_full, o_full;
+  uint64_t z_ready;  // forwards O's first part has its decays; backwards dO is an operand
+  uint64_t x_ready;  // forwards N is an operand
+  uint64_t o_read;   // the row warps are through with a chunk's accumulators
+  uint64_t rows;     // ... and have written their columns of its output rows
   uint64_t drain;
   uint32_t tmem;
   int abort;
@@ -169,14 +178,17 @@ __device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& m
   }
 }
 
-// acc (+)= left B over KS steps of 16 of the contraction; COLS: B's rows are contracted.
+// acc (+)= left B over KS steps of 16 of the contraction; B's first step has the
+// descriptor `b`, the next ones lie COLS ? 2048 : 32 bytes on (and `step` bytes
+// after every fourth, where 64 columns end).
 template <int KS, bool COLS>
-__device__ __forceinline__ void times(uint32_t acc, uint32_t left, uint32_t tile, uint32_t step,
+__device__ __forceinline__ void times(uint32_t acc, uint32_t left, uint64_t b, uint32_t step,
                                       uint32_t idesc, bool fresh) {
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
-    tc_mma_ts(acc, left + 8 * ks, COLS ? desc_cols(tile, ks, step) : desc_rows(tile, ks, step),
-              idesc, !fresh || ks);
+  for (int ks = 0; ks < KS; ++ks) {
+    const uint32_t off = COLS ? ks * 2048 : (ks >> 2) * step + (ks & 3) * 32;
+    tc_mma_ts(acc, left + 8 * ks, b + (off >> 4), idesc, !fresh || ks);
+  }
 }
 
 // One thread issues all products.
@@ -191,61 +203,72 @@ __device__ __forceinline__ void issue(const SeqArgs& a, int chunks, const Smem<D
   constexpr uint32_t kColsDk = idesc_bf16_f32(128, DK, 0, 1);
   constexpr uint32_t kColsCols = idesc_bf16_f32(128, 64, 1, 1);
   constexpr uint32_t kLo = DK / 2;  // from S's hi columns to its lo columns
+  // descriptors of stage 0; a stage is a_bytes (P: kPBytes) further
+  const uint64_t k_rows = desc_rows(smem_u32(sm.a(0)), 0);
+  const uint64_t k_cols = desc_cols(smem_u32(sm.a(0)), 0, kKq);
+  const uint64_t v_cols = desc_cols(smem_u32(sm.v(0)), 0);
+  const uint64_t t_rows = desc_rows(smem_u32(sm.t(0)), 0), t_cols = desc_cols(smem_u32(sm.t(0)), 0);
+  const uint64_t p_rows = desc_rows(smem_u32(sm.p(0)), 0), p_cols = desc_cols(smem_u32(sm.p(0)), 0);
   auto until = [&](uint64_t* bar, int parity) {
     if (!mbar_wait(bar, parity & 1, a.err, &bars.abort)) return false;
     tc_fence_after();
     return true;
   };
   for (int n = 0; n < chunks; ++n) {
-    const int st = n % kStages, turn = n / kStages;
-    const uint32_t K = smem_u32(sm.a(st)), Q = K + kTile;
-    const uint32_t T = smem_u32(sm.t(st)), P = smem_u32(sm.p(st));
-    const uint32_t ro = tm + kRO + 128 * (n & 1);
+    const int st = n & 1, turn = n >> 1;
+    static_assert(kStages == 2, "two stages");
+    const uint32_t da = st * (a_bytes<DK>() >> 4), dp = st * (kPBytes >> 4);
+    const uint32_t ro = tm + kRO + 128 * st;
     if (!until(&bars.full_a[st], turn)) break;
     if constexpr (REV) {
       if (!until(&bars.full_b[st], turn)) break;
-      const uint32_t D = smem_u32(sm.v(st));
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        tc_mma_ss(ro + 64, desc_cols(D, i & 3), desc_cols(P + (i >> 2) * kTile, i & 3), kColsCols,
-                  i > 0);
+        tc_mma_ss(ro + 64, v_cols + da + (i & 3) * 128, p_cols + dp + (i >> 2) * (kTile >> 4) +
+                  (i & 3) * 128, kColsCols, i > 0);
       tc_commit(&bars.empty_b[st]);
       if (!until(&bars.s_ready, n)) break;
-      times<DK / 16, false>(ro, tm + kS, K, kKq, kRows64, true);
-      times<DK / 16, false>(ro, tm + kS + kLo, K, kKq, kRows64, false);
+      times<DK / 16, false>(ro, tm + kS, k_rows + da, kKq, kRows64, true);
+      times<DK / 16, false>(ro, tm + kS + kLo, k_rows + da, kKq, kRows64, false);
       tc_commit(&bars.r_full);
       if (!until(&bars.y_ready, n)) break;
-      times<4, true>(ro, tm + kS, T, kTile, kCols128, true);
-      times<4, true>(ro, tm + kS + 32, T, kTile, kCols64, false);
+      // the row warps have left the last chunk: its accumulators are the next one's, and
+      // no barrier they wait for runs ahead of them by two
+      if (n > 0 && !until(&bars.o_read, n - 1)) break;
+      times<4, true>(ro, tm + kS, t_cols + da, kTile, kCols128, true);
+      times<4, true>(ro, tm + kS + 32, t_cols + da, kTile, kCols64, false);
       tc_commit(&bars.n_full);
       if (!until(&bars.z_ready, n)) break;
-      times<4, true>(tm + kAcc, tm + kD, Q, kKq, kColsDk, true);
-      times<4, true>(tm + kAcc, tm + kD + 32, Q, kKq, kColsDk, false);
+      const uint64_t q_cols = k_cols + (kTile >> 4);
+      times<4, true>(tm + kAcc, tm + kD, q_cols + da, kKq, kColsDk, true);
+      times<4, true>(tm + kAcc, tm + kD + 32, q_cols + da, kKq, kColsDk, false);
       if (!until(&bars.d_ready, n)) break;
-      times<4, true>(tm + kAcc, tm + kS, K, kKq, kColsDk, false);
-      times<4, true>(tm + kAcc, tm + kS + 32, K, kKq, kColsDk, false);
+      times<4, true>(tm + kAcc, tm + kS, k_cols + da, kKq, kColsDk, false);
+      times<4, true>(tm + kAcc, tm + kS + 32, k_cols + da, kKq, kColsDk, false);
       tc_commit(&bars.upd_full);
       tc_commit(&bars.empty_a[st]);
     } else {
       if (!until(&bars.s_ready, n)) break;
-      times<DK / 16, false>(ro, tm + kS, K, kKq, kRows128, true);
-      times<DK / 16, false>(ro, tm + kS + kLo, K, kKq, kRows128, false);
+      times<DK / 16, false>(ro, tm + kS, k_rows + da, kKq, kRows128, true);
+      times<DK / 16, false>(ro, tm + kS + kLo, k_rows + da, kKq, kRows128, false);
       tc_commit(&bars.r_full);
       if (!until(&bars.y_ready, n)) break;
-      times<4, false>(tm + kAcc, tm + kS, T, kTile, kRows128, true);
-      times<4, false>(tm + kAcc, tm + kS + 32, T, kTile, kRows64, false);
+      times<4, false>(tm + kAcc, tm + kS, t_rows + da, kTile, kRows128, true);
+      times<4, false>(tm + kAcc, tm + kS + 32, t_rows + da, kTile, kRows64, false);
       tc_commit(&bars.n_full);
       if (!until(&bars.d_ready, n)) break;
-      times<4, true>(tm + kAcc, tm + kD, K, kKq, kColsDk, true);
-      times<4, true>(tm + kAcc, tm + kD + 32, K, kKq, kColsDk, false);
+      times<4, true>(tm + kAcc, tm + kD, k_cols + da, kKq, kColsDk, true);
+      times<4, true>(tm + kAcc, tm + kD + 32, k_cols + da, kKq, kColsDk, false);
       tc_commit(&bars.upd_full);
       tc_commit(&bars.empty_a[st]);
-      if (!until(&bars.full_b[st], turn)) break;
-      times<4, false>(ro + 64, ro, P, kTile, kRows64, false);
-      times<4, false>(ro + 64, ro + 32, P, kTile, kRows64, false);
-      times<4, false>(ro + 64, ro, P + kTile, kTile, kRows64, false);
+      if (!until(&bars.full_b[st], turn) || !until(&bars.z_ready, n) || !until(&bars.x_ready, n))
+        break;
+      times<4, false>(ro + 64, ro, p_rows + dp, kTile, kRows64, false);
+      times<4, false>(ro + 64, ro + 32, p_rows + dp, kTile, kRows64, false);
+      times<4, false>(ro + 64, ro, p_rows + dp + (kTile >> 4), kTile, kRows64, false);
       tc_commit(&bars.o_full);
       tc_commit(&bars.empty_b[st]);
+      if (n > 0 && !until(&bars.o_read, n - 1)) break;
     }
   }
   // nothing of ours may be in flight when tensor memory is freed
@@ -253,7 +276,7 @@ __device__ __forceinline__ void issue(const SeqArgs& a, int chunks, const Smem<D
   mbar_wait_drain(&bars.drain, 0, kWaitLimitCycles);
 }
 
-// What a thread is: half `half` of column `col` of the value head.
+// What a computing thread is: half `half` of column `col` of the value head.
 struct Lane {
   int row;        // lane of tensor memory, 0 .. 127
   int half;       // which half of the channels, and of the tokens
@@ -281,18 +304,20 @@ __device__ __forceinline__ void store_state(const float (&S)[DK / 2], float* sta
     if (r < p.dk && l.col < p.dv) state[static_cast<int64_t>(r) * p.dv + l.col] = S[i];
   }
 }
-// S <- whole S + what the last chunk added.
+// S <- whole S + what the last chunk added.  All loads are under way before the
+// first is waited for.
 template <int DK>
 __device__ __forceinline__ void add_update(float (&S)[DK / 2], float whole, const Lane& l) {
+  uint32_t r[DK / 64][32];
+#pragma unroll
+  for (int q = 0; q < DK / 64; ++q) tmem_ld32(l.tmem + kAcc + l.half * (DK / 2) + 32 * q, r[q]);
 #pragma unroll
   for (int q = 0; q < DK / 64; ++q) {
-    uint32_t r[32];
-    tmem_ld32(l.tmem + kAcc + l.half * (DK / 2) + 32 * q, r);
-    tc_wait_ld();
+    tc_wait_ld(r[q]);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       const uint64_t x = f2_fma(f2_pack(whole, whole), f2_pack(S[32 * q + i], S[32 * q + i + 1]),
-                                f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+                                f2_pack(__uint_as_float(r[q][i]), __uint_as_float(r[q][i + 1])));
       S[32 * q + i] = f2_lo(x);
       S[32 * q + i + 1] = f2_hi(x);
     }
@@ -326,51 +351,22 @@ __device__ __forceinline__ void put_tokens(const float (&x)[32], uint32_t at, co
   tmem_st16(at + 16 * l.half, hi);
   tmem_st16(at + 32 + 16 * l.half, lo);
 }
-__device__ __forceinline__ void put_image(const uint32_t (&hi)[16], bf16* image, int rows,
-                                          const Lane& l) {
-  if (l.col < rows)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<uint4*>(image + (static_cast<int64_t>(4 * l.half + i) * rows + l.col) * 8) =
-          make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-}
-// This lane's values of its 32 tokens from two 64 x 64 tiles, as pairs of tokens.
-__device__ __forceinline__ void load_values(uint32_t (&x)[16], const unsigned char* v,
-                                            const Lane& l) {
+// This lane's values of its 32 tokens from two 64 x 64 tiles, times a factor a token.
+__device__ __forceinline__ void load_values(float (&x)[32], const unsigned char* v,
+                                            const float* factor, float scale, const Lane& l) {
   v += (l.row >> 6) * kTile + 32 * l.half * 128 + 2 * (l.row & 7);
   const int piece = (l.row & 63) >> 3;
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    x[i] = *reinterpret_cast<const uint16_t*>(v + sw128_offset(2 * i, piece)) |
-           (static_cast<uint32_t>(
-                *reinterpret_cast<const uint16_t*>(v + sw128_offset(2 * i + 1, piece)))
-            << 16);
-}
-// 32 tokens of this lane, as bf16 pairs of tokens, to rows of a contiguous [.., Hv,
-// dv] tensor (`dst`: first row, column 0 of the block), by way of shared memory: the
-// four warps of a half have whole rows of 128 columns between them.
-__device__ __forceinline__ bool put_rows(const uint32_t (&x)[16], unsigned char* out, bf16* dst,
-                                         int64_t stride, int len, int cols, const Lane& l, int n,
-                                         const SeqArgs& a, Bars& bars) {
-  unsigned char* at = out + 32 * l.half * kRowBytes + 2 * l.row;
+  for (int i = 0; i < 32; i += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(factor + 32 * l.half + i);
+    const float fs[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    *reinterpret_cast<uint16_t*>(at + 2 * i * kRowBytes) = static_cast<uint16_t>(x[i]);
-    *reinterpret_cast<uint16_t*>(at + (2 * i + 1) * kRowBytes) =
-        static_cast<uint16_t>(x[i] >> 16);
+    for (int e = 0; e < 4; ++e)
+      x[i + e] = scale * fs[e] *
+                 __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(
+                                     v + sw128_offset(i + e, piece)))
+                                 << 16);
   }
-  signal(&bars.rows[l.half]);
-  if (!wait(&bars.rows[l.half], n, a, bars)) return false;
-  const int piece = (l.row & 15) * 8, first = 32 * l.half + (l.row >> 4);
-  const unsigned char* from = out + first * kRowBytes + 2 * piece;
-  bf16* to = dst + first * stride + piece;
-  if (piece < cols)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (first + 8 * i < len)
-        *reinterpret_cast<uint4*>(to + 8 * i * stride) =
-            *reinterpret_cast<const uint4*>(from + 8 * i * kRowBytes);
-  return true;
 }
 
 template <int DK>
@@ -378,20 +374,7 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
                                      const Lane& l, const Smem<DK>& sm, Bars& bars) {
   const int chunks = (s.len + kChunk - 1) / kChunk, rows = padded_dv(p.dv);
   const int64_t head = (static_cast<int64_t>(blockIdx.x) * p.Hv + hv) * p.dk * p.dv;
-  const int64_t stride = static_cast<int64_t>(p.Hv) * p.dv;
-  const int col0 = l.col - l.row, cols = p.dv - col0, t0 = 32 * l.half;
-  bf16* out = static_cast<bf16*>(a.out) +
-              ((static_cast<int64_t>(s.b) * p.T + s.begin) * p.Hv + hv) * p.dv + col0;
-  auto finish = [&](int n) {  // O of chunk n
-    uint32_t r[32], x[16];
-    tmem_ld32(l.tmem + kRO + 128 * (n & 1) + 64 + t0, r);
-    tc_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      x[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-    return put_rows(x, sm.out(), out + static_cast<int64_t>(n) * kChunk * stride, stride,
-                    s.len - n * kChunk, cols, l, n, a, bars);
-  };
+  const int t0 = 32 * l.half;
   float S[DK / 2];
   load_state<DK>(S, a.state0 ? a.state0 + head : nullptr, p, l);
   float whole = 1.f;
@@ -406,72 +389,66 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
     put_operand<DK>(S, l, a.states ? a.states + slot * DK * rows : nullptr, rows);
     tc_wait_st();
     signal(&bars.s_ready);
-    if (n > 0) {  // beside this chunk's first product
-      if (!wait(&bars.o_full, n - 1, a, bars)) return;
-      if (!finish(n - 1)) return;
-    }
     if (!wait(&bars.full_a[st], turn, a, bars)) return;
     const Block* blk = reinterpret_cast<const Block*>(sm.t(st));
     float y[32];
-    uint32_t r[32], u[32], hi[16];
-    load_values(hi, sm.v(st), l);
+    uint32_t hi[16];
+    load_values(y, sm.v(st), blk->beta, 1.f, l);  // beside the first product
+    whole = blk->grown[kChunk - 1];
     if (!wait(&bars.r_full, n, a, bars)) return;
-    tmem_ld32(ro + t0, r);
-    tc_wait_ld();
+    {
+      uint32_t r[32];
+      tmem_ld32(ro + t0, r);
+      tc_wait_ld(r);
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
-      const float4 b = *reinterpret_cast<const float4*>(blk->beta + t0 + i);
-      const uint32_t v0 = hi[i / 2], v1 = hi[i / 2 + 1];
-      y[i] = b.x * fmaf(-g.x, __uint_as_float(r[i]), lo_of(v0));
-      y[i + 1] = b.y * fmaf(-g.y, __uint_as_float(r[i + 1]), hi_of(v0));
-      y[i + 2] = b.z * fmaf(-g.z, __uint_as_float(r[i + 2]), lo_of(v1));
-      y[i + 3] = b.w * fmaf(-g.w, __uint_as_float(r[i + 3]), hi_of(v1));
+      for (int i = 0; i < 32; i += 4) {  // beta V - (beta e^c) R
+        const float4 g = *reinterpret_cast<const float4*>(blk->both + t0 + i);
+        y[i] = fmaf(-g.x, __uint_as_float(r[i]), y[i]);
+        y[i + 1] = fmaf(-g.y, __uint_as_float(r[i + 1]), y[i + 1]);
+        y[i + 2] = fmaf(-g.z, __uint_as_float(r[i + 2]), y[i + 2]);
+        y[i + 3] = fmaf(-g.w, __uint_as_float(r[i + 3]), y[i + 3]);
+      }
     }
     put_tokens(y, l.tmem + kS, l, hi);
     tc_wait_st();
     signal(&bars.y_ready);
-    whole = blk->grown[kChunk - 1];
-    // beside the product with T: O's part from the state gets its decays
-    tmem_ld32(ro + 64 + t0, r);
-    tc_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
-      r[i] = __float_as_uint(p.scale * g.x * __uint_as_float(r[i]));
-      r[i + 1] = __float_as_uint(p.scale * g.y * __uint_as_float(r[i + 1]));
-      r[i + 2] = __float_as_uint(p.scale * g.z * __uint_as_float(r[i + 2]));
-      r[i + 3] = __float_as_uint(p.scale * g.w * __uint_as_float(r[i + 3]));
-    }
-    tmem_st32(ro + 64 + t0, r);
     if (!wait(&bars.n_full, n, a, bars)) return;
-    tmem_ld32(l.tmem + kAcc + t0, r);
-    tmem_ld32(l.tmem + kAcc + 64 + t0, u);
-    tc_wait_ld();
-    float x[32];
+    {
+      uint32_t r[32], u[32];
+      tmem_ld32(l.tmem + kAcc + t0, r);
+      tmem_ld32(l.tmem + kAcc + 64 + t0, u);
+      tc_wait_ld(r, u);
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(blk->left + t0 + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        x[i + e] = __uint_as_float(r[i + e]) + __uint_as_float(u[i + e]);
-      y[i] = g.x * x[i];
-      y[i + 1] = g.y * x[i + 1];
-      y[i + 2] = g.z * x[i + 2];
-      y[i + 3] = g.w * x[i + 3];
+      for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(r[i]) + __uint_as_float(u[i]);
     }
-    put_tokens(y, l.tmem + kD, l, hi);
-    put_tokens(x, ro, l, hi);
+    {
+      float x[32];
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 g = *reinterpret_cast<const float4*>(blk->left + t0 + i);
+        x[i] = g.x * y[i];
+        x[i + 1] = g.y * y[i + 1];
+        x[i + 2] = g.z * y[i + 2];
+        x[i + 3] = g.w * y[i + 3];
+      }
+      put_tokens(x, l.tmem + kD, l, hi);
+    }
     tc_wait_st();
     signal(&bars.d_ready);
+    put_tokens(y, ro, l, hi);  // beside the state's product
+    tc_wait_st();
+    signal(&bars.x_ready);
     signal(&bars.empty_a[st]);
-    if (a.rows) put_image(hi, a.rows + slot * kChunk * rows, rows, l);
+    if (a.rows && l.col < rows)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4*>(a.rows + slot * kChunk * rows +
+                                  (static_cast<int64_t>(4 * l.half + i) * rows + l.col) * 8) =
+            make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
   }
   if (chunks > 0) {
     if (!wait(&bars.upd_full, chunks - 1, a, bars)) return;
     add_update<DK>(S, whole, l);
-    if (!wait(&bars.o_full, chunks - 1, a, bars)) return;
-    if (!finish(chunks - 1)) return;
   }
   if (a.state1) store_state<DK>(S, a.state1 + head, p, l);
 }
@@ -483,10 +460,7 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
                                           int hv, const Lane& l, const Smem<DK>& sm, Bars& bars) {
   const int chunks = (s.len + kChunk - 1) / kChunk, rows = padded_dv(p.dv);
   const int64_t head = (static_cast<int64_t>(blockIdx.x) * p.Hv + hv) * p.dk * p.dv;
-  const int64_t stride = static_cast<int64_t>(p.Hv) * p.dv;
-  const int col0 = l.col - l.row, cols = p.dv - col0, t0 = 32 * l.half;
-  bf16* out = static_cast<bf16*>(a.out) +
-              ((static_cast<int64_t>(s.b) * p.T + s.begin) * p.Hv + hv) * p.dv + col0;
+  const int t0 = 32 * l.half;
   float S[DK / 2];
   load_state<DK>(S, a.state0 ? a.state0 + head : nullptr, p, l);
   float whole = 1.f;
@@ -503,74 +477,151 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
     signal(&bars.s_ready);
     if (!wait(&bars.full_a[st], turn, a, bars)) return;
     const Block* blk = reinterpret_cast<const Block*>(sm.t(st));
+    whole = blk->grown[kChunk - 1];
     float y[32];
-    uint32_t r[32], u[32], hi[16], d[16];
-    load_values(d, sm.v(st), l);
+    uint32_t hi[16];
     if (!wait(&bars.r_full, n, a, bars)) return;
-    tmem_ld32(ro + t0, r);
-    tmem_ld32(ro + 64 + t0, u);
-    tc_wait_ld();
+    {
+      uint32_t r[32], u[32];
+      tmem_ld32(ro + t0, r);
+      tmem_ld32(ro + 64 + t0, u);
+      tc_wait_ld(r, u);
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(blk->left + t0 + i);
-      y[i] = fmaf(g.x, __uint_as_float(r[i]), __uint_as_float(u[i]));
-      y[i + 1] = fmaf(g.y, __uint_as_float(r[i + 1]), __uint_as_float(u[i + 1]));
-      y[i + 2] = fmaf(g.z, __uint_as_float(r[i + 2]), __uint_as_float(u[i + 2]));
-      y[i + 3] = fmaf(g.w, __uint_as_float(r[i + 3]), __uint_as_float(u[i + 3]));
+      for (int i = 0; i < 32; i += 4) {
+        const float4 g = *reinterpret_cast<const float4*>(blk->left + t0 + i);
+        y[i] = fmaf(g.x, __uint_as_float(r[i]), __uint_as_float(u[i]));
+        y[i + 1] = fmaf(g.y, __uint_as_float(r[i + 1]), __uint_as_float(u[i + 1]));
+        y[i + 2] = fmaf(g.z, __uint_as_float(r[i + 2]), __uint_as_float(u[i + 2]));
+        y[i + 3] = fmaf(g.w, __uint_as_float(r[i + 3]), __uint_as_float(u[i + 3]));
+      }
     }
     put_tokens(y, l.tmem + kS, l, hi);
     tc_wait_st();
     signal(&bars.y_ready);
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {  // beside the product with T
-      const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
-      y[i] = p.scale * g.x * lo_of(d[i / 2]);
-      y[i + 1] = p.scale * g.y * hi_of(d[i / 2]);
-      y[i + 2] = p.scale * g.z * lo_of(d[i / 2 + 1]);
-      y[i + 3] = p.scale * g.w * hi_of(d[i / 2 + 1]);
-    }
+    load_values(y, sm.v(st), blk->grown, p.scale, l);  // beside the product with T
     put_tokens(y, l.tmem + kD, l, hi);
     tc_wait_st();
     signal(&bars.z_ready);
-    whole = blk->grown[kChunk - 1];
     if (!wait(&bars.n_full, n, a, bars)) return;
-    tmem_ld32(ro + t0, r);
-    tmem_ld32(ro + 64 + t0, u);
-    tc_wait_ld();
+    {
+      uint32_t r[32], u[32];
+      tmem_ld32(ro + t0, r);
+      tmem_ld32(ro + 64 + t0, u);
+      tc_wait_ld(r, u);
 #pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
-      const float4 b = *reinterpret_cast<const float4*>(blk->beta + t0 + i);
-      const float ge[4] = {g.x, g.y, g.z, g.w}, be[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = __uint_as_float(r[i + e]) + __uint_as_float(u[i + e]);
-        const float v = be[e] * x;
-        y[i + e] = -ge[e] * v;
-        r[i + e] = __float_as_uint(x);  // dY
-        u[i + e] = __float_as_uint(v);  // dV
+      for (int i = 0; i < 32; i += 4) {
+        const float4 g = *reinterpret_cast<const float4*>(blk->both + t0 + i);
+        y[i] = -g.x * (__uint_as_float(r[i]) + __uint_as_float(u[i]));
+        y[i + 1] = -g.y * (__uint_as_float(r[i + 1]) + __uint_as_float(u[i + 1]));
+        y[i + 2] = -g.z * (__uint_as_float(r[i + 2]) + __uint_as_float(u[i + 2]));
+        y[i + 3] = -g.w * (__uint_as_float(r[i + 3]) + __uint_as_float(u[i + 3]));
       }
     }
     put_tokens(y, l.tmem + kS, l, hi);
     tc_wait_st();
     signal(&bars.d_ready);
     signal(&bars.empty_a[st]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      hi[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-    put_image(hi, a.rows + slot * kChunk * rows, rows, l);
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      hi[i] = pack_bf16x2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-    if (!put_rows(hi, sm.out(), out + static_cast<int64_t>(at) * kChunk * stride, stride,
-                  s.len - at * kChunk, cols, l, n, a, bars))
-      return;
   }
   if (chunks > 0) {
     if (!wait(&bars.upd_full, chunks - 1, a, bars)) return;
     add_update<DK>(S, whole, l);
   }
   if (a.state1) store_state<DK>(S, a.state1 + head, p, l);
+}
+
+// The row warps, one a quadrant of lanes: forwards O's part from the state gets its
+// decays (scale e^c) before N's is added, and O leaves; backwards dY is kept and
+// dV = beta dY leaves.  Rows leave by way of shared memory, 256 bytes together.
+template <int DK, bool REV>
+__device__ __forceinline__ void take_rows(const gsa_delta_t& p, const SeqArgs& a, const Seq& s,
+                                          int hv, int row, int col0, uint32_t tmem,
+                                          const Smem<DK>& sm, Bars& bars) {
+  const int chunks = (s.len + kChunk - 1) / kChunk, rows = padded_dv(p.dv), col = col0 + row;
+  const int64_t stride = static_cast<int64_t>(p.Hv) * p.dv;
+  bf16* out = static_cast<bf16*>(a.out) +
+              ((static_cast<int64_t>(s.b) * p.T + s.begin) * p.Hv + hv) * p.dv + col0;
+  unsigned char* mine = sm.out() + 2 * row;
+  const int piece = (row & 15) * 8, first = row >> 4;
+  for (int n = 0; n < chunks; ++n) {
+    const int st = n % kStages, turn = n / kStages, at = REV ? chunks - 1 - n : n;
+    const uint32_t ro = tmem + kRO + 128 * (n & 1);
+    const int64_t slot = static_cast<int64_t>(s.chunk0 + at) * p.Hv + hv;
+    const Block* blk = reinterpret_cast<const Block*>(sm.t(st));
+    if (!wait(&bars.full_a[st], turn, a, bars)) return;
+    if constexpr (!REV) {
+      if (!wait(&bars.r_full, n, a, bars)) return;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t r[16];
+        tmem_ld16(ro + 64 + 16 * q, r);
+        tc_wait_ld(r);
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const float4 g = *reinterpret_cast<const float4*>(blk->grown + 16 * q + i);
+          r[i] = __float_as_uint(p.scale * g.x * __uint_as_float(r[i]));
+          r[i + 1] = __float_as_uint(p.scale * g.y * __uint_as_float(r[i + 1]));
+          r[i + 2] = __float_as_uint(p.scale * g.z * __uint_as_float(r[i + 2]));
+          r[i + 3] = __float_as_uint(p.scale * g.w * __uint_as_float(r[i + 3]));
+        }
+        tmem_st16(ro + 64 + 16 * q, r);
+      }
+      tc_wait_st();
+      signal(&bars.z_ready);
+      signal(&bars.empty_a[st]);
+    }
+    if (!wait(REV ? &bars.n_full : &bars.o_full, n, a, bars)) return;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t r[16], u[16];
+      tmem_ld16(ro + (REV ? 0 : 64) + 16 * q, r);
+      if constexpr (REV) tmem_ld16(ro + 64 + 16 * q, u);
+      tc_wait_ld(r, u);
+      if constexpr (REV) {
+        uint32_t hi[8];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(u[i]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          hi[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        if (col < rows)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(a.rows + slot * kChunk * rows +
+                                      (static_cast<int64_t>(2 * q + i) * rows + col) * 8) =
+                make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(blk->beta + 16 * q + i);
+          r[i] = __float_as_uint(b.x * __uint_as_float(r[i]));
+          r[i + 1] = __float_as_uint(b.y * __uint_as_float(r[i + 1]));
+          r[i + 2] = __float_as_uint(b.z * __uint_as_float(r[i + 2]));
+          r[i + 3] = __float_as_uint(b.w * __uint_as_float(r[i + 3]));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const uint32_t x = pack_bf16x2(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+        *reinterpret_cast<uint16_t*>(mine + (16 * q + i) * kRowBytes) = static_cast<uint16_t>(x);
+        *reinterpret_cast<uint16_t*>(mine + (16 * q + i + 1) * kRowBytes) =
+            static_cast<uint16_t>(x >> 16);
+      }
+    }
+    signal(&bars.o_read);
+    if constexpr (REV) signal(&bars.empty_a[st]);
+    signal(&bars.rows);
+    if (!wait(&bars.rows, 2 * n, a, bars)) return;
+    const int len = s.len - at * kChunk;
+    if (piece < p.dv - col0)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (first + 8 * i < len)
+          *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(at) * kChunk + first + 8 * i) *
+                                              stride + piece) =
+              *reinterpret_cast<const uint4*>(sm.out() + (first + 8 * i) * kRowBytes + 2 * piece);
+    signal(&bars.rows);  // the rows are read: the next chunk's may be written
+    if (!wait(&bars.rows, 2 * n + 1, a, bars)) return;
+  }
 }
 
 template <int DK, bool REV>
@@ -596,15 +647,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars.full_a[i], 1);
       mbar_init(&bars.full_b[i], 1);
-      mbar_init(&bars.empty_a[i], 1 + kComputeWarps);
+      mbar_init(&bars.empty_a[i], 1 + kComputeWarps + kRowWarps);
       mbar_init(&bars.empty_b[i], 1);
     }
     mbar_init(&bars.s_ready, kComputeWarps);
     mbar_init(&bars.y_ready, kComputeWarps);
-    mbar_init(&bars.z_ready, kComputeWarps);
+    mbar_init(&bars.z_ready, REV ? kComputeWarps : kRowWarps);
     mbar_init(&bars.d_ready, kComputeWarps);
-    mbar_init(&bars.rows[0], kComputeWarps / 2);
-    mbar_init(&bars.rows[1], kComputeWarps / 2);
+    mbar_init(&bars.x_ready, kComputeWarps);
+    mbar_init(&bars.o_read, kRowWarps);
+    mbar_init(&bars.rows, kRowWarps);
     mbar_init(&bars.r_full, 1);
     mbar_init(&bars.n_full, 1);
     mbar_init(&bars.upd_full, 1);
@@ -612,29 +664,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bars.drain, 1);
     fence_mbar_init();
   }
-  if (warp == kComputeWarps) {
+  if (warp == kIssueWarp) {
     tmem_alloc(&bars.tmem, kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kComputeWarps + 1) {
-    produce<DK, REV>(p, maps, a, s, hv, col0, sm, bars);
-  } else if (warp == kComputeWarps) {
-    if ((threadIdx.x & 31) == 0) issue<DK, REV>(a, chunks, sm, bars);
-  } else {
-    const int row = 32 * (warp & 3) + (threadIdx.x & 31);
-    const Lane l = {row, warp >> 2, col0 + row,
-                    bars.tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16)};
+  const int row = 32 * (warp & 3) + (threadIdx.x & 31);
+  const uint32_t tmem = bars.tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+  if (warp < kComputeWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
+    const Lane l = {row, warp >> 2, col0 + row, tmem};
     if constexpr (REV)
       walk_back<DK>(p, a, s, hv, l, sm, bars);
     else
       walk<DK>(p, a, s, hv, l, sm, bars);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kCopyWarp) {
+      produce<DK, REV>(p, maps, a, s, hv, col0, sm, bars);
+    } else if (warp == kIssueWarp) {
+      if ((threadIdx.x & 31) == 0) issue<DK, REV>(a, chunks, sm, bars);
+    } else if (warp < kIssueWarp) {
+      take_rows<DK, REV>(p, a, s, hv, row, col0, tmem, sm, bars);
+    }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kComputeWarps) {
+  if (warp == kIssueWarp) {
     tc_fence_after();
     tmem_dealloc(bars.tmem, kTmemCols);
   }
@@ -643,6 +701,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int DK, bool REV>
 cudaError_t launch(const gsa_delta_t& p, const DeltaMaps& m, const SeqArgs& a,
                    cudaStream_t stream) {
+  // the split of setmaxnreg is valid only for the register count it was written for: with
+  // fewer at launch its `inc` would wait for registers that do not exist
+  static std::atomic<int> regs{0};
+  if (regs.load(std::memory_order_acquire) == 0) {
+    cudaFuncAttributes f;
+    const cudaError_t e = cudaFuncGetAttributes(&f, seq_kernel<DK, REV>);
+    if (e != cudaSuccess) return e;
+    regs.store(f.numRegs, std::memory_order_release);
+  }
+  if (regs.load(std::memory_order_acquire) != kLaunchRegs) return cudaErrorNotSupported;
   const cudaError_t e = allow_smem<seq_kernel<DK, REV>>(seq_smem<DK>());
   if (e != cudaSuccess) return e;
   const int seqs = p.N + (!REV && p.cu_seqlens ? 2 : 0);

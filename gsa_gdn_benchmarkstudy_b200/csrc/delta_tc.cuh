@@ -24,6 +24,17 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// Waits for this thread's tensor-memory loads; the registers they fill are named, so
+// that no use of them moves in front of the wait.
+template <typename... R>
+__device__ __forceinline__ void tc_wait_ld(R&... r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  auto hold = [](auto& a) {
+#pragma unroll
+    for (uint32_t& x : a) asm volatile("" : "+r"(x));
+  };
+  (hold(r), ...);
+}
 // Store 16 consecutive 32-bit columns of this thread's lane (32x32b shape).
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -31,6 +42,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// ... and 8.
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
       : "memory");
 }
 
@@ -93,7 +112,7 @@ struct __align__(16) Block {
   float grown[kChunk];  // e^{c_i}
   float beta[kChunk];
   float left[kChunk];   // e^{c_64 - c_i}
-  float pad[kChunk];
+  float both[kChunk];   // beta_i e^{c_i}
   unsigned char p_hi[kTile], p_lo[kTile];
 };
 constexpr int kTBytes = 2 * static_cast<int>(kTile) + 1024;  // T and the decays
