@@ -55,6 +55,13 @@ int device_state(DeviceState** out) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return set_cuda_error(e);
   if (dev < 0 || dev >= kMaxDevices) return set_error(GSA_ERR_NO_DEVICE, "device index out of range");
+  // Encoding a tensor map is a driver call: it needs the device's context current,
+  // which a thread whose first CUDA call this is (autograd's) does not have yet.
+  static thread_local bool bound = false;
+  if (!bound) {
+    if ((e = cudaSetDevice(dev)) != cudaSuccess) return set_cuda_error(e);
+    bound = true;
+  }
   DeviceState& st = g_dev[dev];
   if (!st.ready.load(std::memory_order_acquire)) {
     std::lock_guard<std::mutex> lock(g_dev_mu);

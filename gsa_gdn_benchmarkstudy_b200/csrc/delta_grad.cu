@@ -208,7 +208,7 @@ __device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& m
 template <int DK>
 __device__ __forceinline__ void issue(const gsa_delta_t& p, const GradArgs& a, uint32_t smem,
                                       Bars& bars) {
-  const uint32_t tm = bars.tmem, K = smem, Q = smem + kTile;
+  const uint32_t tm = __shfl_sync(0xFFFFFFFFu, bars.tmem, 0), K = smem, Q = smem + kTile;
   const uint32_t S0 = smem + kOffS0, S1 = smem + kOffS1, N = smem + kOffN, Y = smem + kOffY;
   const uint32_t D = smem + kOffD, V = smem + kOffV, A = smem + kOffA, M = smem + kOffM;
   constexpr uint32_t kRR = idesc_bf16_f32(128, 64, 0, 0), kCR = idesc_bf16_f32(128, 64, 1, 0);
@@ -217,7 +217,7 @@ __device__ __forceinline__ void issue(const gsa_delta_t& p, const GradArgs& a, u
   int items = 0, loads = 0, heads = 0;
   bool ok = true;
   auto until = [&](uint64_t* bar, int parity) {
-    ok = ok && mbar_wait(bar, parity & 1, a.err, &bars.abort);
+    ok = ok && mbar_wait_warp(bar, parity & 1, a.err, &bars.abort);
     tc_fence_after();
     return ok;
   };
@@ -229,43 +229,45 @@ __device__ __forceinline__ void issue(const gsa_delta_t& p, const GradArgs& a, u
         if (!until(&bars.full_kq, items)) break;
 #pragma unroll
         for (int ks = 0; ks < DK / 16; ++ks) {
-          tc_mma_ss(tm + kKq, desc_kq(K, ks), desc_kq(Q, ks), kRR, ks > 0);
-          tc_mma_ss(tm + kKk, desc_kq(Q, ks), desc_kq(K, ks), kRR, ks > 0);
+          warp_mma_ss(tm + kKq, desc_kq(K, ks), desc_kq(Q, ks), kRR, ks > 0);
+          warp_mma_ss(tm + kKk, desc_kq(Q, ks), desc_kq(K, ks), kRR, ks > 0);
         }
       }
       if (heads > 0 && !until(&bars.x_read, heads - 1)) break;
       for (int col0 = 0; col0 < p.dv; col0 += 128, ++loads) {
         if (!until(&bars.full_h, loads)) break;
         const int steps = min(128, rows - col0) / 16;
+#pragma unroll 4
         for (int ks = 0; ks < steps; ++ks) {
           const uint32_t on = col0 > 0 || ks > 0;
           const uint64_t s0 = desc_image(S0, ks), n = desc_image(N, ks);
-          tc_mma_ss(tm + kTo, s0, desc_rows(D, ks), kCR, on);
-          tc_mma_ss(tm + kTy, s0, desc_image(Y, ks), kCC, on);
-          tc_mma_ss(tm + kTn, desc_image(S1, ks), n, kCC, on);
-          tc_mma_ss(tm + kPd, n, desc_rows(D, ks), kCR, on);
-          tc_mma_ss(tm + kPn, n, n, kCC, on);
-          tc_mma_ss(tm + kPv, n, desc_rows(V, ks), kCR, on);
+          warp_mma_ss(tm + kTo, s0, desc_rows(D, ks), kCR, on);
+          warp_mma_ss(tm + kTy, s0, desc_image(Y, ks), kCC, on);
+          warp_mma_ss(tm + kTn, desc_image(S1, ks), n, kCC, on);
+          warp_mma_ss(tm + kPd, n, desc_rows(D, ks), kCR, on);
+          warp_mma_ss(tm + kPn, n, n, kCC, on);
+          warp_mma_ss(tm + kPv, n, desc_rows(V, ks), kCR, on);
         }
-        tc_commit(&bars.empty_h);
+        warp_commit(&bars.empty_h);
       }
       if (!ok) break;
-      tc_commit(&bars.ph1_full);
+      warp_commit(&bars.ph1_full);
       if (!until(&bars.ph2_ready, heads)) break;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        tc_mma_ss(tm + kPd, desc_kt(K, ks), desc_cols(A, ks), kCC, ks > 0);
-        tc_mma_ss(tm + kPn, desc_kt(Q, ks), desc_rows(A, ks), kCR, ks > 0);
-        tc_mma_ss(tm + kPn, desc_kt(K, ks), desc_cols(M, ks), kCC, 1);
-        tc_mma_ss(tm + kPn, desc_kt(K, ks), desc_rows(M, ks), kCR, 1);
+        warp_mma_ss(tm + kPd, desc_kt(K, ks), desc_cols(A, ks), kCC, ks > 0);
+        warp_mma_ss(tm + kPn, desc_kt(Q, ks), desc_rows(A, ks), kCR, ks > 0);
+        warp_mma_ss(tm + kPn, desc_kt(K, ks), desc_cols(M, ks), kCC, 1);
+        warp_mma_ss(tm + kPn, desc_kt(K, ks), desc_rows(M, ks), kCR, 1);
       }
-      tc_commit(&bars.ph2_full);
-      if (h == group - 1) tc_commit(&bars.empty_kq);
+      warp_commit(&bars.ph2_full);
+      if (h == group - 1) warp_commit(&bars.empty_kq);
     }
     ++items;
   }
-  tc_commit(&bars.drain);
+  warp_commit(&bars.drain);
   mbar_wait_drain(&bars.drain, 0, kWaitLimitCycles);
+  __syncwarp();
 }
 
 struct Sums {  // per token; by quadrant of lanes where several warps have a part
@@ -288,7 +290,7 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
   const int group = p.Hv / p.Hk, rows = padded_dv(p.dv);
   const bool gate16 = p.gate_dtype == GSA_DTYPE_BF16;
   const int64_t qk_step = static_cast<int64_t>(p.Hk) * p.dk;
-  int loads = 0, heads = 0;
+  int items = 0, loads = 0, heads = 0;
   auto until = [&](uint64_t* bar, int parity) {
     const bool ok = mbar_wait_warp(bar, parity & 1, a.err, &bars.abort);
     tc_fence_after();
@@ -324,6 +326,7 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
       }
       continue;
     }
+    if (!until(&bars.full_kq, items++)) return;
     float gq[32], gk[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) gq[i] = gk[i] = 0.f;
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kComputeWarps + 1)
     produce<DK>(p, maps, more, a, smem, bars);
   else if (warp == kComputeWarps) {
-    if ((threadIdx.x & 31) == 0) issue<DK>(p, a, smem_u32(smem), bars);
+    issue<DK>(p, a, smem_u32(smem), bars);
   } else {
     compute<DK>(p, a, smem, bars, sum);
   }

@@ -35,16 +35,15 @@ static_assert(256 * kComputeRegs + 256 * kOtherRegs <= kThreads * kLaunchRegs, "
 constexpr int kCols = 128;  // state columns of a block: the lanes of tensor memory
 constexpr uint32_t kTmemCols = 512;
 
-// Tensor memory, 32-bit columns; b = 0, 1 in turn by chunk.  A product takes about
-// 62 cycles for 16 of the contraction whether its accumulator has 64 columns or
-// 128, so K and Q stand as one right operand of 128 rows (R and O come together),
-// and T_hi and T_lo too (two halves that the threads add).
+// Tensor memory, 32-bit columns; b = 0, 1 in turn by chunk.
 enum : uint32_t {
-  kAcc = 0,    // what a chunk adds to S^T [128][dk]; before that [Y T_hi | Y T_lo]^T
-  kS = 128,    // left operands, two values a column: S^T hi (64), lo (64); then, once
-               // R is there, Y^T (backwards dN^T, then -e^c beta dY^T) hi, lo (32 each)
-  kD = 192,    // and (e^{c_64 - c} N)^T (backwards (scale e^c dO)^T) hi, lo
-  kRO = 256,   // + 128 b: R^T (64), O^T (64); N^T hi, lo in R's place.  Backwards
+  kAcc = 0,    // what a chunk adds to S^T [128][dk]
+  kY = 0,      // forwards, before that: Y^T hi, lo (32 columns of two values each)
+  kS = 128,    // S^T as a left operand hi, lo (64 columns of two values each);
+               // backwards, once dS^T K^T is there: dN^T, then -e^c beta dY^T hi, lo
+  kD = 192,    // then (e^{c_64 - c} N)^T (backwards (scale e^c dO)^T) hi, lo
+  kRO = 256,   // + 128 b: R^T, then N^T (64), O^T (64); N^T as an operand in its own
+               // place, for each half of the tokens hi, lo (16 each).  Backwards
                // dS^T K^T and dO^T P, then [dN T_hi | dN T_lo]^T
 };
 
@@ -74,12 +73,14 @@ struct Smem {
   __device__ unsigned char* out() const { return p(kStages); }
 };
 
-// Every barrier but the queues' completes once a chunk.
+// Every barrier but the queues' completes once a chunk, and never twice while a
+// warp still has to wait for the first of the two (a parity tells only neighbouring
+// phases apart): whoever completes it has waited, since the time before, for
+// something that its waiters signal later.
 struct Bars {
   uint64_t full_a[kStages], empty_a[kStages], full_b[kStages], empty_b[kStages];
-  uint64_t s_ready, r_full, y_ready, n_full, d_ready, upd_full, o_full;
-  uint64_t z_ready;  // forwards O's first part has its decays; backwards dO is an operand
-  uint64_t x_ready;  // forwards N is an operand
+  uint64_t s_ready, r_full, o1_full, y_ready, n_full, d_ready, upd_full, o_full;
+  uint64_t x_ready;  // forwards N is an operand, backwards dO is
   uint64_t o_read;   // the row warps are through with a chunk's accumulators
   uint64_t rows;     // ... and have written their columns of its output rows
   uint64_t drain;
@@ -187,93 +188,113 @@ __device__ __forceinline__ void times(uint32_t acc, uint32_t left, uint64_t b, u
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     const uint32_t off = COLS ? ks * 2048 : (ks >> 2) * step + (ks & 3) * 32;
-    tc_mma_ts(acc, left + 8 * ks, b + (off >> 4), idesc, !fresh || ks);
+    warp_mma_ts(acc, left + 8 * ks, b + (off >> 4), idesc, !fresh || ks);
   }
 }
 
-// One thread issues all products.
+// O^T += N^T P^T: N's halves lie apart.
+__device__ __forceinline__ void times_inner(uint32_t ro, uint64_t p_rows, uint32_t idesc) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i)  // hi P_hi, lo P_hi, hi P_lo
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+      warp_mma_ts(ro + 64, ro + 32 * (ks >> 1) + 8 * (ks & 1) + (i == 1 ? 16 : 0),
+                  p_rows + (i == 2 ? kTile >> 4 : 0) + 2 * ks, idesc, 1);
+}
+
+// One warp issues all products.
 template <int DK, bool REV>
 __device__ __forceinline__ void issue(const SeqArgs& a, int chunks, const Smem<DK>& sm,
                                       Bars& bars) {
-  const uint32_t tm = bars.tmem;
+  const uint32_t tm = __shfl_sync(0xFFFFFFFFu, bars.tmem, 0);
   constexpr uint32_t kRows64 = idesc_bf16_f32(128, 64, 0, 0);
-  constexpr uint32_t kRows128 = idesc_bf16_f32(128, 128, 0, 0);
   constexpr uint32_t kCols64 = idesc_bf16_f32(128, 64, 0, 1);
   constexpr uint32_t kCols128 = idesc_bf16_f32(128, 128, 0, 1);
   constexpr uint32_t kColsDk = idesc_bf16_f32(128, DK, 0, 1);
   constexpr uint32_t kColsCols = idesc_bf16_f32(128, 64, 1, 1);
   constexpr uint32_t kLo = DK / 2;  // from S's hi columns to its lo columns
   // descriptors of stage 0; a stage is a_bytes (P: kPBytes) further
-  const uint64_t k_rows = desc_rows(smem_u32(sm.a(0)), 0);
-  const uint64_t k_cols = desc_cols(smem_u32(sm.a(0)), 0, kKq);
+  const uint64_t k_rows = desc_rows(smem_u32(sm.a(0)), 0), q_rows = k_rows + (kTile >> 4);
+  const uint64_t k_cols = desc_cols(smem_u32(sm.a(0)), 0, kKq), q_cols = k_cols + (kTile >> 4);
   const uint64_t v_cols = desc_cols(smem_u32(sm.v(0)), 0);
   const uint64_t t_rows = desc_rows(smem_u32(sm.t(0)), 0), t_cols = desc_cols(smem_u32(sm.t(0)), 0);
   const uint64_t p_rows = desc_rows(smem_u32(sm.p(0)), 0), p_cols = desc_cols(smem_u32(sm.p(0)), 0);
-  auto until = [&](uint64_t* bar, int parity) {
-    if (!mbar_wait(bar, parity & 1, a.err, &bars.abort)) return false;
-    tc_fence_after();
+  auto inner = [&](int n) {  // forwards: the rest of O of chunk n
+    if (!wait(&bars.full_b[n & 1], n >> 1, a, bars)) return false;
+    times_inner(tm + kRO + 128 * (n & 1), p_rows + (n & 1) * (kPBytes >> 4), kRows64);
+    warp_commit(&bars.o_full);
+    warp_commit(&bars.empty_b[n & 1]);
     return true;
   };
+  static_assert(kStages == 2, "two stages");
   for (int n = 0; n < chunks; ++n) {
     const int st = n & 1, turn = n >> 1;
-    static_assert(kStages == 2, "two stages");
     const uint32_t da = st * (a_bytes<DK>() >> 4), dp = st * (kPBytes >> 4);
     const uint32_t ro = tm + kRO + 128 * st;
-    if (!until(&bars.full_a[st], turn)) break;
+    if (!wait(&bars.full_a[st], turn, a, bars)) break;
     if constexpr (REV) {
-      if (!until(&bars.full_b[st], turn)) break;
+      if (!wait(&bars.full_b[st], turn, a, bars)) break;
+      if (n > 0 && !wait(&bars.upd_full, n - 1, a, bars)) break;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        tc_mma_ss(ro + 64, v_cols + da + (i & 3) * 128, p_cols + dp + (i >> 2) * (kTile >> 4) +
-                  (i & 3) * 128, kColsCols, i > 0);
-      tc_commit(&bars.empty_b[st]);
-      if (!until(&bars.s_ready, n)) break;
+        warp_mma_ss(ro + 64, v_cols + da + (i & 3) * 128,
+                    p_cols + dp + (i >> 2) * (kTile >> 4) + (i & 3) * 128, kColsCols, i > 0);
+      warp_commit(&bars.empty_b[st]);
+      if (!wait(&bars.s_ready, n, a, bars)) break;
       times<DK / 16, false>(ro, tm + kS, k_rows + da, kKq, kRows64, true);
       times<DK / 16, false>(ro, tm + kS + kLo, k_rows + da, kKq, kRows64, false);
-      tc_commit(&bars.r_full);
-      if (!until(&bars.y_ready, n)) break;
+      warp_commit(&bars.r_full);
+      if (!wait(&bars.y_ready, n, a, bars)) break;
       // the row warps have left the last chunk: its accumulators are the next one's, and
       // no barrier they wait for runs ahead of them by two
-      if (n > 0 && !until(&bars.o_read, n - 1)) break;
+      if (n > 0 && !wait(&bars.o_read, n - 1, a, bars)) break;
       times<4, true>(ro, tm + kS, t_cols + da, kTile, kCols128, true);
       times<4, true>(ro, tm + kS + 32, t_cols + da, kTile, kCols64, false);
-      tc_commit(&bars.n_full);
-      if (!until(&bars.z_ready, n)) break;
-      const uint64_t q_cols = k_cols + (kTile >> 4);
+      warp_commit(&bars.n_full);
+      if (!wait(&bars.x_ready, n, a, bars) || !wait(&bars.n_full, n, a, bars)) break;
       times<4, true>(tm + kAcc, tm + kD, q_cols + da, kKq, kColsDk, true);
       times<4, true>(tm + kAcc, tm + kD + 32, q_cols + da, kKq, kColsDk, false);
-      if (!until(&bars.d_ready, n)) break;
+      if (!wait(&bars.d_ready, n, a, bars)) break;
       times<4, true>(tm + kAcc, tm + kS, k_cols + da, kKq, kColsDk, false);
       times<4, true>(tm + kAcc, tm + kS + 32, k_cols + da, kKq, kColsDk, false);
-      tc_commit(&bars.upd_full);
-      tc_commit(&bars.empty_a[st]);
+      warp_commit(&bars.upd_full);
+      warp_commit(&bars.empty_a[st]);
     } else {
-      if (!until(&bars.s_ready, n)) break;
-      times<DK / 16, false>(ro, tm + kS, k_rows + da, kKq, kRows128, true);
-      times<DK / 16, false>(ro, tm + kS + kLo, k_rows + da, kKq, kRows128, false);
-      tc_commit(&bars.r_full);
-      if (!until(&bars.y_ready, n)) break;
-      times<4, false>(tm + kAcc, tm + kS, t_rows + da, kTile, kRows128, true);
-      times<4, false>(tm + kAcc, tm + kS + 32, t_rows + da, kTile, kRows64, false);
-      tc_commit(&bars.n_full);
-      if (!until(&bars.d_ready, n)) break;
+      if (!wait(&bars.s_ready, n, a, bars)) break;
+      times<DK / 16, false>(ro, tm + kS, k_rows + da, kKq, kRows64, true);
+      times<DK / 16, false>(ro, tm + kS + kLo, k_rows + da, kKq, kRows64, false);
+      warp_commit(&bars.r_full);
+      // O's products fill the pipe while the threads work on R, and later on N.  They are
+      // issued once R (N) has arrived: a commit waits for the products behind it too
+      if (n > 1 && !wait(&bars.o_read, n - 2, a, bars)) break;
+      if (!wait(&bars.r_full, n, a, bars)) break;
+      times<DK / 16, false>(ro + 64, tm + kS, q_rows + da, kKq, kRows64, true);
+      times<DK / 16, false>(ro + 64, tm + kS + kLo, q_rows + da, kKq, kRows64, false);
+      warp_commit(&bars.o1_full);
+      if (!wait(&bars.y_ready, n, a, bars)) break;
+      times<4, false>(ro, tm + kY, t_rows + da, kTile, kRows64, true);
+      times<4, false>(ro, tm + kY + 32, t_rows + da, kTile, kRows64, false);
+      times<4, false>(ro, tm + kY, t_rows + da + (kTile >> 4), kTile, kRows64, false);
+      warp_commit(&bars.n_full);
+      if (!wait(&bars.n_full, n, a, bars)) break;
+      if (n > 0 && !inner(n - 1)) break;
+      if (!wait(&bars.d_ready, n, a, bars)) break;
       times<4, true>(tm + kAcc, tm + kD, k_cols + da, kKq, kColsDk, true);
       times<4, true>(tm + kAcc, tm + kD + 32, k_cols + da, kKq, kColsDk, false);
-      tc_commit(&bars.upd_full);
-      tc_commit(&bars.empty_a[st]);
-      if (!until(&bars.full_b[st], turn) || !until(&bars.z_ready, n) || !until(&bars.x_ready, n))
-        break;
-      times<4, false>(ro + 64, ro, p_rows + dp, kTile, kRows64, false);
-      times<4, false>(ro + 64, ro + 32, p_rows + dp, kTile, kRows64, false);
-      times<4, false>(ro + 64, ro, p_rows + dp + (kTile >> 4), kTile, kRows64, false);
-      tc_commit(&bars.o_full);
-      tc_commit(&bars.empty_b[st]);
-      if (n > 0 && !until(&bars.o_read, n - 1)) break;
+      warp_commit(&bars.upd_full);
+      warp_commit(&bars.empty_a[st]);
+      if (!wait(&bars.x_ready, n, a, bars)) break;
+      if (n == chunks - 1) {
+        // as in every step, o_full may complete again only once its last waiters are through
+        if (n > 0 && !wait(&bars.o_read, n - 1, a, bars)) break;
+        if (!inner(n)) break;
+      }
     }
   }
   // nothing of ours may be in flight when tensor memory is freed
-  tc_commit(&bars.drain);
+  warp_commit(&bars.drain);
   mbar_wait_drain(&bars.drain, 0, kWaitLimitCycles);
+  __syncwarp();
 }
 
 // What a computing thread is: half `half` of column `col` of the value head.
@@ -409,17 +430,31 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
         y[i + 3] = fmaf(-g.w, __uint_as_float(r[i + 3]), y[i + 3]);
       }
     }
-    put_tokens(y, l.tmem + kS, l, hi);
+    put_tokens(y, l.tmem + kY, l, hi);
     tc_wait_st();
     signal(&bars.y_ready);
+    if (!wait(&bars.o1_full, n, a, bars)) return;
+    {  // beside the product with T: O's part from the state gets its decays
+      uint32_t r[32];
+      tmem_ld32(ro + 64 + t0, r);
+      tc_wait_ld(r);
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
+        r[i] = __float_as_uint(p.scale * g.x * __uint_as_float(r[i]));
+        r[i + 1] = __float_as_uint(p.scale * g.y * __uint_as_float(r[i + 1]));
+        r[i + 2] = __float_as_uint(p.scale * g.z * __uint_as_float(r[i + 2]));
+        r[i + 3] = __float_as_uint(p.scale * g.w * __uint_as_float(r[i + 3]));
+      }
+      tmem_st32(ro + 64 + t0, r);
+    }
     if (!wait(&bars.n_full, n, a, bars)) return;
     {
-      uint32_t r[32], u[32];
-      tmem_ld32(l.tmem + kAcc + t0, r);
-      tmem_ld32(l.tmem + kAcc + 64 + t0, u);
-      tc_wait_ld(r, u);
+      uint32_t r[32];
+      tmem_ld32(ro + t0, r);
+      tc_wait_ld(r);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(r[i]) + __uint_as_float(u[i]);
+      for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(r[i]);
     }
     {
       float x[32];
@@ -435,7 +470,13 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
     }
     tc_wait_st();
     signal(&bars.d_ready);
-    put_tokens(y, ro, l, hi);  // beside the state's product
+    {  // beside the state's product
+      uint32_t lo[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) split(y[2 * i], y[2 * i + 1], hi[i], lo[i]);
+      tmem_st16(ro + t0, hi);
+      tmem_st16(ro + t0 + 16, lo);
+    }
     tc_wait_st();
     signal(&bars.x_ready);
     signal(&bars.empty_a[st]);
@@ -501,7 +542,7 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
     load_values(y, sm.v(st), blk->grown, p.scale, l);  // beside the product with T
     put_tokens(y, l.tmem + kD, l, hi);
     tc_wait_st();
-    signal(&bars.z_ready);
+    signal(&bars.x_ready);
     if (!wait(&bars.n_full, n, a, bars)) return;
     {
       uint32_t r[32], u[32];
@@ -529,8 +570,7 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
   if (a.state1) store_state<DK>(S, a.state1 + head, p, l);
 }
 
-// The row warps, one a quadrant of lanes: forwards O's part from the state gets its
-// decays (scale e^c) before N's is added, and O leaves; backwards dY is kept and
+// The row warps, one a quadrant of lanes: forwards O leaves; backwards dY is kept and
 // dV = beta dY leaves.  Rows leave by way of shared memory, 256 bytes together.
 template <int DK, bool REV>
 __device__ __forceinline__ void take_rows(const gsa_delta_t& p, const SeqArgs& a, const Seq& s,
@@ -547,28 +587,7 @@ __device__ __forceinline__ void take_rows(const gsa_delta_t& p, const SeqArgs& a
     const uint32_t ro = tmem + kRO + 128 * (n & 1);
     const int64_t slot = static_cast<int64_t>(s.chunk0 + at) * p.Hv + hv;
     const Block* blk = reinterpret_cast<const Block*>(sm.t(st));
-    if (!wait(&bars.full_a[st], turn, a, bars)) return;
-    if constexpr (!REV) {
-      if (!wait(&bars.r_full, n, a, bars)) return;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t r[16];
-        tmem_ld16(ro + 64 + 16 * q, r);
-        tc_wait_ld(r);
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 g = *reinterpret_cast<const float4*>(blk->grown + 16 * q + i);
-          r[i] = __float_as_uint(p.scale * g.x * __uint_as_float(r[i]));
-          r[i + 1] = __float_as_uint(p.scale * g.y * __uint_as_float(r[i + 1]));
-          r[i + 2] = __float_as_uint(p.scale * g.z * __uint_as_float(r[i + 2]));
-          r[i + 3] = __float_as_uint(p.scale * g.w * __uint_as_float(r[i + 3]));
-        }
-        tmem_st16(ro + 64 + 16 * q, r);
-      }
-      tc_wait_st();
-      signal(&bars.z_ready);
-      signal(&bars.empty_a[st]);
-    }
+    if (REV && !wait(&bars.full_a[st], turn, a, bars)) return;
     if (!wait(REV ? &bars.n_full : &bars.o_full, n, a, bars)) return;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -647,17 +666,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars.full_a[i], 1);
       mbar_init(&bars.full_b[i], 1);
-      mbar_init(&bars.empty_a[i], 1 + kComputeWarps + kRowWarps);
+      mbar_init(&bars.empty_a[i], 1 + kComputeWarps + (REV ? kRowWarps : 0));
       mbar_init(&bars.empty_b[i], 1);
     }
     mbar_init(&bars.s_ready, kComputeWarps);
     mbar_init(&bars.y_ready, kComputeWarps);
-    mbar_init(&bars.z_ready, REV ? kComputeWarps : kRowWarps);
     mbar_init(&bars.d_ready, kComputeWarps);
     mbar_init(&bars.x_ready, kComputeWarps);
     mbar_init(&bars.o_read, kRowWarps);
     mbar_init(&bars.rows, kRowWarps);
     mbar_init(&bars.r_full, 1);
+    mbar_init(&bars.o1_full, 1);
     mbar_init(&bars.n_full, 1);
     mbar_init(&bars.upd_full, 1);
     mbar_init(&bars.o_full, 1);
@@ -685,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kCopyWarp) {
       produce<DK, REV>(p, maps, a, s, hv, col0, sm, bars);
     } else if (warp == kIssueWarp) {
-      if ((threadIdx.x & 31) == 0) issue<DK, REV>(a, chunks, sm, bars);
+      issue<DK, REV>(a, chunks, sm, bars);
     } else if (warp < kIssueWarp) {
       take_rows<DK, REV>(p, a, s, hv, row, col0, tmem, sm, bars);
     }
