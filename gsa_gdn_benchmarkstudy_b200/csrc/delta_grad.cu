@@ -26,7 +26,10 @@ namespace delta {
 namespace {
 
 constexpr int kComputeWarps = 8;
-constexpr int kThreads = 32 * (kComputeWarps + 2);
+constexpr int kThreads = 384;  // whole warpgroups: two warps idle
+// Registers: 384 x 168 at launch = 256 x 216 (computing) + 128 x 72 (the others).
+constexpr int kLaunchRegs = 168, kComputeRegs = 216, kOtherRegs = 72;
+static_assert(256 * kComputeRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "register split");
 constexpr uint32_t kTmemCols = 512;
 
 // Shared memory.  K, Q and K again, 64 channels at a time, so that [K; Q] and [Q;
@@ -42,7 +45,10 @@ constexpr int kOffD = kOffY + 8 * kGroup;
 constexpr int kOffV = kOffD + 2 * static_cast<int>(kTile);
 constexpr int kOffA = kOffV + 2 * static_cast<int>(kTile);
 constexpr int kOffM = kOffA + static_cast<int>(kTile);
-constexpr int kSmem = kOffM + static_cast<int>(kTile) + 1024;
+constexpr int kOffG = kOffM + static_cast<int>(kTile);  // gates, of two heads in turn
+constexpr int kSmem = kOffG + 2 * static_cast<int>(sizeof(Gates)) + 1024;
+// The gradients of 64 tokens leave by way of A's and M's place, 256 bytes a token.
+constexpr int kRowBytes = 256;
 
 enum : uint32_t {
   kTo = 0,     // (dO S0^T)^T [channels][tokens]
@@ -57,6 +63,7 @@ enum : uint32_t {
 
 struct GradArgs {
   Table table;
+  const Block* blocks;
   const bf16* news;
   const bf16* states;
   const bf16* back;
@@ -70,7 +77,7 @@ struct GradArgs {
 struct Bars {
   uint64_t full_kq, empty_kq, full_h, empty_h;
   uint64_t ph1_full, ph2_ready, ph2_full, x_read, drain;
-  uint64_t meet;  // the computing warps, twice a head
+  uint64_t meet;  // the computing warps
   uint32_t tmem;
   int abort;
 };
@@ -114,7 +121,7 @@ __device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& m
                                         const DeltaMaps& more, const GradArgs& a,
                                         unsigned char* smem, Bars& bars) {
   const int lane = threadIdx.x & 31, group = p.Hv / p.Hk, rows = padded_dv(p.dv);
-  int items = 0, loads = 0;
+  int items = 0, loads = 0, heads = 0;
   bool ok = true;
   for (int64_t x = blockIdx.x; ok && x < a.items; x += gridDim.x) {
     const int chunk = static_cast<int>(x / p.Hk), hk = static_cast<int>(x % p.Hk);
@@ -146,7 +153,7 @@ __device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& m
       }
     }
     ++items;
-    for (int hv = hk * group; ok && hv < (hk + 1) * group; ++hv) {
+    for (int hv = hk * group; ok && hv < (hk + 1) * group; ++hv, ++heads) {
       const int64_t slot = static_cast<int64_t>(chunk) * p.Hv + hv;
       for (int col0 = 0; col0 < p.dv; col0 += 128) {
         ok = mbar_wait_warp(&bars.empty_h, (loads & 1) ^ 1, a.err, &bars.abort);
@@ -171,8 +178,12 @@ __device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& m
           __syncwarp();
         }
         if (lane == 0) {
-          mbar_arrive_expect_tx(&bars.full_h, (2 * (DK / 8) + 16) * wide +
+          mbar_arrive_expect_tx(&bars.full_h, (col0 ? 0 : sizeof(Gates)) +
+                                                  (2 * (DK / 8) + 16) * wide +
                                                   (int(tma_d) + int(tma_v)) * 2 * kTile);
+          if (col0 == 0)
+            bulk_load(smem + kOffG + (heads & 1) * sizeof(Gates), &a.blocks[slot].gates,
+                      sizeof(Gates), &bars.full_h);
           for (int i = 0; i < 2; ++i) {
             if (tma_d)
               tma_load_rows(smem + kOffD + i * kTile, &more.v, col0 + 64 * i, hv, c.begin, c.b,
@@ -276,9 +287,7 @@ struct Sums {  // per token; by quadrant of lanes where several warps have a par
   float row_m[2][kChunk], col_m[2][kChunk];           // E from M: rows (by half), columns (by quadrant)
   float low[2][kChunk];                               // sum_j l_ij k_i.k_j (by half)
   float yv[kChunk];                                   // dY_i.V_i
-  float cross[kComputeWarps];
-  float grown[kChunk], left[kChunk];
-  Decays d;
+  float cross[2][kComputeWarps];                      // <S0, dS1>, of two heads in turn
 };
 
 template <int DK>
@@ -290,7 +299,7 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
   const int group = p.Hv / p.Hk, rows = padded_dv(p.dv);
   const bool gate16 = p.gate_dtype == GSA_DTYPE_BF16;
   const int64_t qk_step = static_cast<int64_t>(p.Hk) * p.dk;
-  int items = 0, loads = 0, heads = 0;
+  int items = 0, loads = 0, heads = 0, meets = 0;
   auto until = [&](uint64_t* bar, int parity) {
     const bool ok = mbar_wait_warp(bar, parity & 1, a.err, &bars.abort);
     tc_fence_after();
@@ -331,147 +340,175 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
 #pragma unroll
     for (int i = 0; i < 32; ++i) gq[i] = gk[i] = 0.f;
     for (int hv = hk * group; hv < (hk + 1) * group; ++hv, ++heads) {
-      if (warp == 0) {
-        chunk_decays(p, c, hv, sum.d);
-        __syncwarp();
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          sum.grown[lane + 32 * e] = decay_from_start(sum.d, lane + 32 * e);
-          sum.left[lane + 32 * e] = decay_between(sum.d, kChunk - 1, lane + 32 * e);
-        }
-      }
-      signal(&bars.meet);
-      if (!until(&bars.meet, 2 * heads)) return;
-      // <S0, dS1>
+      const Gates& gates =
+          *reinterpret_cast<const Gates*>(smem + kOffG + (heads & 1) * sizeof(Gates));
+      // <S0, dS1>: a column and every second group of 8 channels a thread
       float cross = 0.f;
       for (int col0 = 0; col0 < p.dv; col0 += 128, ++loads) {
         if (!until(&bars.full_h, loads)) return;
-        const int wide = min(128, rows - col0);
-        for (int i = tid; i < DK / 8 * wide; i += 256) {
-          const int at = (i / wide) * kGroup + (i % wide) * 16;
-          const uint4 u = *reinterpret_cast<const uint4*>(smem + kOffS0 + at);
-          const uint4 w = *reinterpret_cast<const uint4*>(smem + kOffS1 + at);
-          const uint32_t us[4] = {u.x, u.y, u.z, u.w}, ws[4] = {w.x, w.y, w.z, w.w};
+        if (col0 + (tid & 127) < rows) {
+          const unsigned char* at = smem + (tid >> 7) * kGroup + (tid & 127) * 16;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            cross = fmaf(lo_of(us[e]), lo_of(ws[e]), cross);
-            cross = fmaf(hi_of(us[e]), hi_of(ws[e]), cross);
+          for (int i = 0; i < DK / 16; ++i) {
+            const uint4 u = *reinterpret_cast<const uint4*>(at + kOffS0 + 2 * i * kGroup);
+            const uint4 w = *reinterpret_cast<const uint4*>(at + kOffS1 + 2 * i * kGroup);
+            const uint32_t us[4] = {u.x, u.y, u.z, u.w}, ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              cross = fmaf(lo_of(us[e]), lo_of(ws[e]), cross);
+              cross = fmaf(hi_of(us[e]), hi_of(ws[e]), cross);
+            }
           }
         }
         signal(&bars.empty_h);
       }
 #pragma unroll
       for (int m = 16; m; m >>= 1) cross += __shfl_xor_sync(0xFFFFFFFFu, cross, m);
-      if (lane == 0) sum.cross[warp] = cross;
+      if (lane == 0) sum.cross[heads & 1][warp] = cross;
 
       if (!until(&bars.ph1_full, heads)) return;
-      // A^T (lanes of tokens j, columns i) and M (lanes of tokens i, columns j)
-      const bool first = quad < 2;
-      const int own = row & 63;  // j, or i
       uint32_t r[32], u[32];
-      tmem_ld32(tm + (first ? kPd : kPn) + t0, r);
-      tmem_ld32(tm + (first ? kKq : kKk) + t0, u);
-      tc_wait_ld(r, u);
-      {
-        float e[32], own_sum = 0.f, low = 0.f;
-        uint32_t packed[16];
-        const float hi0 = sum.d.hi[own], lo0 = sum.d.lo[own], beta0 = sum.d.beta[own];
+      float e[32];
+      const int own = row & 63;
+      const float hi0 = gates.hi[own], lo0 = gates.lo[own], beta0 = gates.beta[own];
+      float own_sum = 0.f;
+      if (quad < 2) {  // A^T: lanes are tokens j, columns i >= j
+        tmem_ld32(tm + kPd + t0, r);
+        tmem_ld32(tm + kKq + t0, u);
+        tc_wait_ld(r, u);
 #pragma unroll
-        for (int z = 0; z < 32; z += 2) {
-          float y[2];
+        for (int i = 0; i < 32; i += 4) {
+          const float4 h = *reinterpret_cast<const float4*>(gates.hi + t0 + i);
+          const float4 o = *reinterpret_cast<const float4*>(gates.lo + t0 + i);
+          const float hs[4] = {h.x, h.y, h.z, h.w}, os[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-          for (int f = 0; f < 2; ++f) {
-            const int other = t0 + z + f;
-            const float dh = sum.d.hi[other] - hi0, dl = sum.d.lo[other] - lo0;
-            // decays run from j to i >= j
-            const bool in = first ? other >= own : other < own;
-            const float w = in ? expf(first ? dh + dl : -(dh + dl)) : 0.f;
-            const float prod = __uint_as_float(r[z + f]), dot = __uint_as_float(u[z + f]);
-            const float l = in ? -prod * w : 0.f;
-            y[f] = first ? -p.scale * l : l * beta0;
-            e[z + f] = in ? y[f] * dot : 0.f;
-            own_sum += e[z + f];
-            low += in ? l * dot : 0.f;
+          for (int f = 0; f < 4; ++f) {
+            const float w = p.scale * exp_of((hs[f] - hi0) + (os[f] - lo0));
+            const float x = t0 + i + f >= own ? w * __uint_as_float(r[i + f]) : 0.f;
+            e[i + f] = t0 + i + f >= own ? x * __uint_as_float(u[i + f]) : 0.f;
+            own_sum += e[i + f];
+            r[i + f] = __float_as_uint(x);
           }
-          packed[z >> 1] = pack_bf16x2(y[0], y[1]);
         }
-        unsigned char* tile = smem + (first ? kOffA : kOffM);
+      } else {  // M: lanes are tokens i, columns j < i
+        float low = 0.f;
+        tmem_ld32(tm + kPn + t0, r);
+        tmem_ld32(tm + kKk + t0, u);
+        tc_wait_ld(r, u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(tile + sw128_offset(own, 4 * half + i)) = make_uint4(
-              packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
-        const float across = fold_lanes(e);  // lane l: column t0 + l over this warp's rows
-        if (first) {
-          sum.col_x[half][own] = own_sum;
-          sum.row_x[quad][t0 + lane] = across;
-        } else {
-          sum.row_m[half][own] = own_sum;
-          sum.col_m[quad - 2][t0 + lane] = across;
-          sum.low[half][own] = low;
-          tmem_ld32(tm + kPv + t0, r);
-          tc_wait_ld(r);
-          float diag = 0.f;
+        for (int i = 0; i < 32; i += 4) {
+          const float4 h = *reinterpret_cast<const float4*>(gates.hi + t0 + i);
+          const float4 o = *reinterpret_cast<const float4*>(gates.lo + t0 + i);
+          const float hs[4] = {h.x, h.y, h.z, h.w}, os[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) diag = own == t0 + i ? __uint_as_float(r[i]) : diag;
-          if ((own >> 5) == half) sum.yv[own] = diag;
+          for (int f = 0; f < 4; ++f) {
+            const bool in = t0 + i + f < own;
+            const float w = exp_of((hi0 - hs[f]) + (lo0 - os[f]));
+            const float l = in ? -w * __uint_as_float(r[i + f]) : 0.f;
+            const float dot = in ? __uint_as_float(u[i + f]) : 0.f;
+            low = fmaf(l, dot, low);
+            e[i + f] = l * beta0 * dot;
+            own_sum += e[i + f];
+            r[i + f] = __float_as_uint(l * beta0);
+          }
+        }
+        sum.low[half][own] = low;
+      }
+      {
+        unsigned char* tile = smem + (quad < 2 ? kOffA : kOffM);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t x[4];
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            x[f] = pack_bf16x2(__uint_as_float(r[8 * i + 2 * f]),
+                               __uint_as_float(r[8 * i + 2 * f + 1]));
+          *reinterpret_cast<uint4*>(tile + sw128_offset(own, 4 * half + i)) =
+              make_uint4(x[0], x[1], x[2], x[3]);
         }
       }
       fence_proxy_async_smem();  // A^T and M are read by the products
-      // channels: what S0 and dS1 give, and its products with q and k
+      signal(&bars.ph2_ready);
+      const float across = fold_lanes(e);  // lane l: column t0 + l over this warp's rows
+      if (quad < 2) {
+        sum.col_x[half][own] = own_sum;
+        sum.row_x[quad][t0 + lane] = across;
+      } else {
+        sum.row_m[half][own] = own_sum;
+        sum.col_m[quad - 2][t0 + lane] = across;
+        tmem_ld32(tm + kPv + t0, r);
+        tc_wait_ld(r);
+        float diag = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) diag = own == t0 + i ? __uint_as_float(r[i]) : diag;
+        if ((own >> 5) == half) sum.yv[own] = diag;
+      }
+      // lanes are channels: what S0 and dS1 give, times q and k, over the channels; and
+      // the gradients' part of it
       {
         const unsigned char* kt = smem + (row >> 6) * kKqkBytes + 2 * (row & 7);
         const int piece = (row & 63) >> 3;
         const bool real = row < DK;
-        float e[32];
         tmem_ld32(tm + kTo + t0, r);
         tc_wait_ld(r);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float v = real ? __uint_as_float(r[i]) : 0.f;
-          gq[i] = fmaf(p.scale * sum.grown[t0 + i], v, gq[i]);
-          e[i] = real ? v * __bfloat162float(*reinterpret_cast<const bf16*>(
-                                kt + kTile + sw128_offset(t0 + i, piece)))
-                      : 0.f;
+        for (int i = 0; i < 32; i += 4) {
+          const float4 g = *reinterpret_cast<const float4*>(gates.grown + t0 + i);
+          const float gs[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            const float v = real ? __uint_as_float(r[i + f]) : 0.f;
+            const float q = __uint_as_float(
+                static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(
+                    kt + kTile + sw128_offset(t0 + i + f, piece)))
+                << 16);
+            gq[i + f] = fmaf(p.scale * gs[f], v, gq[i + f]);
+            e[i + f] = real ? v * q : 0.f;
+          }
         }
         sum.qo[quad][t0 + lane] = fold_lanes(e);
         tmem_ld32(tm + kTy + t0, r);
         tmem_ld32(tm + kTn + t0, u);
         tc_wait_ld(r, u);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float v = real ? __uint_as_float(r[i]) : 0.f;
-          const float k = real ? __bfloat162float(*reinterpret_cast<const bf16*>(
-                                     kt + sw128_offset(t0 + i, piece)))
-                               : 0.f;
-          gk[i] = fmaf(-sum.grown[t0 + i] * sum.d.beta[t0 + i], v, gk[i]);
-          e[i] = v * k;
-          r[i] = __float_as_uint(k);
+        for (int i = 0; i < 32; i += 4) {
+          const float4 g = *reinterpret_cast<const float4*>(gates.both + t0 + i);
+          const float4 h = *reinterpret_cast<const float4*>(gates.left + t0 + i);
+          const float gs[4] = {g.x, g.y, g.z, g.w}, hs[4] = {h.x, h.y, h.z, h.w};
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            const float k =
+                real ? __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(
+                                           kt + sw128_offset(t0 + i + f, piece)))
+                                       << 16)
+                     : 0.f;
+            const float y = real ? __uint_as_float(r[i + f]) : 0.f;
+            const float n = real ? __uint_as_float(u[i + f]) : 0.f;
+            gk[i + f] = fmaf(hs[f], n, fmaf(-gs[f], y, gk[i + f]));
+            e[i + f] = y * k;
+            u[i + f] = __float_as_uint(n * k);
+          }
         }
         sum.ky[quad][t0 + lane] = fold_lanes(e);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float v = real ? __uint_as_float(u[i]) : 0.f;
-          gk[i] = fmaf(sum.left[t0 + i], v, gk[i]);
-          e[i] = v * __uint_as_float(r[i]);
-        }
+        for (int i = 0; i < 32; ++i) e[i] = __uint_as_float(u[i]);
         sum.kn[quad][t0 + lane] = fold_lanes(e);
       }
-      signal(&bars.ph2_ready);
       signal(&bars.meet);
-      if (!until(&bars.meet, 2 * heads + 1)) return;
+      if (!until(&bars.meet, meets++)) return;
       if (warp == 0) {  // two neighbouring tokens a lane
         float rs[2], gs[2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int t = 2 * lane + e;
-          const float g = sum.grown[t], beta = sum.d.beta[t];
+        for (int f = 0; f < 2; ++f) {
+          const int t = 2 * lane + f;
+          const float g = gates.grown[t];
           const float qo = (sum.qo[0][t] + sum.qo[1][t]) + (sum.qo[2][t] + sum.qo[3][t]);
           const float ky = (sum.ky[0][t] + sum.ky[1][t]) + (sum.ky[2][t] + sum.ky[3][t]);
           const float kn = (sum.kn[0][t] + sum.kn[1][t]) + (sum.kn[2][t] + sum.kn[3][t]);
           const float er = (sum.row_x[0][t] + sum.row_x[1][t]) + (sum.row_m[0][t] + sum.row_m[1][t]);
           const float ec = (sum.col_x[0][t] + sum.col_x[1][t]) + (sum.col_m[0][t] + sum.col_m[1][t]);
-          rs[e] = p.scale * g * qo - g * beta * ky + er - ec;
-          gs[e] = sum.left[t] * kn;
+          rs[f] = p.scale * g * qo - gates.both[t] * ky + er - ec;
+          gs[f] = gates.left[t] * kn;
           if (t < c.len)
             store_gate(a.dbeta, (row0 + t) * p.Hv + hv, gate16,
                        sum.yv[t] - g * ky + (sum.low[0][t] + sum.low[1][t]));
@@ -488,10 +525,10 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
         float before = __shfl_up_sync(0xFFFFFFFFu, prefix, 1);
         if (lane == 31) after = 0.f;
         if (lane == 0) before = 0.f;
-        float whole = lane < kComputeWarps ? sum.cross[lane] : 0.f;
+        float whole = lane < kComputeWarps ? sum.cross[heads & 1][lane] : 0.f;
 #pragma unroll
         for (int m = 16; m; m >>= 1) whole += __shfl_xor_sync(0xFFFFFFFFu, whole, m);
-        whole *= sum.grown[kChunk - 1];
+        whole *= gates.grown[kChunk - 1];
         const float dg0 = whole + before + (rs[0] + (rs[1] + after));
         const float dg1 = whole + (before + gs[0]) + (rs[1] + after);
         if (2 * lane < c.len) store_gate(a.dg, (row0 + 2 * lane) * p.Hv + hv, gate16, dg0);
@@ -510,13 +547,29 @@ __device__ __forceinline__ void compute(const gsa_delta_t& p, const GradArgs& a,
         gk[i] += __uint_as_float(u[i]);
       }
     }
-    if (row < p.dk) {
+    // rows leave by way of shared memory
+    unsigned char* mine = smem + kOffA + t0 * kRowBytes + 2 * row;
+    const int piece = (tid & 15) * 8, first = tid >> 4;
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (t0 + i < c.len) {
-          dq_out[(t0 + i) * qk_step + row] = __float2bfloat16_rn(gq[i]);
-          dk_out[(t0 + i) * qk_step + row] = __float2bfloat16_rn(gk[i]);
-        }
+    for (int z = 0; z < 2; ++z) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const uint32_t x = z ? pack_bf16x2(gk[i], gk[i + 1]) : pack_bf16x2(gq[i], gq[i + 1]);
+        *reinterpret_cast<uint16_t*>(mine + i * kRowBytes) = static_cast<uint16_t>(x);
+        *reinterpret_cast<uint16_t*>(mine + (i + 1) * kRowBytes) = static_cast<uint16_t>(x >> 16);
+      }
+      signal(&bars.meet);
+      if (!until(&bars.meet, meets++)) return;
+      bf16* out = z ? dk_out : dq_out;
+      if (piece < p.dk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (first + 16 * i < c.len)
+            *reinterpret_cast<uint4*>(out + (first + 16 * i) * qk_step + piece) =
+                *reinterpret_cast<const uint4*>(smem + kOffA + (first + 16 * i) * kRowBytes +
+                                                2 * piece);
+      signal(&bars.meet);
+      if (!until(&bars.meet, meets++)) return;
     }
   }
 }
@@ -553,12 +606,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kComputeWarps + 1)
-    produce<DK>(p, maps, more, a, smem, bars);
-  else if (warp == kComputeWarps) {
-    issue<DK>(p, a, smem_u32(smem), bars);
-  } else {
+  if (warp < kComputeWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
     compute<DK>(p, a, smem, bars, sum);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kComputeWarps + 1)
+      produce<DK>(p, maps, more, a, smem, bars);
+    else if (warp == kComputeWarps)
+      issue<DK>(p, a, smem_u32(smem), bars);
   }
   tc_fence_before();
   __syncthreads();
@@ -571,7 +627,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int DK>
 cudaError_t launch(const gsa_delta_t& p, const DeltaMaps& maps, const DeltaMaps& more,
                    const GradArgs& a, cudaStream_t stream) {
-  const cudaError_t e = allow_smem<grad_kernel<DK>>(kSmem);
+  cudaError_t e = need_regs<grad_kernel<DK>>(kLaunchRegs);
+  if (e != cudaSuccess) return e;
+  e = allow_smem<grad_kernel<DK>>(kSmem);
   if (e != cudaSuccess) return e;
   const int blocks = static_cast<int>(a.items < 148 ? a.items : 148);
   grad_kernel<DK><<<blocks, kThreads, kSmem, stream>>>(p, maps, more, a);
@@ -583,9 +641,9 @@ cudaError_t launch(const gsa_delta_t& p, const DeltaMaps& maps, const DeltaMaps&
 cudaError_t launch_grad(const gsa_delta_t& p, const DeltaMaps& maps, const DeltaMaps& more,
                         const DeltaGrads& g, const Saved& s, const Scratch& r, const Table& t,
                         int* err, cudaStream_t stream) {
-  const GradArgs a = {t,     s.news, s.states, r.back,  r.states,
-                      g.dout, g.dq,  g.dk,     g.dv,    g.dg,
-                      g.dbeta, max_chunks(p) * p.Hk, err};
+  const GradArgs a = {t,      s.blocks, s.news, s.states, r.back, r.states,
+                      g.dout, g.dq,     g.dk,   g.dv,     g.dg,   g.dbeta,
+                      max_chunks(p) * p.Hk, err};
   if (a.items == 0) return cudaSuccess;
   return p.dk <= 64 ? launch<64>(p, maps, more, a, stream) : launch<128>(p, maps, more, a, stream);
 }

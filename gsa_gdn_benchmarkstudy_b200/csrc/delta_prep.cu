@@ -47,14 +47,14 @@ constexpr int kPrepThreads = 128;
 constexpr int kLdL = kChunk + 4;
 constexpr int kLdX = 36;
 
-// K and Q, whose place the block's image takes once their products are in
-// registers; L, which becomes T in place; a 32 x 32 product.
+// K and Q, whose place P's tiles and a 32 x 32 product take once their products are
+// in registers; L, which becomes T in place.
+constexpr int kPrepTiles = 2 * static_cast<int>(kTile) + 32 * kLdX * 4;
 template <int DK>
 constexpr int prep_smem() {
-  return (2 * (DK / 64) * static_cast<int>(kTile) > static_cast<int>(sizeof(Block))
-              ? 2 * (DK / 64) * static_cast<int>(kTile)
-              : static_cast<int>(sizeof(Block))) +
-         (kChunk * kLdL + 32 * kLdX) * 4 + 1024;
+  return (2 * (DK / 64) * static_cast<int>(kTile) > kPrepTiles ? 2 * (DK / 64) * static_cast<int>(kTile)
+                                                               : kPrepTiles) +
+         kChunk * kLdL * 4 + 1024;
 }
 
 // out[r][c] = sign sum_k a[r][k] b[k][c] for a 32 x 32 block, 2 x 4 a thread.
@@ -145,15 +145,15 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t
   const Chunk c = chunk_at(p, table, blockIdx.x);
   if (!c.valid || c.gap) return;
   const uint32_t K = smem_u32(smem), Q = K + (DK / 64) * kTile;
-  Block* img = reinterpret_cast<Block*>(smem);
-  float* L = reinterpret_cast<float*>(smem + prep_smem<DK>() - 1024) - kChunk * kLdL - 32 * kLdX;
-  float* X = L + kChunk * kLdL;
+  float* X = reinterpret_cast<float*>(smem + 2 * kTile);
+  float* L = reinterpret_cast<float*>(smem + prep_smem<DK>() - 1024) - kChunk * kLdL;
   copy_rows(K, rows_at(p.k, p.k_stride, c.b, c.begin, hk), p.k_stride[1], c.len, DK, p.dk, tid,
             kPrepThreads);
   copy_rows(Q, rows_at(p.q, p.q_stride, c.b, c.begin, hk), p.q_stride[1], c.len, DK, p.dk, tid,
             kPrepThreads);
-  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-  if (tid < 32) chunk_decays(p, c, hk * group, d);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  if (tid < 32) chunk_decays(p, c, hk * group, d);  // beside the copies
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   float kk[8][4] = {}, qk[8][4] = {};
 #pragma unroll
@@ -172,39 +172,53 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t
     }
   }
   for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
-    __syncthreads();  // K and Q, or the last head's image, are read
+    __syncthreads();  // K and Q, or the last head's tiles, are read
     if (hv > hk * group) {
       if (tid < 32) chunk_decays(p, c, hv, d);
       __syncthreads();
     }
+    Block* blk = blocks + static_cast<int64_t>(blockIdx.x) * p.Hv + hv;
     if (tid < kChunk) {
       const float grown = decay_from_start(d, tid);
-      img->grown[tid] = grown;
-      img->beta[tid] = d.beta[tid];
-      img->both[tid] = d.beta[tid] * grown;
-      img->left[tid] = decay_between(d, kChunk - 1, tid);
+      blk->gates.grown[tid] = grown;
+      blk->gates.beta[tid] = d.beta[tid];
+      blk->gates.left[tid] = decay_between(d, kChunk - 1, tid);
+      blk->gates.both[tid] = d.beta[tid] * grown;
+      blk->gates.hi[tid] = d.hi[tid];
+      blk->gates.lo[tid] = d.lo[tid];
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int e = 0; e < 2; ++e) {
+      const int r = m0 + gid + 8 * e;
+      const float hi_r = d.hi[r], lo_r = d.lo[r], beta_r = d.beta[r];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = m0 + gid + 8 * e, cc = 8 * j + 2 * tig;
-        float l[2] = {0.f, 0.f}, x[2] = {0.f, 0.f};
+      for (int j = 0; j < 8; ++j) {
+        const int cc = 8 * j + 2 * tig;
+        const float2 hc = *reinterpret_cast<const float2*>(d.hi + cc);
+        const float2 lc = *reinterpret_cast<const float2*>(d.lo + cc);
+        float l[2], x[2];
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
-          if (r >= cc + f) {
-            const float w = decay_between(d, r, cc + f);
-            if (r > cc + f) l[f] = d.beta[r] * w * kk[j][2 * e + f];
-            x[f] = p.scale * w * qk[j][2 * e + f];
-          }
+        for (int f = 0; f < 2; ++f) {
+          const float w = exp_of((hi_r - (f ? hc.y : hc.x)) + (lo_r - (f ? lc.y : lc.x)));
+          l[f] = r > cc + f ? beta_r * w * kk[j][2 * e + f] : 0.f;
+          x[f] = r >= cc + f ? p.scale * w * qk[j][2 * e + f] : 0.f;
+        }
         *reinterpret_cast<float2*>(L + r * kLdL + cc) = make_float2(l[0], l[1]);
         uint32_t hi, lo;
         split(x[0], x[1], hi, lo);
         const uint32_t at = sw128_offset(r, j) + 4 * tig;
-        *reinterpret_cast<uint32_t*>(img->p_hi + at) = hi;
-        *reinterpret_cast<uint32_t*>(img->p_lo + at) = lo;
+        *reinterpret_cast<uint32_t*>(smem + at) = hi;
+        *reinterpret_cast<uint32_t*>(smem + kTile + at) = lo;
       }
+    }
     __syncthreads();
+    {  // P leaves while T is made
+      uint4* dst = reinterpret_cast<uint4*>(blk->p_hi);
+      const uint4* src = reinterpret_cast<const uint4*>(smem);
+#pragma unroll
+      for (int i = 0; i < kPBytes / 16 / kPrepThreads; ++i)
+        dst[tid + i * kPrepThreads] = src[tid + i * kPrepThreads];
+    }
     invert(L, X);
 #pragma unroll
     for (int i = 0; i < kChunk * 8 / kPrepThreads; ++i) {
@@ -216,13 +230,9 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t
       split(u.z, u.w, hi.y, lo.y);
       split(v.x, v.y, hi.z, lo.z);
       split(v.z, v.w, hi.w, lo.w);
-      *reinterpret_cast<uint4*>(img->t_hi + sw128_offset(r, piece)) = hi;
-      *reinterpret_cast<uint4*>(img->t_lo + sw128_offset(r, piece)) = lo;
+      *reinterpret_cast<uint4*>(blk->t_hi + sw128_offset(r, piece)) = hi;
+      *reinterpret_cast<uint4*>(blk->t_lo + sw128_offset(r, piece)) = lo;
     }
-    __syncthreads();
-    uint4* dst = reinterpret_cast<uint4*>(blocks + static_cast<int64_t>(blockIdx.x) * p.Hv + hv);
-    const uint4* src = reinterpret_cast<const uint4*>(img);
-    for (int i = tid; i < static_cast<int>(sizeof(Block) / 16); i += kPrepThreads) dst[i] = src[i];
   }
 }
 

@@ -411,11 +411,11 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
     tc_wait_st();
     signal(&bars.s_ready);
     if (!wait(&bars.full_a[st], turn, a, bars)) return;
-    const Block* blk = reinterpret_cast<const Block*>(sm.t(st));
+    const Gates* gates = reinterpret_cast<const Gates*>(sm.t(st) + 2 * kTile);
     float y[32];
     uint32_t hi[16];
-    load_values(y, sm.v(st), blk->beta, 1.f, l);  // beside the first product
-    whole = blk->grown[kChunk - 1];
+    load_values(y, sm.v(st), gates->beta, 1.f, l);  // beside the first product
+    whole = gates->grown[kChunk - 1];
     if (!wait(&bars.r_full, n, a, bars)) return;
     {
       uint32_t r[32];
@@ -423,7 +423,7 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
       tc_wait_ld(r);
 #pragma unroll
       for (int i = 0; i < 32; i += 4) {  // beta V - (beta e^c) R
-        const float4 g = *reinterpret_cast<const float4*>(blk->both + t0 + i);
+        const float4 g = *reinterpret_cast<const float4*>(gates->both + t0 + i);
         y[i] = fmaf(-g.x, __uint_as_float(r[i]), y[i]);
         y[i + 1] = fmaf(-g.y, __uint_as_float(r[i + 1]), y[i + 1]);
         y[i + 2] = fmaf(-g.z, __uint_as_float(r[i + 2]), y[i + 2]);
@@ -440,7 +440,7 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
       tc_wait_ld(r);
 #pragma unroll
       for (int i = 0; i < 32; i += 4) {
-        const float4 g = *reinterpret_cast<const float4*>(blk->grown + t0 + i);
+        const float4 g = *reinterpret_cast<const float4*>(gates->grown + t0 + i);
         r[i] = __float_as_uint(p.scale * g.x * __uint_as_float(r[i]));
         r[i + 1] = __float_as_uint(p.scale * g.y * __uint_as_float(r[i + 1]));
         r[i + 2] = __float_as_uint(p.scale * g.z * __uint_as_float(r[i + 2]));
@@ -460,7 +460,7 @@ __device__ __forceinline__ void walk(const gsa_delta_t& p, const SeqArgs& a, con
       float x[32];
 #pragma unroll
       for (int i = 0; i < 32; i += 4) {
-        const float4 g = *reinterpret_cast<const float4*>(blk->left + t0 + i);
+        const float4 g = *reinterpret_cast<const float4*>(gates->left + t0 + i);
         x[i] = g.x * y[i];
         x[i + 1] = g.y * y[i + 1];
         x[i + 2] = g.z * y[i + 2];
@@ -517,8 +517,8 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
     tc_wait_st();
     signal(&bars.s_ready);
     if (!wait(&bars.full_a[st], turn, a, bars)) return;
-    const Block* blk = reinterpret_cast<const Block*>(sm.t(st));
-    whole = blk->grown[kChunk - 1];
+    const Gates* gates = reinterpret_cast<const Gates*>(sm.t(st) + 2 * kTile);
+    whole = gates->grown[kChunk - 1];
     float y[32];
     uint32_t hi[16];
     if (!wait(&bars.r_full, n, a, bars)) return;
@@ -529,7 +529,7 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
       tc_wait_ld(r, u);
 #pragma unroll
       for (int i = 0; i < 32; i += 4) {
-        const float4 g = *reinterpret_cast<const float4*>(blk->left + t0 + i);
+        const float4 g = *reinterpret_cast<const float4*>(gates->left + t0 + i);
         y[i] = fmaf(g.x, __uint_as_float(r[i]), __uint_as_float(u[i]));
         y[i + 1] = fmaf(g.y, __uint_as_float(r[i + 1]), __uint_as_float(u[i + 1]));
         y[i + 2] = fmaf(g.z, __uint_as_float(r[i + 2]), __uint_as_float(u[i + 2]));
@@ -539,7 +539,7 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
     put_tokens(y, l.tmem + kS, l, hi);
     tc_wait_st();
     signal(&bars.y_ready);
-    load_values(y, sm.v(st), blk->grown, p.scale, l);  // beside the product with T
+    load_values(y, sm.v(st), gates->grown, p.scale, l);  // beside the product with T
     put_tokens(y, l.tmem + kD, l, hi);
     tc_wait_st();
     signal(&bars.x_ready);
@@ -551,7 +551,7 @@ __device__ __forceinline__ void walk_back(const gsa_delta_t& p, const SeqArgs& a
       tc_wait_ld(r, u);
 #pragma unroll
       for (int i = 0; i < 32; i += 4) {
-        const float4 g = *reinterpret_cast<const float4*>(blk->both + t0 + i);
+        const float4 g = *reinterpret_cast<const float4*>(gates->both + t0 + i);
         y[i] = -g.x * (__uint_as_float(r[i]) + __uint_as_float(u[i]));
         y[i + 1] = -g.y * (__uint_as_float(r[i + 1]) + __uint_as_float(u[i + 1]));
         y[i + 2] = -g.z * (__uint_as_float(r[i + 2]) + __uint_as_float(u[i + 2]));
@@ -586,7 +586,7 @@ __device__ __forceinline__ void take_rows(const gsa_delta_t& p, const SeqArgs& a
     const int st = n % kStages, turn = n / kStages, at = REV ? chunks - 1 - n : n;
     const uint32_t ro = tmem + kRO + 128 * (n & 1);
     const int64_t slot = static_cast<int64_t>(s.chunk0 + at) * p.Hv + hv;
-    const Block* blk = reinterpret_cast<const Block*>(sm.t(st));
+    const Gates* gates = reinterpret_cast<const Gates*>(sm.t(st) + 2 * kTile);
     if (REV && !wait(&bars.full_a[st], turn, a, bars)) return;
     if (!wait(REV ? &bars.n_full : &bars.o_full, n, a, bars)) return;
 #pragma unroll
@@ -611,7 +611,7 @@ __device__ __forceinline__ void take_rows(const gsa_delta_t& p, const SeqArgs& a
                 make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(blk->beta + 16 * q + i);
+          const float4 b = *reinterpret_cast<const float4*>(gates->beta + 16 * q + i);
           r[i] = __float_as_uint(b.x * __uint_as_float(r[i]));
           r[i + 1] = __float_as_uint(b.y * __uint_as_float(r[i + 1]));
           r[i + 2] = __float_as_uint(b.z * __uint_as_float(r[i + 2]));
@@ -720,17 +720,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int DK, bool REV>
 cudaError_t launch(const gsa_delta_t& p, const DeltaMaps& m, const SeqArgs& a,
                    cudaStream_t stream) {
-  // the split of setmaxnreg is valid only for the register count it was written for: with
-  // fewer at launch its `inc` would wait for registers that do not exist
-  static std::atomic<int> regs{0};
-  if (regs.load(std::memory_order_acquire) == 0) {
-    cudaFuncAttributes f;
-    const cudaError_t e = cudaFuncGetAttributes(&f, seq_kernel<DK, REV>);
-    if (e != cudaSuccess) return e;
-    regs.store(f.numRegs, std::memory_order_release);
-  }
-  if (regs.load(std::memory_order_acquire) != kLaunchRegs) return cudaErrorNotSupported;
-  const cudaError_t e = allow_smem<seq_kernel<DK, REV>>(seq_smem<DK>());
+  cudaError_t e = need_regs<seq_kernel<DK, REV>>(kLaunchRegs);
+  if (e != cudaSuccess) return e;
+  e = allow_smem<seq_kernel<DK, REV>>(seq_smem<DK>());
   if (e != cudaSuccess) return e;
   const int seqs = p.N + (!REV && p.cu_seqlens ? 2 : 0);
   seq_kernel<DK, REV><<<dim3(seqs, p.Hv, (p.dv + kCols - 1) / kCols), kThreads, seq_smem<DK>(),

@@ -95,6 +95,8 @@ __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& 
                                f2_pack(-1.f, -1.f), f2_pack(x, y));
   lo = pack_bf16x2(f2_lo(rest), f2_hi(rest));
 }
+// e^x on the MUFU: 2^-22 of the value, and x log2(e) rounded once: 2^-24 |x|.
+__device__ __forceinline__ float exp_of(float x) { return fast_ex2(x * 1.4426950408889634f); }
 __device__ __forceinline__ float lo_of(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float hi_of(uint32_t r) { return __uint_as_float(r & 0xFFFF0000u); }
 
@@ -129,20 +131,42 @@ __device__ __forceinline__ void tma_load_rows(void* dst, const CUtensorMap* map,
       : "memory");
 }
 
+// A split of registers by setmaxnreg is valid only for the count at launch that it
+// was written for: with fewer, its `inc` would wait for registers that do not exist.
+template <auto Kernel>
+cudaError_t need_regs(int expected) {
+  static std::atomic<int> regs{0};
+  int r = regs.load(std::memory_order_acquire);
+  if (r == 0) {
+    cudaFuncAttributes f;
+    const cudaError_t e = cudaFuncGetAttributes(&f, Kernel);
+    if (e != cudaSuccess) return e;
+    r = f.numRegs;
+    regs.store(r, std::memory_order_release);
+  }
+  return r == expected ? cudaSuccess : cudaErrorNotSupported;
+}
+
 // ---------------------------------------------------------------- workspace
 // For each chunk and value head, T and P as pairs of swizzled tiles with the
 // decays that go with them.
-struct __align__(16) Block {
-  unsigned char t_hi[kTile], t_lo[kTile];
+struct __align__(16) Gates {
   float grown[kChunk];  // e^{c_i}
   float beta[kChunk];
   float left[kChunk];   // e^{c_64 - c_i}
   float both[kChunk];   // beta_i e^{c_i}
+  float hi[kChunk];     // c_i = hi + lo
+  float lo[kChunk];
+  float pad[2 * kChunk];
+};
+struct __align__(16) Block {
+  unsigned char t_hi[kTile], t_lo[kTile];
+  Gates gates;
   unsigned char p_hi[kTile], p_lo[kTile];
 };
-constexpr int kTBytes = 2 * static_cast<int>(kTile) + 1024;  // T and the decays
+constexpr int kTBytes = 2 * static_cast<int>(kTile + sizeof(Gates) / 2);  // T and the gates
 constexpr int kPBytes = 2 * static_cast<int>(kTile);
-static_assert(sizeof(Block) == kTBytes + kPBytes, "block");
+static_assert(sizeof(Gates) == 2048 && sizeof(Block) == kTBytes + kPBytes, "block");
 
 __host__ __device__ inline int padded_dk(int dk) { return dk <= 64 ? 64 : 128; }
 // Rows of the images below: the value columns, rounded up to whole tiles.
