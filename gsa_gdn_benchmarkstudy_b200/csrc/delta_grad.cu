@@ -128,31 +128,34 @@ __device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& m
     const Chunk c = chunk_at(p, a.table, chunk);
     if (!c.valid || c.gap) continue;
     const bool whole = c.len == kChunk || !p.cu_seqlens;
-    ok = mbar_wait_warp(&bars.empty_kq, (items & 1) ^ 1, a.err, &bars.abort);
-    if (!ok) break;
-    if (!whole) {
-      for (int i = 0; i < DK / 64; ++i) {
-        const uint32_t t = smem_u32(smem) + i * kKqkBytes;
-        const bf16* k = rows_at(p.k, p.k_stride, c.b, c.begin, hk) + 64 * i;
-        copy_rows(t, k, p.k_stride[1], c.len, 64, p.dk - 64 * i, lane, 32);
-        copy_rows(t + 2 * kTile, k, p.k_stride[1], c.len, 64, p.dk - 64 * i, lane, 32);
-        copy_rows(t + kTile, rows_at(p.q, p.q_stride, c.b, c.begin, hk) + 64 * i, p.q_stride[1],
-                  c.len, 64, p.dk - 64 * i, lane, 32);
+    // K and Q come behind the first head's operands, whose place is free earlier
+    auto load_kq = [&] {
+      if (!mbar_wait_warp(&bars.empty_kq, (items & 1) ^ 1, a.err, &bars.abort)) return false;
+      if (!whole) {
+        for (int i = 0; i < DK / 64; ++i) {
+          const uint32_t t = smem_u32(smem) + i * kKqkBytes;
+          const bf16* k = rows_at(p.k, p.k_stride, c.b, c.begin, hk) + 64 * i;
+          copy_rows(t, k, p.k_stride[1], c.len, 64, p.dk - 64 * i, lane, 32);
+          copy_rows(t + 2 * kTile, k, p.k_stride[1], c.len, 64, p.dk - 64 * i, lane, 32);
+          copy_rows(t + kTile, rows_at(p.q, p.q_stride, c.b, c.begin, hk) + 64 * i, p.q_stride[1],
+                    c.len, 64, p.dk - 64 * i, lane, 32);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.full_kq);
+      } else if (lane == 0) {
+        mbar_arrive_expect_tx(&bars.full_kq, DK / 64 * kKqkBytes);
+        for (int i = 0; i < DK / 64; ++i) {
+          unsigned char* t = smem + i * kKqkBytes;
+          tma_load_rows(t, &maps.k, 64 * i, hk, c.begin, c.b, &bars.full_kq);
+          tma_load_rows(t + kTile, &maps.q, 64 * i, hk, c.begin, c.b, &bars.full_kq);
+          tma_load_rows(t + 2 * kTile, &maps.k, 64 * i, hk, c.begin, c.b, &bars.full_kq);
+        }
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.full_kq);
-    } else if (lane == 0) {
-      mbar_arrive_expect_tx(&bars.full_kq, DK / 64 * kKqkBytes);
-      for (int i = 0; i < DK / 64; ++i) {
-        unsigned char* t = smem + i * kKqkBytes;
-        tma_load_rows(t, &maps.k, 64 * i, hk, c.begin, c.b, &bars.full_kq);
-        tma_load_rows(t + kTile, &maps.q, 64 * i, hk, c.begin, c.b, &bars.full_kq);
-        tma_load_rows(t + 2 * kTile, &maps.k, 64 * i, hk, c.begin, c.b, &bars.full_kq);
-      }
-    }
-    ++items;
+      ++items;
+      return true;
+    };
     for (int hv = hk * group; ok && hv < (hk + 1) * group; ++hv, ++heads) {
       const int64_t slot = static_cast<int64_t>(chunk) * p.Hv + hv;
       for (int col0 = 0; col0 < p.dv; col0 += 128) {
@@ -207,6 +210,8 @@ __device__ __forceinline__ void produce(const gsa_delta_t& p, const DeltaMaps& m
           bulk_load(smem + kOffY + lane * kGroup, a.back + from, wide, &bars.full_h);
         }
         ++loads;
+        __syncwarp();
+        if (hv == hk * group && col0 == 0 && !(ok = load_kq())) break;
       }
     }
   }
