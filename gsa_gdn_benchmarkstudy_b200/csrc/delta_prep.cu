@@ -249,10 +249,17 @@ cudaError_t launch_prep(const gsa_delta_t& p, const Table& t, Block* blocks, cud
 
 }  // namespace
 
-int64_t bf16_saved_bytes(const gsa_delta_t& p, bool save) {
+namespace {
+// The segments' floats lie behind what the backward pass reads.
+int64_t cuts_offset(const gsa_delta_t& p, bool save) {
   const int64_t n = max_chunks(p) * p.Hv;
-  return table_bytes(p) + n * (static_cast<int64_t>(sizeof(Block)) +
-                               (save ? 2 * (news_elems(p) + state_elems(p)) : 0));
+  return (table_bytes(p) + n * (static_cast<int64_t>(sizeof(Block)) +
+                                (save ? 2 * (news_elems(p) + state_elems(p)) : 0)) + 15) / 16 * 16;
+}
+}  // namespace
+
+int64_t bf16_saved_bytes(const gsa_delta_t& p, bool save) {
+  return cuts_offset(p, save) + 4 * segment_floats(p);
 }
 int64_t bf16_scratch_bytes(const gsa_delta_t& p) {
   return 2 * max_chunks(p) * p.Hv * (news_elems(p) + state_elems(p));
@@ -264,9 +271,17 @@ cudaError_t bf16_forward(const gsa_delta_t& p, const DeltaMaps& m, void* o, floa
   const cudaError_t e = p.dk <= 64 ? launch_prep<64>(p, t, s.blocks, stream)
                                    : launch_prep<128>(p, t, s.blocks, stream);
   if (e != cudaSuccess) return e;
-  const SeqArgs a = {t,           s.blocks,  nullptr, o, p.initial_state,
-                     final_state, save ? s.news : nullptr, save ? s.states : nullptr, err};
-  return launch_seq(p, m, a, false, stream);
+  SeqArgs a = {};
+  a.table = t;
+  a.blocks = s.blocks;
+  a.out = o;
+  a.state0 = p.initial_state;
+  a.state1 = final_state;
+  a.rows = save ? s.news : nullptr;
+  a.states = save ? s.states : nullptr;
+  a.err = err;
+  return launch_forward(
+      p, m, a, reinterpret_cast<float*>(static_cast<char*>(ws) + cuts_offset(p, save)), stream);
 }
 cudaError_t bf16_backward(const gsa_delta_t& p, const DeltaMaps& m, const DeltaMaps& more,
                           const DeltaGrads& g, void* saved, void* scratch, int* err,
@@ -274,8 +289,17 @@ cudaError_t bf16_backward(const gsa_delta_t& p, const DeltaMaps& m, const DeltaM
   const Saved s = saved_at(p, saved);
   const Scratch r = scratch_at(p, scratch);
   const Table t = table_at(saved, p.N);
-  const SeqArgs a = {t, s.blocks, g.dout, g.dv, g.dfinal, g.dinitial, r.back, r.states, err};
-  const cudaError_t e = launch_seq(p, more, a, true, stream);
+  SeqArgs a = {};
+  a.table = t;
+  a.blocks = s.blocks;
+  a.in = g.dout;
+  a.out = g.dv;
+  a.state0 = g.dfinal;
+  a.state1 = g.dinitial;
+  a.rows = r.back;
+  a.states = r.states;
+  a.err = err;
+  const cudaError_t e = launch_backward(p, more, a, stream);
   if (e != cudaSuccess) return e;
   return launch_grad(p, m, more, g, s, r, t, err, stream);
 }

@@ -207,6 +207,20 @@ inline Scratch scratch_at(const gsa_delta_t& p, void* ws) {
   return {b, b + n * news_elems(p)};
 }
 
+// Long sequences with few heads are cut into segments that run side by side
+// (forwards).  What a segment does to a state is affine, S -> M S + B: a first pass
+// finds M and B of every segment but the last, a small kernel goes through them from
+// segment to segment, and a second pass runs all segments from their states.
+struct Segments {
+  int count;   // segments a sequence, 1: uncut
+  int chunks;  // chunks a segment (the last may have fewer)
+};
+Segments segments_of(const gsa_delta_t& p);
+inline int64_t segment_floats(const gsa_delta_t& p) {
+  const int64_t cuts = static_cast<int64_t>(p.N) * (segments_of(p).count - 1) * p.Hv;
+  return cuts * p.dk * (2 * static_cast<int64_t>(p.dv) + p.dk);  // B, S, M
+}
+
 // Launches of the parts (delta_seq.cu, delta_grad.cu).
 struct SeqArgs {
   Table table;
@@ -220,9 +234,14 @@ struct SeqArgs {
   bf16* rows;            // N (forwards; nullptr: inference) or dY
   bf16* states;          // S0 or dS1
   int* err;
+  Segments seg;
+  float *seg_b, *seg_s, *seg_m;  // [sequence][cut][head]: B, S [dk][dv], M [dk][dk]
 };
-cudaError_t launch_seq(const gsa_delta_t& p, const DeltaMaps& m, const SeqArgs& a, bool reverse,
-                       cudaStream_t stream);
+// Forwards: `cuts` holds segment_floats() floats, 16-byte aligned.
+cudaError_t launch_forward(const gsa_delta_t& p, const DeltaMaps& m, SeqArgs a, float* cuts,
+                           cudaStream_t stream);
+cudaError_t launch_backward(const gsa_delta_t& p, const DeltaMaps& m, SeqArgs a,
+                            cudaStream_t stream);
 // maps: q, k, v; more.v: dO.
 cudaError_t launch_grad(const gsa_delta_t& p, const DeltaMaps& maps, const DeltaMaps& more,
                         const DeltaGrads& g, const Saved& s, const Scratch& r, const Table& t,

@@ -78,6 +78,27 @@ def test_head_layouts(dtype, dims):
     check_forward(a, dtype, scale=0.3, initial=r(2, Hv, dk, dv))
 
 
+@pytest.mark.parametrize("shape", [(1, 1024, 1, 1, 128, 128), (1, 1500, 1, 2, 64, 72),
+                                   (2, 2111, 2, 2, 104, 200), (1, 3000, 2, 4, 128, 64)])
+@pytest.mark.parametrize("start", [False, True])
+def test_long_sequences_of_few_heads(shape, start):
+    """Long enough to be cut into segments that run side by side: states, outputs, gradients."""
+    B, T, Hk, Hv, dk, dv = shape
+    *a, r = make(*shape, "bf16", "bf16", seed=T, rate=0.05)  # slow decays: the cuts matter
+    S0 = 0.5 * r(B, Hv, dk, dv) if start else None
+    check_forward(a, "bf16", initial=S0)
+    if not start:
+        return
+    do, dS = r(B, T, Hv, dv).bfloat16(), r(B, Hv, dk, dv)
+    got = grads_of(lambda *x: gsa.gated_delta_rule(*x[:5], initial_state=x[5],
+                                                   output_final_state=True), a + [S0], [do, dS])
+    want = grads_of(lambda *x: delta_ref(*x[:5], dk ** -0.5, x[5]),
+                    [t.double() for t in a + [S0]], [do.double(), dS.double()])
+    for name, x, y in zip(("q", "k", "v", "g", "beta", "S0"), got, want):
+        tol = TOL["state", "bf16"] if name == "S0" else TOL["grad", "bf16"]
+        assert rel(x, y) <= tol, (name, rel(x, y))
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("lens", [[5], [0, 64, 1, 0, 130, 63], [200, 3], [0, 0], [65, 65, 65]])
 @pytest.mark.parametrize("pad", [(0, 0), (7, 70)])
