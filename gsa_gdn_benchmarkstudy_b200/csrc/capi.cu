@@ -1007,8 +1007,9 @@ int check_delta_rule(const gsa_delta_t* p) {
   }
   // the kernels count tokens and chunks in 32 bits
   if (static_cast<int64_t>(p->T) + p->N > INT32_MAX - 256 ||
-      static_cast<int64_t>(p->B) * (p->T / 64 + 1) > INT32_MAX - 256)
-    return set_error(GSA_ERR_UNSUPPORTED, "too many tokens");
+      static_cast<int64_t>(p->B) * (p->T / 64 + 1) > INT32_MAX - 256 ||
+      (static_cast<int64_t>(p->N) + 2) * p->Hv * 16 > INT32_MAX)
+    return set_error(GSA_ERR_UNSUPPORTED, "too many tokens, or sequences times heads");
   return GSA_OK;
 }
 }  // namespace

@@ -51,16 +51,20 @@ __device__ __forceinline__ float bounded_decay(float g) { return g < -110.0f ? -
 //   seq_begin[s], seq_len[s], seq_chunk[s]  first row, rows and first chunk of
 //     "sequence" s; s = N and N + 1 stand for the rows before the first and
 //     behind the last sequence, which get zeros;
+//   order[i]  the i-th longest "sequence" (as they come where they are more than
+//     kSorted): blocks that start last are short;
 //   chunk_seq[c]  the sequence of chunk c, -1 for an unused one.
 struct Table {
   int* seq_begin;
   int* seq_len;
   int* seq_chunk;
+  int* order;
   int* chunk_seq;
 };
+constexpr int kSorted = 1024;
 __host__ __device__ inline Table table_at(void* base, int N) {
   int* p = static_cast<int*>(base);
-  return {p, p + (N + 2), p + 2 * (N + 2), p + 3 * (N + 2)};
+  return {p, p + (N + 2), p + 2 * (N + 2), p + 3 * (N + 2), p + 4 * (N + 2)};
 }
 // Chunks that B * T rows in N sequences can have.
 inline int64_t max_chunks(const gsa_delta_t& p) {
@@ -69,7 +73,7 @@ inline int64_t max_chunks(const gsa_delta_t& p) {
 }
 inline int64_t table_bytes(const gsa_delta_t& p) {
   if (!p.cu_seqlens) return 0;
-  return (4 * (3 * (static_cast<int64_t>(p.N) + 2) + max_chunks(p)) + 255) / 256 * 256;
+  return (4 * (4 * (static_cast<int64_t>(p.N) + 2) + max_chunks(p)) + 255) / 256 * 256;
 }
 
 // A sequence: batch row, first token, tokens, first chunk; `gap`: no sequence

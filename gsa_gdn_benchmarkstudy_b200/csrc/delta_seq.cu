@@ -670,7 +670,7 @@ __device__ __forceinline__ void take_rows(const gsa_delta_t& p, const SeqArgs& a
   }
 }
 
-// Block (sequence or segment, value head, 128 columns).
+// Block (sequence or segment, longest first, and value head; 128 columns).
 template <int DK, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     seq_kernel(const gsa_delta_t p, const __grid_constant__ DeltaMaps maps, const SeqArgs a) {
@@ -679,14 +679,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Smem<DK> sm = {
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~1023ull)};
   __shared__ Bars bars;
-  const int hv = blockIdx.y, warp = threadIdx.x >> 5;
+  const int hv = blockIdx.x % p.Hv, warp = threadIdx.x >> 5;
   const int segs = MODE == kStates ? a.seg.count - 1 : (REV ? 1 : a.seg.count);
-  const int n = blockIdx.x / segs, seg = blockIdx.x % segs;
+  const int rank = blockIdx.x / p.Hv / segs, seg = blockIdx.x / p.Hv % segs;
+  const int n = p.cu_seqlens ? a.table.order[rank] : rank;
   const int blocks_v = (p.dv + kCols - 1) / kCols;
-  const bool matrix = MODE == kStates && static_cast<int>(blockIdx.z) == blocks_v;  // M, not B
-  const int col0 = matrix ? 0 : blockIdx.z * kCols;
+  const bool matrix = MODE == kStates && static_cast<int>(blockIdx.y) == blocks_v;  // M, not B
+  const int col0 = matrix ? 0 : blockIdx.y * kCols;
   Seq s = sequence(p, a.table, n);
-  if (s.gap) {  // rows of no sequence: zeros
+  if (s.gap) {  // rows of no sequence: zeros (backwards the gradients' kernel writes them)
+    if (REV) return;
     const int pieces = min(kCols, p.dv - col0) / 8;
     for (int64_t i = threadIdx.x; i < static_cast<int64_t>(s.len) * pieces; i += blockDim.x)
       *reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) +
@@ -866,10 +868,10 @@ cudaError_t launch(const gsa_delta_t& p, const DeltaMaps& m, const SeqArgs& a,
   e = allow_smem<seq_kernel<DK, MODE>>(seq_smem<DK>());
   if (e != cudaSuccess) return e;
   const int segs = MODE == kStates ? a.seg.count - 1 : (MODE == kForward ? a.seg.count : 1);
-  const int seqs = p.N + (MODE == kForward && p.cu_seqlens ? 2 : 0);
+  const int seqs = p.N + (p.cu_seqlens ? 2 : 0);
   const int cols = (p.dv + kCols - 1) / kCols + (MODE == kStates ? 1 : 0);
-  seq_kernel<DK, MODE><<<dim3(seqs * segs, p.Hv, cols), kThreads, seq_smem<DK>(), stream>>>(p, m,
-                                                                                            a);
+  seq_kernel<DK, MODE>
+      <<<dim3(seqs * segs * p.Hv, cols), kThreads, seq_smem<DK>(), stream>>>(p, m, a);
   return cudaGetLastError();
 }
 
@@ -890,22 +892,26 @@ cudaError_t forward(const gsa_delta_t& p, const DeltaMaps& m, const SeqArgs& a,
 }  // namespace
 
 // Of all cuts the one whose blocks take the least time, counted in rounds of 148
-// blocks: a chunk takes 3.0 us in the full pass and 2.4 us in the one for M and B
-// (128 columns each of B and M, all segments but the last), a step between segments
-// 2 us.  16 heads of 16384 tokens take 0.76 ms uncut.
+// blocks: a chunk takes 2.9 us in the full pass, and 1.4 us more where all SMs read
+// at once; 2.8 us in the one for M and B (128 columns each of B and M, all segments
+// but the last); a step between segments 4.5 us.  16 heads of 16384 tokens take 0.76
+// ms uncut and 0.33 ms in nine segments; 64 heads of 4096 0.23 ms, and 0.24 in two.
 Segments segments_of(const gsa_delta_t& p) {
   if (p.cu_seqlens || p.T < 16 * kChunk) return {1, p.T / kChunk + 1};
   const int chunks = (p.T + kChunk - 1) / kChunk;
   const int64_t cols = (p.dv + kCols - 1) / kCols, heads = static_cast<int64_t>(p.N) * p.Hv;
   auto rounds = [](int64_t blocks) { return static_cast<double>((blocks + 147) / 148); };
   Segments best = {1, chunks};
-  double least = 3.0 * chunks * rounds(heads * cols);
+  auto full = [&](int64_t blocks) {
+    return rounds(blocks) * (2.9 + 1.4 * (blocks < 148 ? blocks / 148.0 : 1.0));
+  };
+  double least = chunks * full(heads * cols);
   for (int n = 2; n <= 16 && heads * n < 2048; ++n) {
     const int each = (chunks + n - 1) / n, count = (chunks + each - 1) / each;
     if (each < 8) break;
-    const double time = each * (2.4 * rounds(heads * (cols + 1) * (count - 1)) +
-                                3.0 * rounds(heads * cols * count)) +
-                        2.0 * count + 10.0;
+    const double time = each * (2.8 * rounds(heads * (cols + 1) * (count - 1)) +
+                                full(heads * cols * count)) +
+                        4.5 * count + 10.0;
     if (time < least) {
       least = time;
       best = {count, each};

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) delta_step_kernel(const gsa_delta_t 
 // the same way and reported in the device error word.
 __global__ void __launch_bounds__(1024) delta_table_kernel(const int32_t* cu, int N, int T,
                                                            int max_chunks, Table t, int* err) {
-  __shared__ int warp_max[32], warp_sum[32];
+  __shared__ int warp_max[32], warp_sum[32], lens[kSorted];
   __shared__ int carry_end, carry_chunk;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int first = min(max(cu[0], 0), T);
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(1024) delta_table_kernel(const int32_t* cu, in
     if (s < N + 2) {
       t.seq_begin[s] = begin;
       t.seq_len[s] = len;
+      if (s < kSorted) lens[s] = len;
       t.seq_chunk[s] = at;
       for (int c = 0; c < chunks; ++c)
         if (at + c < max_chunks) t.chunk_seq[at + c] = s;
@@ -220,6 +221,15 @@ __global__ void __launch_bounds__(1024) delta_table_kernel(const int32_t* cu, in
       carry_chunk = chunk_start + sum;
     }
     __syncthreads();
+  }
+  for (int s = tid; s < N + 2; s += blockDim.x) {
+    int rank = s;
+    if (N + 2 <= kSorted) {
+      rank = 0;
+      const int mine = lens[s];
+      for (int o = 0; o < N + 2; ++o) rank += lens[o] > mine || (lens[o] == mine && o < s);
+    }
+    t.order[rank] = s;
   }
 }
 
