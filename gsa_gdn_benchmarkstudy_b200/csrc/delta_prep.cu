@@ -57,17 +57,23 @@ constexpr int prep_smem() {
          kChunk * kLdL * 4 + 1024;
 }
 
-// out[r][c] = sign sum_k a[r][k] b[k][c] for a 32 x 32 block, 2 x 4 a thread.
-__device__ __forceinline__ void block32(const float* a, int lda, const float* b, int ldb,
-                                        float* out, int ldo, float sign) {
-  const int r = (threadIdx.x >> 3) * 2, c = (threadIdx.x & 7) * 4;
-  float x[2][4] = {};
-#pragma unroll 8
-  for (int k = 0; k < 32; ++k) {
+// out = sign a b for N x N blocks, R x 4 a thread, k = 0 .. N - 1.  LOWER_B: b is lower
+// triangular, k starts at the thread's first column, which a warp's threads nearly
+// share; else a is, and k ends at its last row.
+template <int N, int R, bool LOWER_B>
+__device__ __forceinline__ void block_product(int t, const float* a, const float* b, int ldb,
+                                              float* out, int ldo, float sign) {
+  constexpr int kRows = N / R, kColGroups = N / 4;
+  const int r = (LOWER_B ? t % kRows : t / kColGroups) * R;
+  const int c = (LOWER_B ? t / kRows : t % kColGroups) * 4;
+  float x[R][4] = {};
+  const int first = LOWER_B ? c : 0, last = LOWER_B ? N : r + R;
+#pragma unroll 4
+  for (int k = first; k < last; ++k) {
     const float4 v = *reinterpret_cast<const float4*>(b + k * ldb + c);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float u = a[(r + i) * lda + k];
+    for (int i = 0; i < R; ++i) {
+      const float u = a[(r + i) * kLdL + k];
       x[i][0] = fmaf(u, v.x, x[i][0]);
       x[i][1] = fmaf(u, v.y, x[i][1]);
       x[i][2] = fmaf(u, v.z, x[i][2]);
@@ -75,26 +81,9 @@ __device__ __forceinline__ void block32(const float* a, int lda, const float* b,
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < R; ++i)
     *reinterpret_cast<float4*>(out + (r + i) * ldo + c) =
         make_float4(sign * x[i][0], sign * x[i][1], sign * x[i][2], sign * x[i][3]);
-}
-// The same for the two 16 x 16 blocks of a level, 64 threads and 1 x 4 each.
-__device__ __forceinline__ void block16(const float* a, int lda, const float* b, int ldb,
-                                        float* out, int ldo, float sign) {
-  const int t = threadIdx.x & 63, r = t >> 2, c = (t & 3) * 4;
-  float x[4] = {};
-#pragma unroll
-  for (int k = 0; k < 16; ++k) {
-    const float4 v = *reinterpret_cast<const float4*>(b + k * ldb + c);
-    const float u = a[r * lda + k];
-    x[0] = fmaf(u, v.x, x[0]);
-    x[1] = fmaf(u, v.y, x[1]);
-    x[2] = fmaf(u, v.z, x[2]);
-    x[3] = fmaf(u, v.w, x[3]);
-  }
-  *reinterpret_cast<float4*>(out + r * ldo + c) =
-      make_float4(sign * x[0], sign * x[1], sign * x[2], sign * x[3]);
 }
 
 // L (strictly lower, 64 x 64) becomes T = (I + L)^-1 in place, in fp32: the four
@@ -120,16 +109,16 @@ __device__ __forceinline__ void invert(float* L, float* X) {
       for (int i = 0; i < 16; ++i) D[i * kLdL + j] = col[i];
   }
   __syncthreads();
-  const int b = (tid >> 6) * 32;
+  const int b = (tid >> 6) * 32, t = tid & 63;
   float* D = L + b * kLdL + b;
   float* Y = X + (tid >> 6) * 16 * kLdX;
-  block16(D + 16 * kLdL, kLdL, D, kLdL, Y, kLdX, 1.f);
+  block_product<16, 1, true>(t, D + 16 * kLdL, D, kLdL, Y, kLdX, 1.f);
   __syncthreads();
-  block16(D + 16 * kLdL + 16, kLdL, Y, kLdX, D + 16 * kLdL, kLdL, -1.f);
+  block_product<16, 1, false>(t, D + 16 * kLdL + 16, Y, kLdX, D + 16 * kLdL, kLdL, -1.f);
   __syncthreads();
-  block32(L + 32 * kLdL, kLdL, L, kLdL, X, kLdX, 1.f);
+  block_product<32, 2, true>(tid, L + 32 * kLdL, L, kLdL, X, kLdX, 1.f);
   __syncthreads();
-  block32(L + 32 * kLdL + 32, kLdL, X, kLdX, L + 32 * kLdL, kLdL, -1.f);
+  block_product<32, 2, false>(tid, L + 32 * kLdL + 32, X, kLdX, L + 32 * kLdL, kLdL, -1.f);
   __syncthreads();
 }
 
@@ -163,6 +152,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t
     ldsm(qa, at_mk(Q, m0, 2 * ks));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      if (16 * j > m0) continue;  // above the diagonal
       uint32_t b[4];
       ldsm(b, at_nk(K, 16 * j, 2 * ks));
       mma(kk[2 * j], ka, b[0], b[1]);
@@ -194,6 +184,13 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int cc = 8 * j + 2 * tig;
+        const uint32_t at = sw128_offset(r, j) + 4 * tig;
+        if (8 * j > m0 + 8) {  // above the diagonal, for the whole warp
+          *reinterpret_cast<float2*>(L + r * kLdL + cc) = make_float2(0.f, 0.f);
+          *reinterpret_cast<uint32_t*>(smem + at) = 0;
+          *reinterpret_cast<uint32_t*>(smem + kTile + at) = 0;
+          continue;
+        }
         const float2 hc = *reinterpret_cast<const float2*>(d.hi + cc);
         const float2 lc = *reinterpret_cast<const float2*>(d.lo + cc);
         float l[2], x[2];
@@ -206,7 +203,6 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t
         *reinterpret_cast<float2*>(L + r * kLdL + cc) = make_float2(l[0], l[1]);
         uint32_t hi, lo;
         split(x[0], x[1], hi, lo);
-        const uint32_t at = sw128_offset(r, j) + 4 * tig;
         *reinterpret_cast<uint32_t*>(smem + at) = hi;
         *reinterpret_cast<uint32_t*>(smem + kTile + at) = lo;
       }
