@@ -3,110 +3,113 @@
 // at once, and the launches of the forward and backward pass.
 //
 // One block a chunk and key head makes T and P of the value heads that share the
-// key head.  Its two products (64 x 64 x dk) are mma.sync: they are small, and
-// their results are wanted in registers, where the decays are applied.  T and P
-// leave as hi + lo pairs of bf16, laid out as the shared-memory tiles that the
-// sequential pass copies whole.  Bound by latency: loads, two products, a
-// triangular inverse and 34 KB of stores one after the other; four blocks an SM
-// overlap theirs.
+// key head.  [K; Q] K^T is one tcgen05 product of 128 x 64 x dk: tensor memory
+// keeps it for all of them, a thread reads its row of KK^T or QK^T from there.
+// T and P leave as hi + lo pairs of bf16, laid out as the shared-memory tiles that
+// the sequential pass copies whole, so bulk copies store them.  Bound by latency:
+// loads, the product, a triangular inverse and 34 KB of stores one after the
+// other; five blocks an SM overlap theirs.
 #include "delta_tc.cuh"
 
 namespace gsa {
 namespace delta {
 namespace {
 
-__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                    uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// Right operand, stored [n][k]: the pieces of two n-tiles (rows n0 .. n0 + 15)
-// and 16 columns (piece c, c + 1 of the whole row).  r[0], r[1]: first n-tile.
-__device__ __forceinline__ uint32_t at_nk(uint32_t tile, int n0, int c) {
-  const int l = threadIdx.x & 31, m = l >> 3;
-  const int row = n0 + 8 * (m >> 1) + (l & 7), piece = c + (m & 1);
-  return tile + (piece >> 3) * kTile + sw128_offset(row, piece & 7);
-}
-// Left operand, stored [m][k]: rows m0 .. m0 + 15, pieces c, c + 1.
-__device__ __forceinline__ uint32_t at_mk(uint32_t tile, int m0, int c) {
-  const int l = threadIdx.x & 31, m = l >> 3;
-  const int row = m0 + 8 * (m & 1) + (l & 7), piece = c + (m >> 1);
-  return tile + (piece >> 3) * kTile + sw128_offset(row, piece & 7);
-}
-
 // ---------------------------------------------------------------- prep
 constexpr int kPrepThreads = 128;
 constexpr int kLdL = kChunk + 4;
 constexpr int kLdX = 36;
 
-// K and Q, whose place P's tiles and a 32 x 32 product take once their products are
-// in registers; L, which becomes T in place.
-constexpr int kPrepTiles = 2 * static_cast<int>(kTile) + 32 * kLdX * 4;
-template <int DK>
-constexpr int prep_smem() {
-  return (2 * (DK / 64) * static_cast<int>(kTile) > kPrepTiles ? 2 * (DK / 64) * static_cast<int>(kTile)
-                                                               : kPrepTiles) +
-         kChunk * kLdL * 4 + 1024;
+// Shared memory: K and Q (64 columns of K, of Q, the next 64 of K, of Q); once they
+// are multiplied, the gates, P's tiles, L (which becomes T in place, in fp32) and the
+// inner products of its inverse.  T's tiles take the place of the gates and P.
+constexpr int kOffPTiles = sizeof(Gates), kOffL = kOffPTiles + kPBytes;
+constexpr int kOffX = kOffL + kChunk * kLdL * 4, kPrepUsed = kOffX + 32 * kLdX * 4;
+constexpr int kPrepSmem = kPrepUsed + 1024;
+static_assert(kPrepUsed >= 4 * static_cast<int>(kTile), "K and Q");
+
+struct PrepBars {
+  uint64_t full, product;
+  uint32_t tmem;
+  int abort;
+};
+
+__device__ __forceinline__ void bulk_store(void* dst, const void* smem_src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                   reinterpret_cast<uint64_t>(dst)),
+               "r"(smem_u32(smem_src)), "r"(bytes)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Until the stores of this thread have read shared memory, or have arrived.
+__device__ __forceinline__ void bulk_stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_stores_done() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
-// out = sign a b for N x N blocks, R x 4 a thread, k = 0 .. N - 1.  LOWER_B: b is lower
-// triangular, k starts at the thread's first column, which a warp's threads nearly
-// share; else a is, and k ends at its last row.
+// out = sign a b for N x N blocks, R x 4 a thread, four k at a time.  LOWER_B: b is
+// lower triangular, k starts at the thread's first column, which a warp's threads
+// nearly share; else a is, and k ends behind its last row.
 template <int N, int R, bool LOWER_B>
 __device__ __forceinline__ void block_product(int t, const float* a, const float* b, int ldb,
                                               float* out, int ldo, float sign) {
-  constexpr int kRows = N / R, kColGroups = N / 4;
-  const int r = (LOWER_B ? t % kRows : t / kColGroups) * R;
+  constexpr int kRows = N / R, kColGroups = N / 4, kApart = LOWER_B ? kRows : 1;
+  const int r = LOWER_B ? t % kRows : t / kColGroups * R;
   const int c = (LOWER_B ? t / kRows : t % kColGroups) * 4;
   float x[R][4] = {};
   const int first = LOWER_B ? c : 0, last = LOWER_B ? N : r + R;
-#pragma unroll 4
-  for (int k = first; k < last; ++k) {
-    const float4 v = *reinterpret_cast<const float4*>(b + k * ldb + c);
+#pragma unroll 2
+  for (int k = first; k < last; k += 4) {
+    float4 u[R], v[4];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const float u = a[(r + i) * kLdL + k];
-      x[i][0] = fmaf(u, v.x, x[i][0]);
-      x[i][1] = fmaf(u, v.y, x[i][1]);
-      x[i][2] = fmaf(u, v.z, x[i][2]);
-      x[i][3] = fmaf(u, v.w, x[i][3]);
-    }
+    for (int i = 0; i < R; ++i)
+      u[i] = *reinterpret_cast<const float4*>(a + (r + i * kApart) * kLdL + k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float4*>(b + (k + j) * ldb + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const float f = j == 0 ? u[i].x : j == 1 ? u[i].y : j == 2 ? u[i].z : u[i].w;
+        x[i][0] = fmaf(f, v[j].x, x[i][0]);
+        x[i][1] = fmaf(f, v[j].y, x[i][1]);
+        x[i][2] = fmaf(f, v[j].z, x[i][2]);
+        x[i][3] = fmaf(f, v[j].w, x[i][3]);
+      }
   }
 #pragma unroll
   for (int i = 0; i < R; ++i)
-    *reinterpret_cast<float4*>(out + (r + i) * ldo + c) =
+    *reinterpret_cast<float4*>(out + (r + i * kApart) * ldo + c) =
         make_float4(sign * x[i][0], sign * x[i][1], sign * x[i][2], sign * x[i][3]);
 }
 
-// L (strictly lower, 64 x 64) becomes T = (I + L)^-1 in place, in fp32: the four
-// 16 x 16 diagonal blocks by substitution, then T21 = -T22 L21 T11 twice over.
-// A column a thread over all 64 rows took 2.5 times as long: half the threads
-// idle, 64 values of a column in registers.
+// L (strictly lower, 64 x 64, its upper right quarter unused) becomes
+// T = (I + L)^-1 in place, in fp32: the four 16 x 16 diagonal blocks by
+// substitution, then T21 = -T22 L21 T11 twice over.
 __device__ __forceinline__ void invert(float* L, float* X) {
-  const int tid = threadIdx.x;
-  {
-    const int b = (tid & 63) >> 4, j = tid & 15;
+  const int tid = threadIdx.x, warp = tid >> 5;
+  if ((warp & 1) == 0) {  // the warps that had less of L and P to make
+    const int b = warp + ((tid >> 4) & 1), j = tid & 15;
     float* D = L + 16 * b * kLdL + 16 * b;
     float col[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float s = i == j ? 1.f : 0.f;
 #pragma unroll
-      for (int m = 0; m < i; ++m) s = fmaf(-D[i * kLdL + m], col[m], s);
+      for (int m = 0; m < i; m += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(D + i * kLdL + m);
+        s = fmaf(-v.x, col[m], s);
+        if (m + 1 < i) s = fmaf(-v.y, col[m + 1], s);
+        if (m + 2 < i) s = fmaf(-v.z, col[m + 2], s);
+        if (m + 3 < i) s = fmaf(-v.w, col[m + 3], s);
+      }
       col[i] = s;
     }
-    __syncthreads();
-    if (tid < 64)
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) D[i * kLdL + j] = col[i];
+    for (int i = 0; i < 16; ++i) D[i * kLdL + j] = col[i];
   }
   __syncthreads();
   const int b = (tid >> 6) * 32, t = tid & 63;
@@ -119,133 +122,192 @@ __device__ __forceinline__ void invert(float* L, float* X) {
   block_product<32, 2, true>(tid, L + 32 * kLdL, L, kLdL, X, kLdX, 1.f);
   __syncthreads();
   block_product<32, 2, false>(tid, L + 32 * kLdL + 32, X, kLdX, L + 32 * kLdL, kLdL, -1.f);
-  __syncthreads();
+}
+
+// 8 values as hi + lo in piece `at` of a pair of tiles.
+__device__ __forceinline__ void put_pairs(unsigned char* tiles, uint32_t at, const float (&x)[8]) {
+  uint4 hi, lo;
+  split(x[0], x[1], hi.x, lo.x);
+  split(x[2], x[3], hi.y, lo.y);
+  split(x[4], x[5], hi.z, lo.z);
+  split(x[6], x[7], hi.w, lo.w);
+  *reinterpret_cast<uint4*>(tiles + at) = hi;
+  *reinterpret_cast<uint4*>(tiles + kTile + at) = lo;
+}
+
+// Row `r` of L (of P with `is_p`), 32 columns from tensor memory at a time.
+__device__ __forceinline__ void make_row(const Decays& d, uint32_t tmem, int r, bool is_p,
+                                         float factor, float* L, unsigned char* P) {
+  const float hi_r = d.hi[r], lo_r = d.lo[r];
+  const int half = r >> 5;
+  for (int h = 0; h <= half; ++h) {
+    uint32_t raw[32];
+    tmem_ld32(tmem + 32 * h, raw);
+    tc_wait_ld(raw);
+    // the diagonal is in the last 32 columns: what lies behind it is dropped
+    const int limit = r - 32 * h + (is_p ? 1 : 0);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = 8 * g + i;
+        const float w = exp_of((hi_r - d.hi[32 * h + c]) + (lo_r - d.lo[32 * h + c]));
+        x[i] = c < limit ? factor * w * __uint_as_float(raw[c]) : 0.f;
+      }
+      if (is_p) {
+        put_pairs(P, sw128_offset(r, 4 * h + g), x);
+      } else {
+        float4* to = reinterpret_cast<float4*>(L + r * kLdL + 32 * h + 8 * g);
+        to[0] = make_float4(x[0], x[1], x[2], x[3]);
+        to[1] = make_float4(x[4], x[5], x[6], x[7]);
+      }
+    }
+  }
+  if (half == 0 && is_p)
+#pragma unroll
+    for (int g = 4; g < 8; ++g) {
+      *reinterpret_cast<uint4*>(P + sw128_offset(r, g)) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(P + kTile + sw128_offset(r, g)) = make_uint4(0, 0, 0, 0);
+    }
 }
 
 template <int DK>
-__global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const gsa_delta_t p, Table table,
-                                                               Block* blocks) {
+__global__ void __launch_bounds__(kPrepThreads, 5)
+    prep_kernel(const gsa_delta_t p, const __grid_constant__ DeltaMaps maps, Table table,
+                Block* blocks, int* err) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~1023ull);
   __shared__ Decays d;
+  __shared__ PrepBars bars;
   const int hk = blockIdx.y, group = p.Hv / p.Hk, tid = threadIdx.x, lane = tid & 31;
-  const int m0 = (tid >> 5) * 16, gid = lane >> 2, tig = lane & 3;
+  const int warp = tid >> 5;
   const Chunk c = chunk_at(p, table, blockIdx.x);
   if (!c.valid || c.gap) return;
-  const uint32_t K = smem_u32(smem), Q = K + (DK / 64) * kTile;
-  float* X = reinterpret_cast<float*>(smem + 2 * kTile);
-  float* L = reinterpret_cast<float*>(smem + prep_smem<DK>() - 1024) - kChunk * kLdL;
-  copy_rows(K, rows_at(p.k, p.k_stride, c.b, c.begin, hk), p.k_stride[1], c.len, DK, p.dk, tid,
-            kPrepThreads);
-  copy_rows(Q, rows_at(p.q, p.q_stride, c.b, c.begin, hk), p.q_stride[1], c.len, DK, p.dk, tid,
-            kPrepThreads);
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  if (tid < 32) chunk_decays(p, c, hk * group, d);  // beside the copies
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  float kk[8][4] = {}, qk[8][4] = {};
-#pragma unroll
-  for (int ks = 0; ks < DK / 16; ++ks) {
-    uint32_t ka[4], qa[4];
-    ldsm(ka, at_mk(K, m0, 2 * ks));
-    ldsm(qa, at_mk(Q, m0, 2 * ks));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (16 * j > m0) continue;  // above the diagonal
-      uint32_t b[4];
-      ldsm(b, at_nk(K, 16 * j, 2 * ks));
-      mma(kk[2 * j], ka, b[0], b[1]);
-      mma(kk[2 * j + 1], ka, b[2], b[3]);
-      mma(qk[2 * j], qa, b[0], b[1]);
-      mma(qk[2 * j + 1], qa, b[2], b[3]);
-    }
-  }
-  for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
-    __syncthreads();  // K and Q, or the last head's tiles, are read
-    if (hv > hk * group) {
-      if (tid < 32) chunk_decays(p, c, hv, d);
-      __syncthreads();
-    }
-    Block* blk = blocks + static_cast<int64_t>(blockIdx.x) * p.Hv + hv;
-    if (tid < kChunk) {
-      const float grown = decay_from_start(d, tid);
-      blk->gates.grown[tid] = grown;
-      blk->gates.beta[tid] = d.beta[tid];
-      blk->gates.left[tid] = decay_between(d, kChunk - 1, tid);
-      blk->gates.both[tid] = d.beta[tid] * grown;
-      blk->gates.hi[tid] = d.hi[tid];
-      blk->gates.lo[tid] = d.lo[tid];
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = m0 + gid + 8 * e;
-      const float hi_r = d.hi[r], lo_r = d.lo[r], beta_r = d.beta[r];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int cc = 8 * j + 2 * tig;
-        const uint32_t at = sw128_offset(r, j) + 4 * tig;
-        if (8 * j > m0 + 8) {  // above the diagonal, for the whole warp
-          *reinterpret_cast<float2*>(L + r * kLdL + cc) = make_float2(0.f, 0.f);
-          *reinterpret_cast<uint32_t*>(smem + at) = 0;
-          *reinterpret_cast<uint32_t*>(smem + kTile + at) = 0;
-          continue;
-        }
-        const float2 hc = *reinterpret_cast<const float2*>(d.hi + cc);
-        const float2 lc = *reinterpret_cast<const float2*>(d.lo + cc);
-        float l[2], x[2];
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const float w = exp_of((hi_r - (f ? hc.y : hc.x)) + (lo_r - (f ? lc.y : lc.x)));
-          l[f] = r > cc + f ? beta_r * w * kk[j][2 * e + f] : 0.f;
-          x[f] = r >= cc + f ? p.scale * w * qk[j][2 * e + f] : 0.f;
-        }
-        *reinterpret_cast<float2*>(L + r * kLdL + cc) = make_float2(l[0], l[1]);
-        uint32_t hi, lo;
-        split(x[0], x[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(smem + at) = hi;
-        *reinterpret_cast<uint32_t*>(smem + kTile + at) = lo;
+  // Rows past the tensor's end come out of TMA as zeros; a chunk that ends before its
+  // 64th row inside a packed batch takes its rows one by one.
+  const bool whole = c.len == kChunk || !p.cu_seqlens;
+  if (tid == 0) {
+    bars.abort = 0;
+    mbar_init(&bars.full, 1);
+    mbar_init(&bars.product, 1);
+    fence_mbar_init();
+    if (whole) {
+      mbar_arrive_expect_tx(&bars.full, DK / 64 * 2 * kTile);
+      for (int i = 0; i < DK / 64; ++i) {
+        tma_load_rows(smem + 2 * i * kTile, &maps.k, 64 * i, hk, c.begin, c.b, &bars.full);
+        tma_load_rows(smem + (2 * i + 1) * kTile, &maps.q, 64 * i, hk, c.begin, c.b, &bars.full);
       }
     }
-    __syncthreads();
-    {  // P leaves while T is made
-      uint4* dst = reinterpret_cast<uint4*>(blk->p_hi);
-      const uint4* src = reinterpret_cast<const uint4*>(smem);
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars.tmem, 64);
+    tmem_relinquish();
+  }
+  if (!whole) {
+    copy_rows(smem_u32(smem), rows_at(p.k, p.k_stride, c.b, c.begin, hk), p.k_stride[1], c.len, DK,
+              p.dk, tid, kPrepThreads, 2 * kTile);
+    copy_rows(smem_u32(smem) + kTile, rows_at(p.q, p.q_stride, c.b, c.begin, hk), p.q_stride[1],
+              c.len, DK, p.dk, tid, kPrepThreads, 2 * kTile);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    fence_proxy_async_smem();
+  }
+  if (warp == 2) chunk_decays(p, c, hk * group, d);  // beside the copies
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, bars.tmem, 0);
+  bool ok = true;
+  if (warp == 0) {
+    if (whole) ok = mbar_wait_warp(&bars.full, 0, err, &bars.abort);
+    if (ok) {
+      const uint32_t tile = smem_u32(smem);
 #pragma unroll
-      for (int i = 0; i < kPBytes / 16 / kPrepThreads; ++i)
-        dst[tid + i * kPrepThreads] = src[tid + i * kPrepThreads];
+      for (int ks = 0; ks < DK / 16; ++ks) {
+        const uint64_t kq = desc_rows(tile, ks, 2 * kTile);
+        warp_mma_ss(tmem, kq, kq, idesc_bf16_f32(128, 64, 0, 0), ks);
+      }
+      warp_commit(&bars.product);
     }
-    invert(L, X);
+    // no copy and no product of ours may outlive the block
+    if (!ok)
+      mbar_wait_drain(&bars.full, 0, kWaitLimitCycles);
+    else if (!(ok = mbar_wait_warp(&bars.product, 0, err, &bars.abort)))
+      mbar_wait_drain(&bars.product, 0, kWaitLimitCycles);
+  }
+  ok = ok && mbar_wait_warp(&bars.product, 0, err, &bars.abort);
+  if (__syncthreads_and(ok)) {
+    tc_fence_after();
+    float* L = reinterpret_cast<float*>(smem + kOffL);
+    float* X = reinterpret_cast<float*>(smem + kOffX);
+    Gates* gates = reinterpret_cast<Gates*>(smem);
+    const int row = 32 * (warp & 1) + lane;
+    const uint32_t mine = tmem + (static_cast<uint32_t>(32 * warp) << 16);
+    constexpr int kStorer = 96;
+    for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
+      if (hv > hk * group) {
+        if (warp == 2) chunk_decays(p, c, hv, d);
+        if (tid == kStorer) bulk_stores_read();
+        __syncthreads();
+      }
+      Block* blk = blocks + static_cast<int64_t>(blockIdx.x) * p.Hv + hv;
+      make_row(d, mine, row, warp >= 2, warp >= 2 ? p.scale : d.beta[row], L, smem + kOffPTiles);
+      if ((warp & 1) == 0) {
+        const int i = tid < 32 ? tid : tid - 32;
+        const float grown = decay_from_start(d, i);
+        gates->grown[i] = grown;
+        gates->beta[i] = d.beta[i];
+        gates->left[i] = decay_between(d, kChunk - 1, i);
+        gates->both[i] = d.beta[i] * grown;
+        gates->hi[i] = d.hi[i];
+        gates->lo[i] = d.lo[i];
+      }
+      fence_proxy_async_smem();
+      __syncthreads();
+      if (tid == kStorer)  // P leaves while T is made
+        bulk_store(&blk->gates, smem, static_cast<uint32_t>(sizeof(Gates)) + kPBytes);
+      invert(L, X);
+      if (tid == kStorer) bulk_stores_read();
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kChunk * 8 / kPrepThreads; ++i) {
-      const int x = tid + i * kPrepThreads, r = x >> 3, piece = x & 7;
-      const float4 u = *reinterpret_cast<const float4*>(L + r * kLdL + piece * 8);
-      const float4 v = *reinterpret_cast<const float4*>(L + r * kLdL + piece * 8 + 4);
-      uint4 hi, lo;
-      split(u.x, u.y, hi.x, lo.x);
-      split(u.z, u.w, hi.y, lo.y);
-      split(v.x, v.y, hi.z, lo.z);
-      split(v.z, v.w, hi.w, lo.w);
-      *reinterpret_cast<uint4*>(blk->t_hi + sw128_offset(r, piece)) = hi;
-      *reinterpret_cast<uint4*>(blk->t_lo + sw128_offset(r, piece)) = lo;
+      for (int i = 0; i < kChunk * 8 / kPrepThreads; ++i) {
+        const int x = tid + i * kPrepThreads, r = x >> 3, piece = x & 7;
+        float t[8] = {};
+        if (r >= 32 || piece < 4) {
+          const float4 u = *reinterpret_cast<const float4*>(L + r * kLdL + piece * 8);
+          const float4 v = *reinterpret_cast<const float4*>(L + r * kLdL + piece * 8 + 4);
+          t[0] = u.x, t[1] = u.y, t[2] = u.z, t[3] = u.w;
+          t[4] = v.x, t[5] = v.y, t[6] = v.z, t[7] = v.w;
+        }
+        put_pairs(smem, sw128_offset(r, piece), t);
+      }
+      fence_proxy_async_smem();
+      __syncthreads();
+      if (tid == kStorer) bulk_store(blk->t_hi, smem, kPBytes);
     }
+    if (tid == kStorer) bulk_stores_done();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 64);
   }
 }
 
 template <int DK>
-cudaError_t launch_prep(const gsa_delta_t& p, const Table& t, Block* blocks, cudaStream_t stream) {
+cudaError_t launch_prep(const gsa_delta_t& p, const DeltaMaps& m, const Table& t, Block* blocks,
+                        int* err, cudaStream_t stream) {
   const int64_t chunks = max_chunks(p);
   if (chunks == 0) return cudaSuccess;
-  const cudaError_t e = allow_smem<prep_kernel<DK>>(prep_smem<DK>());
+  const cudaError_t e = allow_smem<prep_kernel<DK>>(kPrepSmem);
   if (e != cudaSuccess) return e;
-  prep_kernel<DK><<<dim3(static_cast<unsigned>(chunks), p.Hk), kPrepThreads, prep_smem<DK>(),
-                    stream>>>(p, t, blocks);
+  prep_kernel<DK><<<dim3(static_cast<unsigned>(chunks), p.Hk), kPrepThreads, kPrepSmem, stream>>>(
+      p, m, t, blocks, err);
   return cudaGetLastError();
 }
 
-}  // namespace
-
-namespace {
 // The segments' floats lie behind what the backward pass reads.
 int64_t cuts_offset(const gsa_delta_t& p, bool save) {
   const int64_t n = max_chunks(p) * p.Hv;
@@ -264,8 +326,8 @@ cudaError_t bf16_forward(const gsa_delta_t& p, const DeltaMaps& m, void* o, floa
                          bool save, void* ws, int* err, cudaStream_t stream) {
   const Saved s = saved_at(p, ws);
   const Table t = table_at(ws, p.N);
-  const cudaError_t e = p.dk <= 64 ? launch_prep<64>(p, t, s.blocks, stream)
-                                   : launch_prep<128>(p, t, s.blocks, stream);
+  const cudaError_t e = p.dk <= 64 ? launch_prep<64>(p, m, t, s.blocks, err, stream)
+                                   : launch_prep<128>(p, m, t, s.blocks, err, stream);
   if (e != cudaSuccess) return e;
   SeqArgs a = {};
   a.table = t;
