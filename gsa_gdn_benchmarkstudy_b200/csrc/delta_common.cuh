@@ -108,7 +108,7 @@ __device__ __forceinline__ Chunk chunk_at(const gsa_delta_t& p, const Table& t, 
 // Cumulative decays c_i of a chunk by one warp (lane l: tokens 2l, 2l + 1), as
 // hi + lo pairs of fp32 so that differences keep fp32's accuracy however far
 // the sums have gone.  Rows past `len` repeat the last sum and have beta 0.
-struct Decays {
+struct __align__(16) Decays {
   float hi[kChunk], lo[kChunk], beta[kChunk];
 };
 __device__ __forceinline__ void chunk_decays(const gsa_delta_t& p, const Chunk& c, int hv,

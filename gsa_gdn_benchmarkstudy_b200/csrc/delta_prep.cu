@@ -8,7 +8,7 @@
 // T and P leave as hi + lo pairs of bf16, laid out as the shared-memory tiles that
 // the sequential pass copies whole, so bulk copies store them.  Bound by latency:
 // loads, the product, a triangular inverse and 34 KB of stores one after the
-// other; five blocks an SM overlap theirs.
+// other; six blocks an SM overlap theirs.
 #include "delta_tc.cuh"
 
 namespace gsa {
@@ -18,13 +18,13 @@ namespace {
 // ---------------------------------------------------------------- prep
 constexpr int kPrepThreads = 128;
 constexpr int kLdL = kChunk + 4;
-constexpr int kLdX = 36;
 
 // Shared memory: K and Q (64 columns of K, of Q, the next 64 of K, of Q); once they
-// are multiplied, the gates, P's tiles, L (which becomes T in place, in fp32) and the
-// inner products of its inverse.  T's tiles take the place of the gates and P.
+// are multiplied, the gates, P's tiles and L, which becomes T in place, in fp32; the
+// inner products of its inverse lie in L's upper right quarter.  T's tiles take the
+// place of the gates and P.  Six blocks fit into an SM.
 constexpr int kOffPTiles = sizeof(Gates), kOffL = kOffPTiles + kPBytes;
-constexpr int kOffX = kOffL + kChunk * kLdL * 4, kPrepUsed = kOffX + 32 * kLdX * 4;
+constexpr int kPrepUsed = kOffL + kChunk * kLdL * 4;
 constexpr int kPrepSmem = kPrepUsed + 1024;
 static_assert(kPrepUsed >= 4 * static_cast<int>(kTile), "K and Q");
 
@@ -53,8 +53,8 @@ __device__ __forceinline__ void bulk_stores_done() {
 // lower triangular, k starts at the thread's first column, which a warp's threads
 // nearly share; else a is, and k ends behind its last row.
 template <int N, int R, bool LOWER_B>
-__device__ __forceinline__ void block_product(int t, const float* a, const float* b, int ldb,
-                                              float* out, int ldo, float sign) {
+__device__ __forceinline__ void block_product(int t, const float* a, const float* b, float* out,
+                                              float sign) {
   constexpr int kRows = N / R, kColGroups = N / 4, kApart = LOWER_B ? kRows : 1;
   const int r = LOWER_B ? t % kRows : t / kColGroups * R;
   const int c = (LOWER_B ? t / kRows : t % kColGroups) * 4;
@@ -67,7 +67,7 @@ __device__ __forceinline__ void block_product(int t, const float* a, const float
     for (int i = 0; i < R; ++i)
       u[i] = *reinterpret_cast<const float4*>(a + (r + i * kApart) * kLdL + k);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float4*>(b + (k + j) * ldb + c);
+    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float4*>(b + (k + j) * kLdL + c);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -81,14 +81,14 @@ __device__ __forceinline__ void block_product(int t, const float* a, const float
   }
 #pragma unroll
   for (int i = 0; i < R; ++i)
-    *reinterpret_cast<float4*>(out + (r + i * kApart) * ldo + c) =
+    *reinterpret_cast<float4*>(out + (r + i * kApart) * kLdL + c) =
         make_float4(sign * x[i][0], sign * x[i][1], sign * x[i][2], sign * x[i][3]);
 }
 
-// L (strictly lower, 64 x 64, its upper right quarter unused) becomes
+// L (strictly lower, 64 x 64, its upper right quarter free) becomes
 // T = (I + L)^-1 in place, in fp32: the four 16 x 16 diagonal blocks by
 // substitution, then T21 = -T22 L21 T11 twice over.
-__device__ __forceinline__ void invert(float* L, float* X) {
+__device__ __forceinline__ void invert(float* L) {
   const int tid = threadIdx.x, warp = tid >> 5;
   if ((warp & 1) == 0) {  // the warps that had less of L and P to make
     const int b = warp + ((tid >> 4) & 1), j = tid & 15;
@@ -114,14 +114,14 @@ __device__ __forceinline__ void invert(float* L, float* X) {
   __syncthreads();
   const int b = (tid >> 6) * 32, t = tid & 63;
   float* D = L + b * kLdL + b;
-  float* Y = X + (tid >> 6) * 16 * kLdX;
-  block_product<16, 1, true>(t, D + 16 * kLdL, D, kLdL, Y, kLdX, 1.f);
+  float *X = L + 32, *Y = X + (tid >> 6) * 16 * kLdL;
+  block_product<16, 1, true>(t, D + 16 * kLdL, D, Y, 1.f);
   __syncthreads();
-  block_product<16, 1, false>(t, D + 16 * kLdL + 16, Y, kLdX, D + 16 * kLdL, kLdL, -1.f);
+  block_product<16, 1, false>(t, D + 16 * kLdL + 16, Y, D + 16 * kLdL, -1.f);
   __syncthreads();
-  block_product<32, 2, true>(tid, L + 32 * kLdL, L, kLdL, X, kLdX, 1.f);
+  block_product<32, 2, true>(tid, L + 32 * kLdL, L, X, 1.f);
   __syncthreads();
-  block_product<32, 2, false>(tid, L + 32 * kLdL + 32, X, kLdX, L + 32 * kLdL, kLdL, -1.f);
+  block_product<32, 2, false>(tid, L + 32 * kLdL + 32, X, L + 32 * kLdL, -1.f);
 }
 
 // 8 values as hi + lo in piece `at` of a pair of tiles.
@@ -138,7 +138,9 @@ __device__ __forceinline__ void put_pairs(unsigned char* tiles, uint32_t at, con
 // Row `r` of L (of P with `is_p`), 32 columns from tensor memory at a time.
 __device__ __forceinline__ void make_row(const Decays& d, uint32_t tmem, int r, bool is_p,
                                          float factor, float* L, unsigned char* P) {
-  const float hi_r = d.hi[r], lo_r = d.lo[r];
+  const uint64_t hi_r = f2_pack(d.hi[r], d.hi[r]), lo_r = f2_pack(d.lo[r], d.lo[r]);
+  const uint64_t less = f2_pack(-1.f, -1.f), scale = f2_pack(factor, factor);
+  const uint64_t log2e = f2_pack(kLog2e, kLog2e);
   const int half = r >> 5;
   for (int h = 0; h <= half; ++h) {
     uint32_t raw[32];
@@ -150,10 +152,17 @@ __device__ __forceinline__ void make_row(const Decays& d, uint32_t tmem, int r, 
     for (int g = 0; g < 4; ++g) {
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 8; i += 2) {
         const int c = 8 * g + i;
-        const float w = exp_of((hi_r - d.hi[32 * h + c]) + (lo_r - d.lo[32 * h + c]));
-        x[i] = c < limit ? factor * w * __uint_as_float(raw[c]) : 0.f;
+        const uint64_t hi_c = *reinterpret_cast<const uint64_t*>(d.hi + 32 * h + c);
+        const uint64_t lo_c = *reinterpret_cast<const uint64_t*>(d.lo + 32 * h + c);
+        const uint64_t e =
+            f2_mul(f2_add(f2_fma(hi_c, less, hi_r), f2_fma(lo_c, less, lo_r)), log2e);
+        const uint64_t w = f2_pack(fast_ex2(f2_lo(e)), fast_ex2(f2_hi(e)));
+        const uint64_t y = f2_mul(
+            f2_mul(w, scale), f2_pack(__uint_as_float(raw[c]), __uint_as_float(raw[c + 1])));
+        x[i] = c < limit ? f2_lo(y) : 0.f;
+        x[i + 1] = c + 1 < limit ? f2_hi(y) : 0.f;
       }
       if (is_p) {
         put_pairs(P, sw128_offset(r, 4 * h + g), x);
@@ -173,7 +182,7 @@ __device__ __forceinline__ void make_row(const Decays& d, uint32_t tmem, int r, 
 }
 
 template <int DK>
-__global__ void __launch_bounds__(kPrepThreads, 5)
+__global__ void __launch_bounds__(kPrepThreads, 6)
     prep_kernel(const gsa_delta_t p, const __grid_constant__ DeltaMaps maps, Table table,
                 Block* blocks, int* err) {
   extern __shared__ unsigned char smem_raw[];
@@ -240,7 +249,6 @@ __global__ void __launch_bounds__(kPrepThreads, 5)
   if (__syncthreads_and(ok)) {
     tc_fence_after();
     float* L = reinterpret_cast<float*>(smem + kOffL);
-    float* X = reinterpret_cast<float*>(smem + kOffX);
     Gates* gates = reinterpret_cast<Gates*>(smem);
     const int row = 32 * (warp & 1) + lane;
     const uint32_t mine = tmem + (static_cast<uint32_t>(32 * warp) << 16);
@@ -267,7 +275,7 @@ __global__ void __launch_bounds__(kPrepThreads, 5)
       __syncthreads();
       if (tid == kStorer)  // P leaves while T is made
         bulk_store(&blk->gates, smem, static_cast<uint32_t>(sizeof(Gates)) + kPBytes);
-      invert(L, X);
+      invert(L);
       if (tid == kStorer) bulk_stores_read();
       __syncthreads();
 #pragma unroll

@@ -88,6 +88,11 @@ __device__ __forceinline__ uint64_t desc_cols(uint32_t tile, int ks, uint32_t st
   return sdesc_sw128(tile + ks * 2048, step, 1024);
 }
 
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 // x, y as hi + lo pairs of bf16.
 __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = pack_bf16x2(x, y);
@@ -96,7 +101,8 @@ __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& 
   lo = pack_bf16x2(f2_lo(rest), f2_hi(rest));
 }
 // e^x on the MUFU: 2^-22 of the value, and x log2(e) rounded once: 2^-24 |x|.
-__device__ __forceinline__ float exp_of(float x) { return fast_ex2(x * 1.4426950408889634f); }
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp_of(float x) { return fast_ex2(x * kLog2e); }
 __device__ __forceinline__ float lo_of(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float hi_of(uint32_t r) { return __uint_as_float(r & 0xFFFF0000u); }
 
