@@ -151,5 +151,99 @@ __device__ __forceinline__ float decay_from_start(const Decays& d, int i) {
   return expf(d.hi[i] + d.lo[i]);
 }
 
+// What the sequential pass and the gradients need of a chunk's decays.
+struct __align__(16) Gates {
+  float grown[kChunk];  // e^{c_i}
+  float beta[kChunk];
+  float left[kChunk];   // e^{c_64 - c_i}
+  float both[kChunk];   // beta_i e^{c_i}
+  float hi[kChunk];     // c_i = hi + lo
+  float lo[kChunk];
+  float pad[2 * kChunk];
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(real ? 16 : 0)
+               : "memory");
+}
+
+constexpr int kLdL = kChunk + 4;
+// out = sign a b for N x N blocks, R x 4 a thread, four k at a time.  LOWER_B: b is
+// lower triangular, k starts at the thread's first column, which a warp's threads
+// nearly share; else a is, and k ends behind its last row.
+template <int N, int R, bool LOWER_B>
+__device__ __forceinline__ void block_product(int t, const float* a, const float* b, float* out,
+                                              float sign) {
+  constexpr int kRows = N / R, kColGroups = N / 4, kApart = LOWER_B ? kRows : 1;
+  const int r = LOWER_B ? t % kRows : t / kColGroups * R;
+  const int c = (LOWER_B ? t / kRows : t % kColGroups) * 4;
+  float x[R][4] = {};
+  const int first = LOWER_B ? c : 0, last = LOWER_B ? N : r + R;
+#pragma unroll 2
+  for (int k = first; k < last; k += 4) {
+    float4 u[R], v[4];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      u[i] = *reinterpret_cast<const float4*>(a + (r + i * kApart) * kLdL + k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float4*>(b + (k + j) * kLdL + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const float f = j == 0 ? u[i].x : j == 1 ? u[i].y : j == 2 ? u[i].z : u[i].w;
+        x[i][0] = fmaf(f, v[j].x, x[i][0]);
+        x[i][1] = fmaf(f, v[j].y, x[i][1]);
+        x[i][2] = fmaf(f, v[j].z, x[i][2]);
+        x[i][3] = fmaf(f, v[j].w, x[i][3]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    *reinterpret_cast<float4*>(out + (r + i * kApart) * kLdL + c) =
+        make_float4(sign * x[i][0], sign * x[i][1], sign * x[i][2], sign * x[i][3]);
+}
+
+// L (strictly lower, 64 x 64, its upper right quarter free) becomes
+// T = (I + L)^-1 in place, in fp32: the four 16 x 16 diagonal blocks by
+// substitution, then T21 = -T22 L21 T11 twice over.  By the block's first 128 threads.
+__device__ __forceinline__ void invert(float* L) {
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const bool works = tid < 128;
+  if (warp == 0 || warp == 2) {
+    const int b = warp + ((tid >> 4) & 1), j = tid & 15;
+    float* D = L + 16 * b * kLdL + 16 * b;
+    float col[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == j ? 1.f : 0.f;
+#pragma unroll
+      for (int m = 0; m < i; m += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(D + i * kLdL + m);
+        s = fmaf(-v.x, col[m], s);
+        if (m + 1 < i) s = fmaf(-v.y, col[m + 1], s);
+        if (m + 2 < i) s = fmaf(-v.z, col[m + 2], s);
+        if (m + 3 < i) s = fmaf(-v.w, col[m + 3], s);
+      }
+      col[i] = s;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) D[i * kLdL + j] = col[i];
+  }
+  __syncthreads();
+  const int b = (tid >> 6) * 32, t = tid & 63;
+  float* D = L + b * kLdL + b;
+  float *X = L + 32, *Y = X + (tid >> 6) * 16 * kLdL;
+  if (works) block_product<16, 1, true>(t, D + 16 * kLdL, D, Y, 1.f);
+  __syncthreads();
+  if (works) block_product<16, 1, false>(t, D + 16 * kLdL + 16, Y, D + 16 * kLdL, -1.f);
+  __syncthreads();
+  if (works) block_product<32, 2, true>(tid, L + 32 * kLdL, L, X, 1.f);
+  __syncthreads();
+  if (works) block_product<32, 2, false>(tid, L + 32 * kLdL + 32, X, L + 32 * kLdL, -1.f);
+}
+
 }  // namespace delta
 }  // namespace gsa

@@ -106,11 +106,6 @@ __device__ __forceinline__ float exp_of(float x) { return fast_ex2(x * kLog2e); 
 __device__ __forceinline__ float lo_of(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float hi_of(uint32_t r) { return __uint_as_float(r & 0xFFFF0000u); }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(real ? 16 : 0)
-               : "memory");
-}
 __device__ __forceinline__ const bf16* rows_at(const void* base, const int64_t (&stride)[3], int b,
                                                int64_t row, int h) {
   return static_cast<const bf16*>(base) + b * stride[0] + row * stride[1] + h * stride[2];
@@ -156,15 +151,6 @@ cudaError_t need_regs(int expected) {
 // ---------------------------------------------------------------- workspace
 // For each chunk and value head, T and P as pairs of swizzled tiles with the
 // decays that go with them.
-struct __align__(16) Gates {
-  float grown[kChunk];  // e^{c_i}
-  float beta[kChunk];
-  float left[kChunk];   // e^{c_64 - c_i}
-  float both[kChunk];   // beta_i e^{c_i}
-  float hi[kChunk];     // c_i = hi + lo
-  float lo[kChunk];
-  float pad[2 * kChunk];
-};
 struct __align__(16) Block {
   unsigned char t_hi[kTile], t_lo[kTile];
   Gates gates;
