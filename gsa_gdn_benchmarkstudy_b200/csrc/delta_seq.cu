@@ -776,14 +776,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // From segment to segment: S_1 = B_0, S_{i+1} = M_i S_i + B_i, in fp32.  A block has
-// 16 columns of a head's state; M_{i+1} is on its way while M_i is used.  256
-// threads hold 2 rows x 4 columns.
+// 16 columns of a head's state; M_{i+1} is on its way while M_i is used.  Bound by
+// shared memory: 64 threads hold 8 rows x 4 columns each, and four such groups share
+// the contraction (one group of 256 threads with 2 x 4: twice the loads).
 constexpr int kLdCut = 132, kCutCols = 16, kCutThreads = 256;
-constexpr int kCutSmem = (2 * 128 * kLdCut + 2 * 128 * kCutCols) * 4;
+constexpr int kCutSmem = (2 * 128 * kLdCut + 6 * 128 * kCutCols) * 4;
 __global__ void __launch_bounds__(kCutThreads) cut_kernel(const gsa_delta_t p, const SeqArgs a) {
   extern __shared__ float cut_smem[];
   float* M = cut_smem;                  // [2][128][kLdCut]
   float* S = M + 2 * 128 * kLdCut;      // [2][128][kCutCols]
+  float* parts = S + 2 * 128 * kCutCols;  // [4][128][kCutCols]
   const int tid = threadIdx.x, hv = blockIdx.y, col0 = blockIdx.z * kCutCols;
   const int cuts = a.seg.count - 1;
   const int64_t size = static_cast<int64_t>(p.dk) * p.dv;
@@ -791,10 +793,11 @@ __global__ void __launch_bounds__(kCutThreads) cut_kernel(const gsa_delta_t p, c
   auto fetch = [&](int i) {
     const float* m = a.seg_m + at(i) * p.dk * p.dk;
     const uint32_t to = smem_u32(M + (i & 1) * 128 * kLdCut);
-    for (int x = tid; x < p.dk * p.dk / 4; x += kCutThreads) {
-      const int r = x / (p.dk / 4), c = x % (p.dk / 4) * 4;
-      cp16(to + (r * kLdCut + c) * 4, m + r * p.dk + c, true);
-    }
+    const int c = (tid & 31) * 4;  // a row a warp
+    if (c < p.dk)
+#pragma unroll 4
+      for (int r = tid >> 5; r < p.dk; r += kCutThreads / 32)
+        cp16(to + (r * kLdCut + c) * 4, m + r * p.dk + c, true);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (cuts > 1) fetch(1);
@@ -808,8 +811,17 @@ __global__ void __launch_bounds__(kCutThreads) cut_kernel(const gsa_delta_t p, c
       S[x] = 0.f;
     }
   }
-  const int r0 = (tid >> 2) * 2, c0 = (tid & 3) * 4;
+  // sums and stores: rows r0 and r0 + 64
+  const int r0 = tid >> 2, c0 = (tid & 3) * 4;
+  const bool real = col0 + c0 < p.dv;
   for (int i = 1; i < cuts; ++i) {
+    const int64_t at_i = at(i) * size + static_cast<int64_t>(r0) * p.dv + col0 + c0;
+    float4 add[2];  // B_i, on its way while M_i is used
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+      add[y] = real && r0 + 64 * y < p.dk
+                   ? *reinterpret_cast<const float4*>(a.seg_b + at_i + 64 * y * p.dv)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
     if (i + 1 < cuts) {
       fetch(i + 1);
       asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -817,45 +829,48 @@ __global__ void __launch_bounds__(kCutThreads) cut_kernel(const gsa_delta_t p, c
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     __syncthreads();
-    const float* m = M + (i & 1) * 128 * kLdCut + r0 * kLdCut;
+    const int rr = (tid >> 2) & 15, part = tid >> 6;
+    const float* m = M + (i & 1) * 128 * kLdCut + rr * kLdCut;
     const float* s = S + ((i & 1) ^ 1) * 128 * kCutCols + c0;
     float* next = S + (i & 1) * 128 * kCutCols;
-    if (r0 < p.dk && col0 + c0 < p.dv) {
-      float acc[2][4];
-      const float* b = a.seg_b + at(i) * size + static_cast<int64_t>(r0) * p.dv + col0 + c0;
-      float* out = a.seg_s + at(i) * size + static_cast<int64_t>(r0) * p.dv + col0 + c0;
+    float acc[8][4] = {};
+#pragma unroll 2
+    for (int k = 4 * part; k < p.dk; k += 16) {
+      float4 u[8], v[4];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const float4 v = *reinterpret_cast<const float4*>(b + y * p.dv);
-        acc[y][0] = v.x; acc[y][1] = v.y; acc[y][2] = v.z; acc[y][3] = v.w;
-      }
-      for (int k = 0; k < p.dk; k += 4) {
-        const float4 m0 = *reinterpret_cast<const float4*>(m + k);
-        const float4 m1 = *reinterpret_cast<const float4*>(m + kLdCut + k);
-        const float ms[2][4] = {{m0.x, m0.y, m0.z, m0.w}, {m1.x, m1.y, m1.z, m1.w}};
+      for (int y = 0; y < 8; ++y)
+        u[y] = *reinterpret_cast<const float4*>(m + 16 * y * kLdCut + k);
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const float4 v = *reinterpret_cast<const float4*>(s + (k + z) * kCutCols);
+      for (int z = 0; z < 4; ++z) v[z] = *reinterpret_cast<const float4*>(s + (k + z) * kCutCols);
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            acc[y][0] = fmaf(ms[y][z], v.x, acc[y][0]);
-            acc[y][1] = fmaf(ms[y][z], v.y, acc[y][1]);
-            acc[y][2] = fmaf(ms[y][z], v.z, acc[y][2]);
-            acc[y][3] = fmaf(ms[y][z], v.w, acc[y][3]);
-          }
+      for (int z = 0; z < 4; ++z)
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const float f = z == 0 ? u[y].x : z == 1 ? u[y].y : z == 2 ? u[y].z : u[y].w;
+          acc[y][0] = fmaf(f, v[z].x, acc[y][0]);
+          acc[y][1] = fmaf(f, v[z].y, acc[y][1]);
+          acc[y][2] = fmaf(f, v[z].z, acc[y][2]);
+          acc[y][3] = fmaf(f, v[z].w, acc[y][3]);
         }
-      }
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const float4 v = make_float4(acc[y][0], acc[y][1], acc[y][2], acc[y][3]);
-        *reinterpret_cast<float4*>(out + y * p.dv) = v;
-        *reinterpret_cast<float4*>(next + (r0 + y) * kCutCols + c0) = v;
-      }
-    } else if (r0 < p.dk) {  // no column of the state: keep the tile's zeros
-      *reinterpret_cast<float4*>(next + r0 * kCutCols + c0) = make_float4(0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<float4*>(next + (r0 + 1) * kCutCols + c0) =
-          make_float4(0.f, 0.f, 0.f, 0.f);
     }
+#pragma unroll
+    for (int y = 0; y < 8; ++y)
+      *reinterpret_cast<float4*>(parts + (part * 128 + rr + 16 * y) * kCutCols + c0) =
+          make_float4(acc[y][0], acc[y][1], acc[y][2], acc[y][3]);
+    __syncthreads();
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+      if (r0 + 64 * y < p.dk) {
+        float4 v = add[y];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float4 o = *reinterpret_cast<const float4*>(
+              parts + (x * 128 + r0 + 64 * y) * kCutCols + c0);
+          v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+        }
+        if (real) *reinterpret_cast<float4*>(a.seg_s + at_i + 64 * y * p.dv) = v;
+        *reinterpret_cast<float4*>(next + (r0 + 64 * y) * kCutCols + c0) = v;
+      }
     __syncthreads();
   }
 }
@@ -894,7 +909,7 @@ cudaError_t forward(const gsa_delta_t& p, const DeltaMaps& m, const SeqArgs& a,
 // Of all cuts the one whose blocks take the least time, counted in rounds of 148
 // blocks: a chunk takes 2.9 us in the full pass, and 1.4 us more where all SMs read
 // at once; 2.8 us in the one for M and B (128 columns each of B and M, all segments
-// but the last); a step between segments 4.5 us.  16 heads of 16384 tokens take 0.76
+// but the last); a step between segments 3.2 us.  16 heads of 16384 tokens take 0.76
 // ms uncut and 0.33 ms in nine segments; 64 heads of 4096 0.23 ms, and 0.24 in two.
 Segments segments_of(const gsa_delta_t& p) {
   if (p.cu_seqlens || p.T < 16 * kChunk) return {1, p.T / kChunk + 1};
@@ -911,7 +926,7 @@ Segments segments_of(const gsa_delta_t& p) {
     if (each < 8) break;
     const double time = each * (2.8 * rounds(heads * (cols + 1) * (count - 1)) +
                                 full(heads * cols * count)) +
-                        4.5 * count + 10.0;
+                        3.2 * count + 10.0;
     if (time < least) {
       least = time;
       best = {count, each};
