@@ -5,7 +5,12 @@
 //   r = a S^T k,  w = a S^T q,  u = beta (v - r),  o = scale (w + (q.k) u),
 //   S <- a S + k u^T,
 // so the state is read once, stays in registers over all tokens of the call,
-// and is written once.  Bound by HBM: 8 * dk * dv bytes a head and sequence.
+// and is written once.  Bound by HBM: 8 * dk * dv bytes a head and sequence, and by
+// how many of them are on their way: 128 sequences of 16 heads of 128 x 128 take 49 us
+// with seven blocks of 16 KB an SM (72 registers a thread) and states that leave the
+// caches early, 53 with the four that 109 registers allow, 52 with eight, which spill
+// (a plain copy of the bytes takes 41).  Blocks of 64 and 128 columns take 61 and 83:
+// more warps meet at each barrier.
 #include "delta_common.cuh"
 
 namespace gsa {
@@ -18,7 +23,7 @@ constexpr int kRowGroups = kThreads / 8;
 constexpr int kMaxRows = kDeltaMaxDk / kRowGroups;
 
 template <typename E>
-__global__ void __launch_bounds__(kThreads) delta_step_kernel(const gsa_delta_t p, float* pool,
+__global__ void __launch_bounds__(kThreads, 7) delta_step_kernel(const gsa_delta_t p, float* pool,
                                                               int64_t slots,
                                                               const int32_t* indices, E* out,
                                                               int* err) {
@@ -41,7 +46,7 @@ __global__ void __launch_bounds__(kThreads) delta_step_kernel(const gsa_delta_t 
     const int r = rg + i * kRowGroups;
     S[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (inside && live && r < p.dk)
-      S[i] = *reinterpret_cast<const float4*>(state + static_cast<int64_t>(r) * p.dv + col);
+      S[i] = __ldcs(reinterpret_cast<const float4*>(state + static_cast<int64_t>(r) * p.dv + col));
   }
   // Two rows of the batch must not share a state: the later one is refused, as
   // is an index outside the pool (-1 is an empty row): NaN out, no state
@@ -144,7 +149,7 @@ __global__ void __launch_bounds__(kThreads) delta_step_kernel(const gsa_delta_t 
   for (int i = 0; i < kMaxRows; ++i) {
     const int r = rg + i * kRowGroups;
     if (live && r < p.dk)
-      *reinterpret_cast<float4*>(state + static_cast<int64_t>(r) * p.dv + col) = S[i];
+      __stcs(reinterpret_cast<float4*>(state + static_cast<int64_t>(r) * p.dv + col), S[i]);
   }
 }
 
