@@ -16,7 +16,8 @@
 // row was measured at 16384 rows of 2048 (bf16, residual; a plain copy of the
 // same bytes takes 41 us): 32 threads x 8 vectors 55 us, 64 x 4 47, 128 x 2 47,
 // 256 x 1 51; with an 8-bit output (36 us) 62, 47, 53, 63.  Fewer vectors a thread
-// leave too few loads in flight, more of them too few warps.
+// leave too few loads in flight, more of them too few warps.  Held to 64 registers
+// (of 70) 64 x 4 takes 45 and 46.
 #include <cuda_fp8.h>
 
 #include "kernels.h"
@@ -42,7 +43,9 @@ __device__ __forceinline__ int column(int i, int e, int t, int tpr) {
   return VECTOR ? (i * tpr + t) * kVec + e : (i * kVec + e) * tpr + t;
 }
 
-// Eight values as they lie in memory: loads that can wait to be converted.
+// Eight values as they lie in memory: loads that can wait to be converted.  ONCE:
+// they leave the caches early.  The backward pass gains by it (54 to 50 us, figures as
+// above), the forward pass loses (45 to 51): its inputs and outputs are often in L2.
 template <typename E>
 struct Raw {
   static constexpr int kWords = kVec * sizeof(E) / 16;
@@ -65,14 +68,16 @@ __device__ __forceinline__ void unpack(float (&v)[kVec], const Raw<float>& r) {
     v[4 * j + 3] = __uint_as_float(r.w[j].w);
   }
 }
-template <bool VECTOR, typename E>
+template <bool VECTOR, bool ONCE, typename E>
 __device__ __forceinline__ void load_raw(Raw<E>& r, const E* row, int i, int t, int tpr,
                                          int width) {
   if constexpr (VECTOR) {
     const int c = column<true>(i, 0, t, tpr);
 #pragma unroll
-    for (int j = 0; j < Raw<E>::kWords; ++j)
-      r.w[j] = c < width ? reinterpret_cast<const uint4*>(row + c)[j] : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < Raw<E>::kWords; ++j) {
+      const uint4* at = reinterpret_cast<const uint4*>(row + c) + j;
+      r.w[j] = c < width ? (ONCE ? __ldcs(at) : *at) : make_uint4(0, 0, 0, 0);
+    }
   } else {
     E e[kVec];
 #pragma unroll
@@ -87,7 +92,7 @@ template <bool VECTOR, typename E>
 __device__ __forceinline__ void load8(float (&v)[kVec], const E* row, int i, int t, int tpr,
                                       int width) {
   Raw<E> r;
-  load_raw<VECTOR>(r, row, i, t, tpr, width);
+  load_raw<VECTOR, false>(r, row, i, t, tpr, width);
   unpack(v, r);
 }
 
@@ -174,7 +179,8 @@ enum NormOut { kNormPlain = 0, kNormRow8 = 1, kNormGroup8 = 2 };
 // tpr threads share a row; a block holds blockDim.x / tpr rows (more than one
 // only where a row is a warp or less).
 template <typename E, bool VECTOR, int NV, int OUT, int THREADS>
-__global__ void __launch_bounds__(THREADS) rms_norm_kernel(RmsNormArgs a, int tpr) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1)
+    rms_norm_kernel(RmsNormArgs a, int tpr) {
   __shared__ float slots[2][32];
   const int t = threadIdx.x % tpr;
   int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
@@ -276,11 +282,11 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(RmsNormBackw
     rstd_next = a.rstd[row];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      load_raw<VECTOR>(h_raw[i], static_cast<const E*>(a.h) + row * a.h_stride, i, t, tpr, a.width);
-      load_raw<VECTOR>(dy_raw[i], static_cast<const E*>(a.dy) + row * a.dy_stride, i, t, tpr,
+      load_raw<VECTOR, true>(h_raw[i], static_cast<const E*>(a.h) + row * a.h_stride, i, t, tpr, a.width);
+      load_raw<VECTOR, true>(dy_raw[i], static_cast<const E*>(a.dy) + row * a.dy_stride, i, t, tpr,
                        a.width);
       if (a.dh)
-        load_raw<VECTOR>(d_raw[i], static_cast<const E*>(a.dh) + row * a.dh_stride, i, t, tpr,
+        load_raw<VECTOR, true>(d_raw[i], static_cast<const E*>(a.dh) + row * a.dh_stride, i, t, tpr,
                          a.width);
     }
   };
@@ -347,8 +353,8 @@ __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* partial,
 
 // Threads for a row of `width` values and vectors for each of them (measured
 // above): four vectors a thread where rows fill the SMs, one where they do not;
-// backwards one, and two past 2048 values; no fewer than `least` threads: 8, 16 where they hold a group of 128 values, 32
-// backwards, where a row is a block's.
+// backwards one, and two past 2048 values; no fewer than `least` threads: 8, 16 where
+// they hold a group of 128 values, 32 backwards, where a row is a block's.
 struct Shape {
   int tpr, nv;
 };
@@ -362,7 +368,7 @@ Shape shape_of(int64_t rows, int width, int least) {
   return {tpr, nv};
 }
 
-// Blocks of up to 256 threads may use 255 registers a thread, wider ones 64.
+// Wider blocks than 256 threads are kernels of their own.
 template <typename E, bool VECTOR, int NV, int THREADS>
 cudaError_t launch_norm_nv(const RmsNormArgs& a, int tpr, cudaStream_t stream) {
   const int rows_per_block = tpr <= 32 ? 128 / tpr : 1;
@@ -425,7 +431,7 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, int dtype, cudaStream_t stream
 }
 
 // 768 threads an SM, each with the next row's loads in flight: 16384 rows of 2048
-// take 53 us so, 57 with twice as many, 65 with two thirds (41 us for the bytes);
+// took 53 us so, 57 with twice as many, 65 with two thirds (41 us for the bytes);
 // more blocks also mean more partial sums of dw.
 int rms_norm_backward_blocks(int64_t rows, int width) {
   const Shape s = shape_of(rows, width, 32);
