@@ -17,7 +17,7 @@
 // same bytes takes 41 us): 32 threads x 8 vectors 55 us, 64 x 4 47, 128 x 2 47,
 // 256 x 1 51; with an 8-bit output (36 us) 62, 47, 53, 63.  Fewer vectors a thread
 // leave too few loads in flight, more of them too few warps.  Held to 64 registers
-// (of 70) 64 x 4 takes 45 and 46.
+// (of 70) 64 x 4 takes 45; the other forms would spill.
 #include <cuda_fp8.h>
 
 #include "kernels.h"
@@ -179,7 +179,7 @@ enum NormOut { kNormPlain = 0, kNormRow8 = 1, kNormGroup8 = 2 };
 // tpr threads share a row; a block holds blockDim.x / tpr rows (more than one
 // only where a row is a warp or less).
 template <typename E, bool VECTOR, int NV, int OUT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1)
+__global__ void __launch_bounds__(THREADS, THREADS == 256 && VECTOR && sizeof(E) == 2 ? 4 : 1)
     rms_norm_kernel(RmsNormArgs a, int tpr) {
   __shared__ float slots[2][32];
   const int t = threadIdx.x % tpr;
