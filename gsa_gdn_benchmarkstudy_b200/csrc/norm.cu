@@ -403,6 +403,8 @@ void launch_back(const RmsNormBackwardArgs& a, const Shape& s, int blocks, cudaS
   if (s.tpr <= 256)
     s.nv == 1 ? rms_norm_backward_kernel<E, VECTOR, 1, 256><<<blocks, s.tpr, 0, stream>>>(a)
               : rms_norm_backward_kernel<E, VECTOR, 2, 256><<<blocks, s.tpr, 0, stream>>>(a);
+  else if (s.tpr == 512)  // two vectors a thread
+    rms_norm_backward_kernel<E, VECTOR, 2, 512><<<blocks, s.tpr, 0, stream>>>(a);
   else if (s.nv <= 2)
     rms_norm_backward_kernel<E, VECTOR, 2, 1024><<<blocks, s.tpr, 0, stream>>>(a);
   else
@@ -432,10 +434,12 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, int dtype, cudaStream_t stream
 
 // 768 threads an SM, each with the next row's loads in flight: 16384 rows of 2048
 // took 53 us so, 57 with twice as many, 65 with two thirds (41 us for the bytes);
-// more blocks also mean more partial sums of dw.
+// more blocks also mean more partial sums of dw.  512 threads where each holds two
+// vectors, so that all blocks run at once: 8192 rows of 4096 take 70 us with 768.
 int rms_norm_backward_blocks(int64_t rows, int width) {
   const Shape s = shape_of(rows, width, 32);
-  const int64_t most = 148 * (768 / s.tpr < 1 ? 1 : 768 / s.tpr);
+  const int threads = s.nv == 1 ? 768 : 512;
+  const int64_t most = 148 * (threads / s.tpr < 1 ? 1 : threads / s.tpr);
   return static_cast<int>(rows < most ? rows : most);
 }
 
