@@ -35,12 +35,32 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float
 __device__ __forceinline__ float round_f(float v, float) { return v; }
 __device__ __forceinline__ float round_f(float v, __nv_bfloat16) { return bf16_round(v); }
 
-// Column of value e of a thread's vector i.  Vector form: 8 neighbours, so a
-// thread moves 16 bytes (bf16) at once.  Plain form (a width or an address that
-// breaks the 16-byte rule): neighbours go to neighbouring threads.
-template <bool VECTOR>
-__device__ __forceinline__ int column(int i, int e, int t, int tpr) {
-  return VECTOR ? (i * tpr + t) * kVec + e : (i * kVec + e) * tpr + t;
+// How a thread's vectors of 8 values lie in a row.
+//   kPlain    neighbours go to neighbouring threads, one value a load;
+//   kVector   8 neighbours, 16 bytes (bf16) at once;
+//   kShifted  the same where rows start off the 16-byte grid (an odd width): windows
+//             of 8 on the grid, the first one `shift` values before the row, so all but
+//             a row's first and last still move 16 bytes at once.  All tensors of a
+//             call then start off the grid alike.
+// 8192 rows of 4099 in bf16 with a residual take 357 us plain and 106 shifted (41
+// for the bytes).
+enum Form { kPlain = 0, kVector = 1, kShifted = 2 };
+// Column of value e of vector i.
+template <int FORM>
+__device__ __forceinline__ int column(int i, int e, int t, int tpr, int shift) {
+  return FORM == kPlain ? (i * kVec + e) * tpr + t
+                        : (i * tpr + t) * kVec + e - (FORM == kShifted ? shift : 0);
+}
+// Whether vector i lies in the row, and whole.
+template <int FORM>
+__device__ __forceinline__ bool whole_vector(int c, int width) {
+  return FORM == kShifted ? c >= 0 && c + kVec <= width : FORM == kVector && c < width;
+}
+
+// Values between the 8-value grid and p.
+template <typename E>
+__host__ __device__ __forceinline__ int off_grid(const E* p) {
+  return static_cast<int>((reinterpret_cast<uintptr_t>(p) / sizeof(E)) % kVec);
 }
 
 // Eight values as they lie in memory: loads that can wait to be converted.  ONCE:
@@ -68,11 +88,11 @@ __device__ __forceinline__ void unpack(float (&v)[kVec], const Raw<float>& r) {
     v[4 * j + 3] = __uint_as_float(r.w[j].w);
   }
 }
-template <bool VECTOR, bool ONCE, typename E>
+template <int FORM, bool ONCE, typename E>
 __device__ __forceinline__ void load_raw(Raw<E>& r, const E* row, int i, int t, int tpr,
-                                         int width) {
-  if constexpr (VECTOR) {
-    const int c = column<true>(i, 0, t, tpr);
+                                         int width, int shift) {
+  const int c = column<FORM>(i, 0, t, tpr, shift);
+  if (FORM == kVector || whole_vector<FORM>(c, width)) {
 #pragma unroll
     for (int j = 0; j < Raw<E>::kWords; ++j) {
       const uint4* at = reinterpret_cast<const uint4*>(row + c) + j;
@@ -81,27 +101,70 @@ __device__ __forceinline__ void load_raw(Raw<E>& r, const E* row, int i, int t, 
   } else {
     E e[kVec];
 #pragma unroll
-    for (int x = 0; x < kVec; ++x) {
-      const int c = column<false>(i, x, t, tpr);
-      e[x] = c < width ? row[c] : from_f<E>(0.f);
-    }
+    for (int x = 0; x < kVec; ++x) e[x] = from_f<E>(0.f);
+    if (c < width)
+#pragma unroll
+      for (int x = 0; x < kVec; ++x) {
+        const int at = column<FORM>(i, x, t, tpr, shift);
+        if (at >= 0 && at < width) e[x] = row[at];
+      }
     memcpy(&r, e, sizeof(r));
   }
 }
-template <bool VECTOR, typename E>
+template <int FORM, typename E>
 __device__ __forceinline__ void load8(float (&v)[kVec], const E* row, int i, int t, int tpr,
-                                      int width) {
+                                      int width, int shift) {
   Raw<E> r;
-  load_raw<VECTOR, false>(r, row, i, t, tpr, width);
+  load_raw<FORM, false>(r, row, i, t, tpr, width, shift);
   unpack(v, r);
 }
 
-template <bool VECTOR, typename E>
+// The weight's values for vector i.  Shifted: two vectors of a weight in bf16 on the
+// grid, and the 8 values from their middle.
+template <int FORM, typename A>
+__device__ __forceinline__ void load_weight(float (&w)[kVec], const A& a, int i, int t, int tpr,
+                                            int shift) {
+  if constexpr (FORM != kShifted) {
+    if (a.weight_f32)
+      load8<FORM>(w, static_cast<const float*>(a.weight), i, t, tpr, a.width, 0);
+    else
+      load8<FORM>(w, static_cast<const __nv_bfloat16*>(a.weight), i, t, tpr, a.width, 0);
+  } else {
+    const int c = column<FORM>(i, 0, t, tpr, shift), from = c & ~7;
+    if (!a.weight_f32 && c >= 0 && from + 2 * kVec <= a.width) {
+      const uint4* at = reinterpret_cast<const uint4*>(
+          static_cast<const __nv_bfloat16*>(a.weight) + from);
+      const uint4 x = at[0], y = at[1];
+      uint32_t r[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int j = 0; j < 6; ++j) r[j] = c & 4 ? r[j + 2] : r[j];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) r[j] = c & 2 ? r[j + 1] : r[j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t z = c & 1 ? __funnelshift_r(r[j], r[j + 1], 16) : r[j];
+        w[2 * j] = __uint_as_float(z << 16);
+        w[2 * j + 1] = __uint_as_float(z & 0xFFFF0000u);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) w[e] = 0.f;
+      if (c < a.width)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (c + e >= 0 && c + e < a.width)
+            w[e] = a.weight_f32 ? static_cast<const float*>(a.weight)[c + e]
+                                : __bfloat162float(
+                                      static_cast<const __nv_bfloat16*>(a.weight)[c + e]);
+    }
+  }
+}
+
+template <int FORM, typename E>
 __device__ __forceinline__ void store8(const float (&v)[kVec], E* row, int i, int t, int tpr,
-                                       int width) {
-  if constexpr (VECTOR) {
-    const int c = column<true>(i, 0, t, tpr);
-    if (c >= width) return;
+                                       int width, int shift) {
+  const int c = column<FORM>(i, 0, t, tpr, shift);
+  if (whole_vector<FORM>(c, width)) {
     if constexpr (sizeof(E) == 2) {
       uint4 raw;
       raw.x = pack_bf16x2(v[0], v[1]);
@@ -113,18 +176,18 @@ __device__ __forceinline__ void store8(const float (&v)[kVec], E* row, int i, in
       *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
       *reinterpret_cast<float4*>(row + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
     }
-  } else {
+  } else if (FORM != kVector && c < width) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
-      const int c = column<false>(i, e, t, tpr);
-      if (c < width) row[c] = from_f<E>(v[e]);
+      const int at = column<FORM>(i, e, t, tpr, shift);
+      if (at >= 0 && at < width) row[at] = from_f<E>(v[e]);
     }
   }
 }
 
-template <bool VECTOR>
+template <int FORM>
 __device__ __forceinline__ void store8_e4m3(const float (&v)[kVec], uint8_t* row, int i, int t,
-                                            int tpr, int width) {
+                                            int tpr, int width, int shift) {
   uint32_t lo = 0, hi = 0;
 #pragma unroll
   for (int e = 0; e < 4; e += 2) {
@@ -133,14 +196,14 @@ __device__ __forceinline__ void store8_e4m3(const float (&v)[kVec], uint8_t* row
     hi |= uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(v[e + 4], v[e + 5]), __NV_SATFINITE,
                                             __NV_E4M3)) << (8 * e);
   }
-  if constexpr (VECTOR) {
-    const int c = column<true>(i, 0, t, tpr);
-    if (c < width) *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
-  } else {
+  const int c = column<FORM>(i, 0, t, tpr, shift);
+  if (whole_vector<FORM>(c, width)) {
+    *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+  } else if (FORM != kVector && c < width) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
-      const int c = column<false>(i, e, t, tpr);
-      if (c < width) row[c] = static_cast<uint8_t>((e < 4 ? lo : hi) >> (8 * (e & 3)));
+      const int at = column<FORM>(i, e, t, tpr, shift);
+      if (at >= 0 && at < width) row[at] = static_cast<uint8_t>((e < 4 ? lo : hi) >> (8 * (e & 3)));
     }
   }
 }
@@ -153,7 +216,7 @@ __device__ __forceinline__ float fold_max(float a, float b) {
   return r;
 }
 
-// Sum or maximum over the tpr threads of a row (a power of two from 8 on; rows
+// Sum or maximum over the tpr threads of a row (8, 16, 32, or whole warps; rows
 // within a warp need no barrier).  `slot` has room for 32 values and is not used
 // again before the caller's next barrier.
 template <bool MAX>
@@ -167,19 +230,20 @@ __device__ __forceinline__ float row_fold(float v, float* slot, int tpr) {
   if (lane == 0) slot[warp] = v;
   __syncthreads();
   v = lane < nw ? slot[lane] : 0.f;
-  for (int m = nw >> 1; m; m >>= 1) {
+#pragma unroll
+  for (int m = 16; m; m >>= 1) {
     const float o = __shfl_xor_sync(0xFFFFFFFFu, v, m);
     v = MAX ? fold_max(v, o) : fold_sum(v, o);
   }
-  return __shfl_sync(0xFFFFFFFFu, v, 0);
+  return v;
 }
 
 enum NormOut { kNormPlain = 0, kNormRow8 = 1, kNormGroup8 = 2 };
 
 // tpr threads share a row; a block holds blockDim.x / tpr rows (more than one
 // only where a row is a warp or less).
-template <typename E, bool VECTOR, int NV, int OUT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 && VECTOR && sizeof(E) == 2 ? 4 : 1)
+template <typename E, int FORM, int NV, int OUT, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 && FORM == kVector && sizeof(E) == 2 ? 4 : 1)
     rms_norm_kernel(RmsNormArgs a, int tpr) {
   __shared__ float slots[2][32];
   const int t = threadIdx.x % tpr;
@@ -189,19 +253,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 && VECTOR && sizeof(E)
   if (!live) row = a.rows - 1;
   const E* x = static_cast<const E*>(a.x) + row * a.x_stride;
   const E* res = a.residual ? static_cast<const E*>(a.residual) + row * a.residual_stride : nullptr;
+  const int shift = FORM == kShifted ? off_grid(x) : 0;
   float v[NV][kVec];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) load8<VECTOR>(v[i], x, i, t, tpr, a.width);
+  for (int i = 0; i < NV; ++i) load8<FORM>(v[i], x, i, t, tpr, a.width, shift);
   if (res) {
     float r[NV][kVec];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load8<VECTOR>(r[i], res, i, t, tpr, a.width);
+    for (int i = 0; i < NV; ++i) load8<FORM>(r[i], res, i, t, tpr, a.width, shift);
     E* h = static_cast<E*>(a.h) + row * a.h_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) v[i][e] = round_f(v[i][e] + r[i][e], E());
-      if (live) store8<VECTOR>(v[i], h, i, t, tpr, a.width);
+      if (live) store8<FORM>(v[i], h, i, t, tpr, a.width, shift);
     }
   }
   float s = 0.f;
@@ -215,10 +280,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 && VECTOR && sizeof(E)
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     float w[kVec];
-    if (a.weight_f32)
-      load8<VECTOR>(w, static_cast<const float*>(a.weight), i, t, tpr, a.width);
-    else
-      load8<VECTOR>(w, static_cast<const __nv_bfloat16*>(a.weight), i, t, tpr, a.width);
+    load_weight<FORM>(w, a, i, t, tpr, shift);
 #pragma unroll
     for (int e = 0; e < kVec; ++e) v[i][e] = v[i][e] * rstd * w[e];
   }
@@ -226,7 +288,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 && VECTOR && sizeof(E)
     E* y = static_cast<E*>(a.y) + row * a.y_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (live) store8<VECTOR>(v[i], y, i, t, tpr, a.width);
+      if (live) store8<FORM>(v[i], y, i, t, tpr, a.width, shift);
   } else {
     uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.y_stride;
     float most = 0.f;
@@ -247,14 +309,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 && VECTOR && sizeof(E)
 #pragma unroll
         for (int m = 8; m; m >>= 1) most = fold_max(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
         most = fold_max(most, 1e-12f);
-        const int c = column<true>(i, 0, t, tpr);
+        const int c = column<FORM>(i, 0, t, tpr, shift);
         if (live && c < a.width && (t & 15) == 0)
           a.scale[row * (a.width >> 7) + (c >> 7)] = most / 448.0f;
       }
       const float inv = 448.0f / most;
 #pragma unroll
       for (int e = 0; e < kVec; ++e) v[i][e] *= inv;
-      if (live) store8_e4m3<VECTOR>(v[i], y, i, t, tpr, a.width);
+      if (live) store8_e4m3<FORM>(v[i], y, i, t, tpr, a.width, shift);
     }
   }
 }
@@ -263,31 +325,30 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 && VECTOR && sizeof(E)
 // share of dw in registers over all of them; the shares go to partial[b] and
 // are added in block order by rms_norm_dw_kernel, so equal inputs give equal
 // bits.  The next row's loads are in flight while a row's sum crosses the block.
-template <typename E, bool VECTOR, int NV, int THREADS>
+template <typename E, int FORM, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(RmsNormBackwardArgs a) {
   __shared__ float slots[2][32];
   const int tpr = blockDim.x, t = threadIdx.x;
+  // a shifted form's grid is a multiple of 8, so that a block's rows start alike
+  const int shift =
+      FORM == kShifted ? off_grid(static_cast<const E*>(a.h) + blockIdx.x * a.h_stride) : 0;
   float dw[NV][kVec] = {};
   float w[NV][kVec];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (a.weight_f32)
-      load8<VECTOR>(w[i], static_cast<const float*>(a.weight), i, t, tpr, a.width);
-    else
-      load8<VECTOR>(w[i], static_cast<const __nv_bfloat16*>(a.weight), i, t, tpr, a.width);
-  }
+  for (int i = 0; i < NV; ++i) load_weight<FORM>(w[i], a, i, t, tpr, shift);
   Raw<E> h_raw[NV], dy_raw[NV], d_raw[NV];
   float rstd_next = 0.f;
   auto fetch = [&](int64_t row) {
     rstd_next = a.rstd[row];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      load_raw<VECTOR, true>(h_raw[i], static_cast<const E*>(a.h) + row * a.h_stride, i, t, tpr, a.width);
-      load_raw<VECTOR, true>(dy_raw[i], static_cast<const E*>(a.dy) + row * a.dy_stride, i, t, tpr,
-                       a.width);
+      load_raw<FORM, true>(h_raw[i], static_cast<const E*>(a.h) + row * a.h_stride, i, t, tpr, a.width,
+                           shift);
+      load_raw<FORM, true>(dy_raw[i], static_cast<const E*>(a.dy) + row * a.dy_stride, i, t, tpr,
+                           a.width, shift);
       if (a.dh)
-        load_raw<VECTOR, true>(d_raw[i], static_cast<const E*>(a.dh) + row * a.dh_stride, i, t, tpr,
-                         a.width);
+        load_raw<FORM, true>(d_raw[i], static_cast<const E*>(a.dh) + row * a.dh_stride, i, t, tpr,
+                             a.width, shift);
     }
   };
   if (blockIdx.x < a.rows) fetch(blockIdx.x);
@@ -317,7 +378,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(RmsNormBackw
         const float g = rstd * (dy[i][e] * w[i][e] - h[i][e] * back);
         h[i][e] = a.dh ? g + d[i][e] : g;
       }
-      store8<VECTOR>(h[i], static_cast<E*>(a.dx) + row * a.dx_stride, i, t, tpr, a.width);
+      store8<FORM>(h[i], static_cast<E*>(a.dx) + row * a.dx_stride, i, t, tpr, a.width, shift);
     }
   }
   if (a.partial) {
@@ -326,8 +387,8 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(RmsNormBackw
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        const int c = column<VECTOR>(i, e, t, tpr);
-        if (c < a.width) p[c] = dw[i][e];
+        const int c = column<FORM>(i, e, t, tpr, shift);
+        if (c >= 0 && c < a.width) p[c] = dw[i][e];
       }
   }
 }
@@ -352,7 +413,8 @@ __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* partial,
 }
 
 // Threads for a row of `width` values and vectors for each of them (measured
-// above): four vectors a thread where rows fill the SMs, one where they do not;
+// above): four vectors a thread where rows fill the SMs, one where they do not, in
+// whole warps (rows of 2100: 75 us with a power of two of threads, 63 with 96);
 // backwards one, and two past 2048 values; no fewer than `least` threads: 8, 16 where
 // they hold a group of 128 values, 32 backwards, where a row is a block's.
 struct Shape {
@@ -362,57 +424,98 @@ Shape shape_of(int64_t rows, int width, int least) {
   const int vectors = (width + kVec - 1) / kVec;
   int tpr = least;
   const int most = least == 32 ? (vectors > 256 ? 2 : 1) : (rows >= 2048 ? 4 : 1);
-  while (tpr < 1024 && tpr * most < vectors) tpr *= 2;
+  while (tpr < 32 && tpr * most < vectors) tpr *= 2;
+  if (tpr * most < vectors) {  // whole warps
+    tpr = ((vectors + most - 1) / most + 31) / 32 * 32;
+    tpr = tpr < 1024 ? tpr : 1024;
+  }
   int nv = 1;
   while (tpr * nv < vectors) nv *= 2;
   return {tpr, nv};
 }
 
 // Wider blocks than 256 threads are kernels of their own.
-template <typename E, bool VECTOR, int NV, int THREADS>
+template <typename E, int FORM, int NV, int THREADS>
 cudaError_t launch_norm_nv(const RmsNormArgs& a, int tpr, cudaStream_t stream) {
   const int rows_per_block = tpr <= 32 ? 128 / tpr : 1;
   const int64_t blocks = (a.rows + rows_per_block - 1) / rows_per_block;
   const dim3 grid(static_cast<unsigned>(blocks)), block(tpr * rows_per_block);
   if (!a.scale)
-    rms_norm_kernel<E, VECTOR, NV, kNormPlain, THREADS><<<grid, block, 0, stream>>>(a, tpr);
+    rms_norm_kernel<E, FORM, NV, kNormPlain, THREADS><<<grid, block, 0, stream>>>(a, tpr);
   else if (a.group == 0)
-    rms_norm_kernel<E, VECTOR, NV, kNormRow8, THREADS><<<grid, block, 0, stream>>>(a, tpr);
-  else if constexpr (VECTOR)
-    rms_norm_kernel<E, true, NV, kNormGroup8, THREADS><<<grid, block, 0, stream>>>(a, tpr);
+    rms_norm_kernel<E, FORM, NV, kNormRow8, THREADS><<<grid, block, 0, stream>>>(a, tpr);
+  else if constexpr (FORM == kVector)
+    rms_norm_kernel<E, kVector, NV, kNormGroup8, THREADS><<<grid, block, 0, stream>>>(a, tpr);
   return cudaGetLastError();
 }
 
-template <typename E, bool VECTOR>
+template <typename E, int FORM>
 cudaError_t launch_norm(const RmsNormArgs& a, cudaStream_t stream) {
-  const Shape s = shape_of(a.rows, a.width, a.group ? 16 : 8);
+  const Shape s = shape_of(a.rows, a.width + (FORM == kShifted ? kVec - 1 : 0), a.group ? 16 : 8);
   if (s.tpr > 256) switch (s.nv) {
-      case 1: return launch_norm_nv<E, VECTOR, 1, 1024>(a, s.tpr, stream);
-      case 2: return launch_norm_nv<E, VECTOR, 2, 1024>(a, s.tpr, stream);
-      default: return launch_norm_nv<E, VECTOR, 4, 1024>(a, s.tpr, stream);
+      case 1: return launch_norm_nv<E, FORM, 1, 1024>(a, s.tpr, stream);
+      case 2: return launch_norm_nv<E, FORM, 2, 1024>(a, s.tpr, stream);
+      default: return launch_norm_nv<E, FORM, 4, 1024>(a, s.tpr, stream);
     }
   switch (s.nv) {
-    case 1: return launch_norm_nv<E, VECTOR, 1, 256>(a, s.tpr, stream);
-    case 2: return launch_norm_nv<E, VECTOR, 2, 256>(a, s.tpr, stream);
-    default: return launch_norm_nv<E, VECTOR, 4, 256>(a, s.tpr, stream);
+    case 1: return launch_norm_nv<E, FORM, 1, 256>(a, s.tpr, stream);
+    case 2: return launch_norm_nv<E, FORM, 2, 256>(a, s.tpr, stream);
+    default: return launch_norm_nv<E, FORM, 4, 256>(a, s.tpr, stream);
   }
 }
 
-template <typename E, bool VECTOR>
+template <typename E, int FORM>
 void launch_back(const RmsNormBackwardArgs& a, const Shape& s, int blocks, cudaStream_t stream) {
   if (s.tpr <= 256)
-    s.nv == 1 ? rms_norm_backward_kernel<E, VECTOR, 1, 256><<<blocks, s.tpr, 0, stream>>>(a)
-              : rms_norm_backward_kernel<E, VECTOR, 2, 256><<<blocks, s.tpr, 0, stream>>>(a);
-  else if (s.tpr == 512)  // two vectors a thread
-    rms_norm_backward_kernel<E, VECTOR, 2, 512><<<blocks, s.tpr, 0, stream>>>(a);
+    s.nv == 1 ? rms_norm_backward_kernel<E, FORM, 1, 256><<<blocks, s.tpr, 0, stream>>>(a)
+              : rms_norm_backward_kernel<E, FORM, 2, 256><<<blocks, s.tpr, 0, stream>>>(a);
+  else if (s.tpr <= 512)  // two vectors a thread
+    rms_norm_backward_kernel<E, FORM, 2, 512><<<blocks, s.tpr, 0, stream>>>(a);
   else if (s.nv <= 2)
-    rms_norm_backward_kernel<E, VECTOR, 2, 1024><<<blocks, s.tpr, 0, stream>>>(a);
+    rms_norm_backward_kernel<E, FORM, 2, 1024><<<blocks, s.tpr, 0, stream>>>(a);
   else
-    rms_norm_backward_kernel<E, VECTOR, 4, 1024><<<blocks, s.tpr, 0, stream>>>(a);
+    rms_norm_backward_kernel<E, FORM, 4, 1024><<<blocks, s.tpr, 0, stream>>>(a);
 }
 
 bool vector_ok(const void* p, int64_t stride, int elem) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride * elem) % 16 == 0;
+}
+
+// Whether the rows of all tensors start off the 8-value grid alike.
+struct Grid {
+  int64_t rows;
+  int off, step;
+  bool alike = true;
+  Grid(const void* p, int64_t stride, int elem, int64_t n)
+      : rows(n), off(place(p, elem)), step(static_cast<int>(stride % kVec)) {}
+  static int place(const void* p, int elem) {
+    return static_cast<int>((reinterpret_cast<uintptr_t>(p) / elem) % kVec);
+  }
+  void with(const void* p, int64_t stride, int elem) {
+    alike = alike && place(p, elem) == off && (rows < 2 || stride % kVec == step);
+  }
+};
+// The widest row's windows are 1024 threads' four vectors.
+bool shifted_ok(const Grid& g, const void* weight, int width) {
+  return g.alike && vector_ok(weight, 0, 1) && (width + 2 * (kVec - 1)) / kVec <= 4096;
+}
+
+template <typename E>
+cudaError_t launch_form(const RmsNormArgs& a, int form, cudaStream_t stream) {
+  switch (form) {
+    case kVector: return launch_norm<E, kVector>(a, stream);
+    case kShifted: return launch_norm<E, kShifted>(a, stream);
+    default: return launch_norm<E, kPlain>(a, stream);
+  }
+}
+template <typename E>
+void launch_back_form(const RmsNormBackwardArgs& a, int form, const Shape& s, int blocks,
+                      cudaStream_t stream) {
+  switch (form) {
+    case kVector: return launch_back<E, kVector>(a, s, blocks, stream);
+    case kShifted: return launch_back<E, kShifted>(a, s, blocks, stream);
+    default: return launch_back<E, kPlain>(a, s, blocks, stream);
+  }
 }
 
 }  // namespace
@@ -426,10 +529,15 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, int dtype, cudaStream_t stream
   vec = vec && (a.scale ? reinterpret_cast<uintptr_t>(a.y) % 8 == 0 && a.y_stride % 8 == 0
                         : vector_ok(a.y, a.y_stride, e));
   if (a.scale && a.group && !vec) return cudaErrorMisalignedAddress;
-  if (dtype == GSA_DTYPE_BF16)
-    return vec ? launch_norm<__nv_bfloat16, true>(a, stream)
-               : launch_norm<__nv_bfloat16, false>(a, stream);
-  return vec ? launch_norm<float, true>(a, stream) : launch_norm<float, false>(a, stream);
+  Grid grid(a.x, a.x_stride, e, a.rows);
+  grid.with(a.y, a.y_stride, a.scale ? 1 : e);
+  if (a.residual) {
+    grid.with(a.residual, a.residual_stride, e);
+    grid.with(a.h, a.h_stride, e);
+  }
+  const int form = vec ? kVector : shifted_ok(grid, a.weight, a.width) ? kShifted : kPlain;
+  return dtype == GSA_DTYPE_BF16 ? launch_form<__nv_bfloat16>(a, form, stream)
+                                 : launch_form<float>(a, form, stream);
 }
 
 // 768 threads an SM, each with the next row's loads in flight: 16384 rows of 2048
@@ -449,15 +557,19 @@ cudaError_t launch_rms_norm_backward(const RmsNormBackwardArgs& a, int dtype,
   const bool vec = a.width % kVec == 0 && vector_ok(a.h, a.h_stride, e) &&
                    vector_ok(a.dy, a.dy_stride, e) && vector_ok(a.weight, 0, 1) &&
                    (!a.dh || vector_ok(a.dh, a.dh_stride, e)) && vector_ok(a.dx, a.dx_stride, e);
-  const int blocks = rms_norm_backward_blocks(a.rows, a.width);
+  Grid grid_of(a.h, a.h_stride, e, a.rows);
+  grid_of.with(a.dy, a.dy_stride, e);
+  grid_of.with(a.dx, a.dx_stride, e);
+  if (a.dh) grid_of.with(a.dh, a.dh_stride, e);
+  const int form = vec ? kVector : shifted_ok(grid_of, a.weight, a.width) ? kShifted : kPlain;
+  int blocks = rms_norm_backward_blocks(a.rows, a.width);
+  if (form == kShifted && blocks < a.rows) blocks = blocks / kVec * kVec;
   if (blocks > 0) {
-    const Shape s = shape_of(a.rows, a.width, 32);
+    const Shape s = shape_of(a.rows, a.width + (form == kShifted ? kVec - 1 : 0), 32);
     if (dtype == GSA_DTYPE_BF16)
-      vec ? launch_back<__nv_bfloat16, true>(a, s, blocks, stream)
-          : launch_back<__nv_bfloat16, false>(a, s, blocks, stream);
+      launch_back_form<__nv_bfloat16>(a, form, s, blocks, stream);
     else
-      vec ? launch_back<float, true>(a, s, blocks, stream)
-          : launch_back<float, false>(a, s, blocks, stream);
+      launch_back_form<float>(a, form, s, blocks, stream);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return err;
   }

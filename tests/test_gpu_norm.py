@@ -208,3 +208,51 @@ def test_graph_and_stream():
     torch.cuda.synchronize()
     assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8))
     assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("wdtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("width,rows", [(9, 4001), (15, 3), (17, 4001), (250, 2100), (2047, 700),
+                                        (4099, 2050), (8191, 300), (16389, 20), (32761, 9),
+                                        (32767, 9)])
+def test_rows_off_the_grid(dtype, wdtype, width, rows):
+    """Widths that put every row at another place of the 16-byte grid, more of them than blocks."""
+    x, res = rnd(rows, width, seed=21).to(DT[dtype]), rnd(rows, width, seed=22).to(DT[dtype])
+    w = (1 + 0.2 * rnd(width, seed=23)).to(DT[wdtype])
+    dy, dh = rnd(rows, width, seed=24).to(DT[dtype]), rnd(rows, width, seed=25).to(DT[dtype])
+    leaves = [t.detach().requires_grad_() for t in (x, w, res)]
+    y, h = gsa.rms_norm(leaves[0], leaves[1], residual=leaves[2])
+    got = torch.autograd.grad([y, h], leaves, [dy, dh])
+    ry, rh = norm_ref(x, w, 1e-6, res)
+    assert torch.equal(h.double(), rh)
+    err = (y.double() - ry).abs()
+    assert (err <= (TOL[dtype] + 4e-6) * ry.abs()).all()
+    # the gradients' formulas in 64 bits, from the h that the norm read
+    hd, wd, dyd = h.detach().double(), w.double(), dy.double()
+    r = (hd.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    p = dyd * wd
+    dx = r * (p - hd * r * r * (p * hd).mean(-1, keepdim=True)) + dh.double()
+    # dx is a sum of terms that may cancel: their rounding in fp32, and the output's own
+    size = r * (p.abs() + hd.abs() * r * r * (p * hd).mean(-1, keepdim=True).abs()) + dh.abs()
+    assert ((got[0].double() - dx).abs() <= TOL[dtype] * dx.abs() + 4e-6 * size).all()
+    assert torch.equal(got[0], got[2])
+    assert rel(got[1], (dyd * hd * r).sum(0)) <= (1e-5 if wdtype == "fp32" else 2.0 ** -8)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_one_tensor_off_the_others_grid(dtype):
+    """An odd width whose residual, or gradient, lies in wider rows than the input."""
+    x, wide = rnd(40, 1001, seed=26).to(DT[dtype]), rnd(41, 1004, seed=27).to(DT[dtype])
+    w = (1 + 0.2 * rnd(1001, seed=28)).to(DT[dtype])
+    for res in (wide[:40, 2:1003], wide[1:, :1001], rnd(40 * 1001 + 3, seed=29).to(
+            DT[dtype])[3:].view(40, 1001)):
+        y, h = gsa.rms_norm(x, w, residual=res)
+        ry, rh = norm_ref(x, w, 1e-6, res)
+        assert torch.equal(h.double(), rh) and rel(y, ry) <= TOL[dtype]
+        y8, s = gsa.rms_norm_fp8(x, w, residual=res)[:2]
+        assert rel(s, ry.abs().amax(-1, keepdim=True) / 448) <= 4e-6
+        leaf = x.detach().requires_grad_()
+        out = gsa.rms_norm(leaf, w)
+        a, = torch.autograd.grad(out, leaf, res, retain_graph=True)
+        b, = torch.autograd.grad(out, leaf, res.contiguous())
+        assert rel(a, b) <= 2 * TOL[dtype]
