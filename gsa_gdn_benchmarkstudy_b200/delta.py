@@ -44,43 +44,51 @@ def _gates_ok(t: torch.Tensor) -> torch.Tensor:
 
 
 def _check(q, k, v, g, beta, *others) -> None:
-    _cuda(q, k, v, g, beta, *others)
-    for name, t, dims in (("q", q, 4), ("v", v, 4)):
-        if t.dim() != dims:
-            raise ValueError(f"{name}: expected {dims} dims, got {tuple(t.shape)}")
-    if q.dtype not in _DTYPES or g.dtype not in _DTYPES:
+    if not q.is_cuda:
+        _cuda(q, k, v, g, beta, *others)
+    device = q.get_device()
+    for t in (k, v, g, beta, *others):
+        if t is not None and t.get_device() != device:
+            _cuda(q, k, v, g, beta, *others)
+            raise ValueError("all tensors must be on one device")
+    q_shape, v_shape, g_shape = q.shape, v.shape, g.shape
+    for name, shape in (("q", q_shape), ("v", v_shape)):
+        if len(shape) != 4:
+            raise ValueError(f"{name}: expected 4 dims, got {tuple(shape)}")
+    dtype, gates = q.dtype, g.dtype
+    if dtype not in _DTYPES or gates not in _DTYPES:
         _dtype_code(q), _dtype_code(g)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError("q, k and v must share a dtype")
-    if beta.dtype != g.dtype:
+    if beta.dtype is not gates:
         raise ValueError("g and beta must share a dtype")
-    B, T, Hk, dk = q.shape
-    vB, vT, Hv, dv = v.shape
-    if k.shape != q.shape:
+    B, T, Hk, dk = q_shape
+    vB, vT, Hv, dv = v_shape
+    if k.shape != q_shape:
         raise ValueError(f"k must be [{B}, {T}, {Hk}, {dk}], got {tuple(k.shape)}")
     if vB != B or vT != T or Hk == 0 or Hv == 0 or Hv % Hk:
         raise ValueError(f"v must be [{B}, {T}, Hv, dv] with Hv a multiple of {Hk}, got "
-                         f"{tuple(v.shape)}")
-    gates = (B, T, Hv)
-    if g.shape != gates or beta.shape != gates:
-        raise ValueError(f"g and beta must be [{B}, {T}, {Hv}], got {tuple(g.shape)} and "
+                         f"{tuple(v_shape)}")
+    if g_shape != (B, T, Hv) or beta.shape != g_shape:
+        raise ValueError(f"g and beta must be [{B}, {T}, {Hv}], got {tuple(g_shape)} and "
                          f"{tuple(beta.shape)}")
     if dk % 8 or dv % 8 or not 0 < dk <= 128 or not 0 < dv <= 256:
         raise ValueError(f"dk and dv must be multiples of 8, dk <= 128 and dv <= 256, got "
                          f"{dk} and {dv}")
-    device = q.get_device()
-    for t in (k, v, g, beta, *others):
-        if t is not None and t.get_device() != device:
-            raise ValueError("all tensors must be on one device")
 
 
 def _args(q, k, v, g, beta, scale, N, cu, initial) -> bytes:
     """gsa_delta_t."""
     B, T, Hk, dk = q.shape
     _, _, Hv, dv = v.shape
+    q0, q1, q2, _ = q.stride()
+    k0, k1, k2, _ = k.stride()
+    v0, v1, v2, _ = v.stride()
+    g0, g1, _ = g.stride()
+    b0, b1, _ = beta.stride()
     return _lib.DELTA_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
-        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride()[:2], *beta.stride()[:2],
+        q0, q1, q2, k0, k1, k2, v0, v1, v2, g0, g1, b0, b1,
         0 if cu is None else cu.data_ptr(), 0 if initial is None else initial.data_ptr(),
         _DTYPES[q.dtype], _DTYPES[g.dtype], scale, B, T, Hk, Hv, dk, dv, N)
 

@@ -26,7 +26,13 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _check(x, weight, residual) -> None:
-    _cuda(x, weight, residual)
+    if not x.is_cuda:
+        _cuda(x, weight, residual)
+    device = x.get_device()
+    if weight.get_device() != device or (residual is not None
+                                         and residual.get_device() != device):
+        _cuda(x, weight, residual)
+        raise ValueError("all tensors must be on one device")
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError(f"x must have a last dim of at least 1, got {tuple(shape)}")
@@ -37,13 +43,8 @@ def _check(x, weight, residual) -> None:
         raise ValueError(f"rows of at most 32768 values, got {width}")
     if weight.shape != (width,):
         raise ValueError(f"weight must be [{width}], got {tuple(weight.shape)}")
-    if weight.device != x.device:
-        raise ValueError("all tensors must be on one device")
-    if residual is not None:
-        if residual.shape != shape or residual.dtype != x.dtype:
-            raise ValueError("residual must match x in shape and dtype")
-        if residual.device != x.device:
-            raise ValueError("all tensors must be on one device")
+    if residual is not None and (residual.shape != shape or residual.dtype is not x.dtype):
+        raise ValueError("residual must match x in shape and dtype")
 
 
 def _forward(x, weight, residual, eps, want_rstd):
@@ -146,6 +147,15 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     return y if h is None else (y, h)
 
 
+def _rows_of(t: torch.Tensor, width: int, group_size) -> torch.Tensor:
+    """t as rows [R, width] that the 8-bit kernel reads: group scales move 16 bytes at a time, so
+    rows that are not on 16 bytes are copied for them."""
+    t = _unit(t if t.dim() == 2 else t.reshape(-1, width))
+    if group_size and (t.data_ptr() % 16 or _row_stride(t) * t.element_size() % 16):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
                  residual: torch.Tensor | None = None, group_size: int | None = None):
     """``rms_norm`` with its output in 8 bits (torch.float8_e4m3fn) and fp32 scales.
@@ -165,29 +175,20 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
             residual is not None and residual.requires_grad)):
         raise RuntimeError("rms_norm_fp8 has no gradients; use rms_norm")
 
-    def usable(t):
-        """Group scales move 16 bytes at a time: rows that are not on 16 bytes are copied."""
-        es = t.element_size()
-        if group_size and (t.data_ptr() % 16 or _row_stride(t) * es % 16):
-            return t.clone(memory_format=torch.contiguous_format)
-        return t
-
-    x2 = usable(_unit(x if x.dim() == 2 else x.reshape(-1, width)))
-    r2 = None
-    if residual is not None:
-        r2 = usable(_unit(residual if x.dim() == 2 else residual.reshape(-1, width)))
+    x2 = _rows_of(x, width, group_size)
+    r2 = None if residual is None else _rows_of(residual, width, group_size)
     weight = weight.contiguous()
     if group_size and weight.data_ptr() % 16:
         weight = weight.clone()
     rows, groups = x2.shape[0], width // group_size if group_size else 1
     device, dtype = x.device, x.dtype
-    y = torch.empty((rows, width), dtype=torch.float8_e4m3fn, device=device)
-    scale = torch.empty((rows, groups), dtype=torch.float32, device=device)
+    y = (torch.empty_like(x2, dtype=torch.float8_e4m3fn) if x2.is_contiguous() else
+         x2.new_empty((rows, width), dtype=torch.float8_e4m3fn))
+    scale = x2.new_empty((rows, groups), dtype=torch.float32)
     h = h_ptr = r_ptr = None
     r_stride = 0
     if r2 is not None:
-        h = torch.empty_like(x2) if x2.is_contiguous() else torch.empty(
-            (rows, width), dtype=dtype, device=device)
+        h = torch.empty_like(x2) if x2.is_contiguous() else x2.new_empty((rows, width))
         h_ptr, r_ptr, r_stride = h.data_ptr(), r2.data_ptr(), _row_stride(r2)
     with _on(device):
         rc = _lib.load().gsa_rms_norm_fp8(
