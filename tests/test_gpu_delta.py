@@ -426,3 +426,45 @@ def test_inputs_changed_before_the_backward_are_noticed():
     v.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         o.sum().backward()
+
+
+def test_two_calls_at_once():
+    """Forward and backward on two streams side by side: each the same bits as alone."""
+    def run(leaves, do):
+        o, S = gsa.gated_delta_rule(*leaves, output_final_state=True)
+        return (o, S) + torch.autograd.grad(o, leaves, do)
+
+    work = []
+    for seed, (B, T, H) in enumerate([(1, 1500, 8), (4, 333, 16)]):
+        *a, r = make(B, T, H, H, 128, 128, seed=seed)
+        work.append(([t.requires_grad_() for t in a], r(B, T, H, 128).bfloat16()))
+    alone = [run(*w) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(5):
+        got = []
+        for s, w in zip(streams, work):
+            with torch.cuda.stream(s):
+                got.append(run(*w))
+        torch.cuda.synchronize()
+        for x, y in zip(alone, got):
+            assert all(torch.equal(p, q) for p, q in zip(x, y))
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_states_off_the_grid_and_inputs_that_are_one_tensor(dtype):
+    q, _, v, g, beta, r = make(2, 90, 2, 2, 64, 64, dtype, "fp32", seed=8)
+    S0 = r(2 * 2 * 64 * 64 + 1)[1:].view(2, 2, 64, 64)
+    check_forward((q, q, v, g, g.exp()), dtype, initial=S0)
+    dS = r(2 * 2 * 64 * 64 + 1)[1:].view(2, 2, 64, 64)
+    leaves = [t.requires_grad_() for t in (q, v, g)] + [S0.requires_grad_()]
+    got = torch.autograd.grad(
+        gsa.gated_delta_rule(q, q, v, g, beta, initial_state=S0, output_final_state=True)[1],
+        leaves, dS)
+    exact = [t.detach().double().requires_grad_() for t in leaves]
+    want = torch.autograd.grad(
+        delta_ref(exact[0], exact[0], exact[1], exact[2], beta, 0.125, exact[3])[1], exact,
+        dS.double())
+    for name, x, y in zip(("q and k", "v", "g", "S0"), got, want):
+        assert rel(x, y) <= (TOL["state", dtype] * 2 if name == "S0" else TOL["grad", dtype]), name

@@ -256,3 +256,19 @@ def test_one_tensor_off_the_others_grid(dtype):
         a, = torch.autograd.grad(out, leaf, res, retain_graph=True)
         b, = torch.autograd.grad(out, leaf, res.contiguous())
         assert rel(a, b) <= 2 * TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_residual_that_is_the_input_and_a_broadcast_gradient(dtype):
+    x = rnd(6, 200, seed=30).to(DT[dtype]).requires_grad_()
+    w = (1 + 0.2 * rnd(200, seed=31)).to(DT[dtype]).requires_grad_()
+    y, h = gsa.rms_norm(x, w, residual=x)
+    assert torch.equal(h, x + x)
+    got = torch.autograd.grad(y.sum(), [x, w])  # a gradient with strides of zero
+    xd, wd = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    hd = xd + xd
+    want = torch.autograd.grad((hd / torch.sqrt((hd * hd).mean(-1, keepdim=True) + 1e-6) * wd).sum(),
+                               [xd, wd])
+    # x gets two equal gradients, added up in its type
+    assert rel(got[0], want[0]) <= 2 * TOL[dtype]
+    assert rel(got[1], want[1]) <= (1e-5 if dtype == "fp32" else 2.0 ** -8)
