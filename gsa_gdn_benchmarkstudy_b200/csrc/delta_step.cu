@@ -6,11 +6,11 @@
 //   S <- a S + k u^T,
 // so the state is read once, stays in registers over all tokens of the call,
 // and is written once.  Bound by HBM: 8 * dk * dv bytes a head and sequence, and by
-// how many of them are on their way: 128 sequences of 16 heads of 128 x 128 take 49 us
-// with seven blocks of 16 KB an SM (72 registers a thread) and states that leave the
-// caches early, 53 with the four that 109 registers allow, 52 with eight, which spill
-// (a plain copy of the bytes takes 41).  Blocks of 64 and 128 columns take 61 and 83:
-// more warps meet at each barrier.
+// how many of them are on their way: 128 sequences of 16 heads of 128 x 128 take 48 us
+// with six blocks of 16 KB an SM (80 registers a thread, two columns an instruction)
+// and states that leave the caches early, 53 with the four that 109 registers allow,
+// 51 with eight, which spill (a plain copy of the bytes takes 41).  Blocks of 64 and
+// 128 columns took 61 and 83: more warps meet at each barrier.
 #include "delta_common.cuh"
 
 namespace gsa {
@@ -23,11 +23,11 @@ constexpr int kRowGroups = kThreads / 8;
 constexpr int kMaxRows = kDeltaMaxDk / kRowGroups;
 
 template <typename E>
-__global__ void __launch_bounds__(kThreads, 7) delta_step_kernel(const gsa_delta_t p, float* pool,
+__global__ void __launch_bounds__(kThreads, 6) delta_step_kernel(const gsa_delta_t p, float* pool,
                                                               int64_t slots,
                                                               const int32_t* indices, E* out,
                                                               int* err) {
-  __shared__ float sk[kDeltaMaxDk], sq[kDeltaMaxDk];
+  __shared__ uint64_t sk[kDeltaMaxDk], sq[kDeltaMaxDk];  // each value twice, for two columns
   __shared__ float part[4][2][kCols];
   __shared__ float dots[4];
   const int b = blockIdx.x, hv = blockIdx.y, col0 = blockIdx.z * kCols;
@@ -39,14 +39,18 @@ __global__ void __launch_bounds__(kThreads, 7) delta_step_kernel(const gsa_delta
   const int64_t slot = indices ? indices[b] : b;
   const bool inside = slot >= 0 && slot < slots;
 
-  float4 S[kMaxRows];
+  uint64_t S[kMaxRows][2];  // two pairs of columns
   float* state = pool + ((inside ? slot : 0) * p.Hv + hv) * static_cast<int64_t>(p.dk) * p.dv;
 #pragma unroll
   for (int i = 0; i < kMaxRows; ++i) {
     const int r = rg + i * kRowGroups;
-    S[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (inside && live && r < p.dk)
-      S[i] = __ldcs(reinterpret_cast<const float4*>(state + static_cast<int64_t>(r) * p.dv + col));
+    S[i][0] = S[i][1] = 0;
+    if (inside && live && r < p.dk) {
+      const ulonglong2 x = __ldcs(
+          reinterpret_cast<const ulonglong2*>(state + static_cast<int64_t>(r) * p.dv + col));
+      S[i][0] = x.x;
+      S[i][1] = x.y;
+    }
   }
   // Two rows of the batch must not share a state: the later one is refused, as
   // is an index outside the pool (-1 is an empty row): NaN out, no state
@@ -75,8 +79,8 @@ __global__ void __launch_bounds__(kThreads, 7) delta_step_kernel(const gsa_delta
           p.k)[b * p.k_stride[0] + tok * p.k_stride[1] + hk * p.k_stride[2] + i]);
       const float qv = to_float(static_cast<const E*>(
           p.q)[b * p.q_stride[0] + tok * p.q_stride[1] + hk * p.q_stride[2] + i]);
-      sk[i] = kv;
-      sq[i] = qv;
+      sk[i] = f2_pack(kv, kv);
+      sq[i] = f2_pack(qv, qv);
       qk = fmaf(qv, kv, qk);
     }
     const float a = expf(load_gate(p.g, b * p.g_stride[0] + tok * p.g_stride[1] + hv, gate16));
@@ -95,19 +99,23 @@ __global__ void __launch_bounds__(kThreads, 7) delta_step_kernel(const gsa_delta
     __syncthreads();
     qk = (dots[0] + dots[1]) + (dots[2] + dots[3]);
 
-    float r[4] = {}, w[4] = {};
+    uint64_t r2[2] = {}, w2[2] = {};
+    const uint64_t a2 = f2_pack(a, a);
 #pragma unroll
     for (int i = 0; i < kMaxRows; ++i) {
       const int row = rg + i * kRowGroups;
       if (row < p.dk) {
-        const float kv = sk[row], qv = sq[row];
-        S[i].x *= a; S[i].y *= a; S[i].z *= a; S[i].w *= a;
-        r[0] = fmaf(kv, S[i].x, r[0]); w[0] = fmaf(qv, S[i].x, w[0]);
-        r[1] = fmaf(kv, S[i].y, r[1]); w[1] = fmaf(qv, S[i].y, w[1]);
-        r[2] = fmaf(kv, S[i].z, r[2]); w[2] = fmaf(qv, S[i].z, w[2]);
-        r[3] = fmaf(kv, S[i].w, r[3]); w[3] = fmaf(qv, S[i].w, w[3]);
+        const uint64_t kv = sk[row], qv = sq[row];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          S[i][e] = f2_mul(S[i][e], a2);
+          r2[e] = f2_fma(kv, S[i][e], r2[e]);
+          w2[e] = f2_fma(qv, S[i][e], w2[e]);
+        }
       }
     }
+    float r[4] = {f2_lo(r2[0]), f2_hi(r2[0]), f2_lo(r2[1]), f2_hi(r2[1])};
+    float w[4] = {f2_lo(w2[0]), f2_hi(w2[0]), f2_lo(w2[1]), f2_hi(w2[1])};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {  // the warp's four row groups
 #pragma unroll
@@ -132,15 +140,14 @@ __global__ void __launch_bounds__(kThreads, 7) delta_step_kernel(const gsa_delta
         out[((static_cast<int64_t>(b) * p.T + tok) * p.Hv + hv) * p.dv + col + e] =
             from_float<E>(p.scale * fmaf(qk, u[e], ws));
     }
+    const uint64_t u2[2] = {f2_pack(u[0], u[1]), f2_pack(u[2], u[3])};
 #pragma unroll
     for (int i = 0; i < kMaxRows; ++i) {
       const int row = rg + i * kRowGroups;
       if (row < p.dk) {
-        const float kv = sk[row];
-        S[i].x = fmaf(kv, u[0], S[i].x);
-        S[i].y = fmaf(kv, u[1], S[i].y);
-        S[i].z = fmaf(kv, u[2], S[i].z);
-        S[i].w = fmaf(kv, u[3], S[i].w);
+        const uint64_t kv = sk[row];
+        S[i][0] = f2_fma(kv, u2[0], S[i][0]);
+        S[i][1] = f2_fma(kv, u2[1], S[i][1]);
       }
     }
     __syncthreads();  // sk, sq, part and dots are written again by the next token
@@ -149,7 +156,8 @@ __global__ void __launch_bounds__(kThreads, 7) delta_step_kernel(const gsa_delta
   for (int i = 0; i < kMaxRows; ++i) {
     const int r = rg + i * kRowGroups;
     if (live && r < p.dk)
-      __stcs(reinterpret_cast<float4*>(state + static_cast<int64_t>(r) * p.dv + col), S[i]);
+      __stcs(reinterpret_cast<ulonglong2*>(state + static_cast<int64_t>(r) * p.dv + col),
+             make_ulonglong2(S[i][0], S[i][1]));
   }
 }
 

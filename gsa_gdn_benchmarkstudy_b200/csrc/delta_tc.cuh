@@ -88,11 +88,6 @@ __device__ __forceinline__ uint64_t desc_cols(uint32_t tile, int ks, uint32_t st
   return sdesc_sw128(tile + ks * 2048, step, 1024);
 }
 
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // x, y as hi + lo pairs of bf16.
 __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = pack_bf16x2(x, y);

@@ -16,8 +16,8 @@
 // row was measured at 16384 rows of 2048 (bf16, residual; a plain copy of the
 // same bytes takes 41 us): 32 threads x 8 vectors 55 us, 64 x 4 47, 128 x 2 47,
 // 256 x 1 51; with an 8-bit output (36 us) 62, 47, 53, 63.  Fewer vectors a thread
-// leave too few loads in flight, more of them too few warps.  Held to 64 registers
-// (of 70) 64 x 4 takes 45; the other forms would spill.
+// leave too few loads in flight, more of them too few warps.  Sums and products two
+// values at a time bring 64 x 4 to 44 and 46.
 #include <cuda_fp8.h>
 
 #include "kernels.h"
@@ -32,8 +32,15 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
-__device__ __forceinline__ float round_f(float v, float) { return v; }
-__device__ __forceinline__ float round_f(float v, __nv_bfloat16) { return bf16_round(v); }
+// Two values at a time: the sums and products are one instruction for both.
+__device__ __forceinline__ uint64_t pair(const float (&v)[kVec], int e) {
+  return f2_pack(v[e], v[e + 1]);
+}
+__device__ __forceinline__ uint64_t round_f(uint64_t v, float) { return v; }
+__device__ __forceinline__ uint64_t round_f(uint64_t v, __nv_bfloat16) {
+  const uint32_t r = pack_bf16x2(f2_lo(v), f2_hi(v));
+  return f2_pack(__uint_as_float(r << 16), __uint_as_float(r & 0xFFFF0000u));
+}
 
 // How a thread's vectors of 8 values lie in a row.
 //   kPlain    neighbours go to neighbouring threads, one value a load;
@@ -65,7 +72,7 @@ __host__ __device__ __forceinline__ int off_grid(const E* p) {
 
 // Eight values as they lie in memory: loads that can wait to be converted.  ONCE:
 // they leave the caches early.  The backward pass gains by it (54 to 50 us, figures as
-// above), the forward pass loses (45 to 51): its inputs and outputs are often in L2.
+// above), the forward pass loses (45 to 51).
 template <typename E>
 struct Raw {
   static constexpr int kWords = kVec * sizeof(E) / 16;
@@ -243,8 +250,7 @@ enum NormOut { kNormPlain = 0, kNormRow8 = 1, kNormGroup8 = 2 };
 // tpr threads share a row; a block holds blockDim.x / tpr rows (more than one
 // only where a row is a warp or less).
 template <typename E, int FORM, int NV, int OUT, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 && FORM == kVector && sizeof(E) == 2 ? 4 : 1)
-    rms_norm_kernel(RmsNormArgs a, int tpr) {
+__global__ void __launch_bounds__(THREADS) rms_norm_kernel(RmsNormArgs a, int tpr) {
   __shared__ float slots[2][32];
   const int t = threadIdx.x % tpr;
   int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
@@ -265,16 +271,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 && FORM == kVector && 
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[i][e] = round_f(v[i][e] + r[i][e], E());
+      for (int e = 0; e < kVec; e += 2) {
+        const uint64_t h2 = round_f(f2_add(pair(v[i], e), pair(r[i], e)), E());
+        v[i][e] = f2_lo(h2);
+        v[i][e + 1] = f2_hi(h2);
+      }
       if (live) store8<FORM>(v[i], h, i, t, tpr, a.width, shift);
     }
   }
-  float s = 0.f;
+  uint64_t s2 = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) s = fmaf(v[i][e], v[i][e], s);
-  s = row_fold<false>(s, slots[0], tpr);
+    for (int e = 0; e < kVec; e += 2) s2 = f2_fma(pair(v[i], e), pair(v[i], e), s2);
+  const float s = row_fold<false>(f2_lo(s2) + f2_hi(s2), slots[0], tpr);
   const float rstd = 1.0f / sqrtf(s / static_cast<float>(a.width) + a.eps);
   if (a.rstd && live && t == 0) a.rstd[row] = rstd;
 #pragma unroll
@@ -282,7 +292,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 && FORM == kVector && 
     float w[kVec];
     load_weight<FORM>(w, a, i, t, tpr, shift);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) v[i][e] = v[i][e] * rstd * w[e];
+    for (int e = 0; e < kVec; e += 2) {
+      const uint64_t y2 = f2_mul(f2_mul(pair(v[i], e), f2_pack(rstd, rstd)), pair(w, e));
+      v[i][e] = f2_lo(y2);
+      v[i][e + 1] = f2_hi(y2);
+    }
   }
   if constexpr (OUT == kNormPlain) {
     E* y = static_cast<E*>(a.y) + row * a.y_stride;
@@ -315,7 +329,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 && FORM == kVector && 
       }
       const float inv = 448.0f / most;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[i][e] *= inv;
+      for (int e = 0; e < kVec; e += 2) {
+        const uint64_t y2 = f2_mul(pair(v[i], e), f2_pack(inv, inv));
+        v[i][e] = f2_lo(y2);
+        v[i][e + 1] = f2_hi(y2);
+      }
       if (live) store8_e4m3<FORM>(v[i], y, i, t, tpr, a.width, shift);
     }
   }
@@ -542,7 +560,8 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, int dtype, cudaStream_t stream
 
 // 768 threads an SM, each with the next row's loads in flight: 16384 rows of 2048
 // took 53 us so, 57 with twice as many, 65 with two thirds (41 us for the bytes);
-// more blocks also mean more partial sums of dw.  512 threads where each holds two
+// more blocks also mean more partial sums of dw.  (Two values at a time, as forwards: 51
+// to 50 us, but 51 to 61 at 4096 rows of 8192, where registers run out.)  512 threads where each holds two
 // vectors, so that all blocks run at once: 8192 rows of 4096 take 70 us with 768.
 int rms_norm_backward_blocks(int64_t rows, int width) {
   const Shape s = shape_of(rows, width, 32);
