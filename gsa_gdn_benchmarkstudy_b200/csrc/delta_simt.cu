@@ -12,7 +12,9 @@
 // 128 with zeros, so every leading dimension is a constant, 4 past a multiple of 8
 // words: 16-byte loads of eight rows then touch every bank once.
 // Bound by shared memory (4 + NJ to 4 + 4 NJ loads for 16 NJ multiply-adds) and,
-// with few sequences and heads, by the length of a chunk's chain of products.
+// with few sequences and heads, by the length of a chunk's chain of products: 2 x 333
+// tokens, 4 heads of 64 x 96, take 10 us prep, 54 chain, 55 rev, 64 grad (465 us with a
+// load for every value, copies that nothing overlaps, and a column a thread of T).
 #include "delta_common.cuh"
 
 namespace gsa {

@@ -559,10 +559,11 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, int dtype, cudaStream_t stream
 }
 
 // 768 threads an SM, each with the next row's loads in flight: 16384 rows of 2048
-// took 53 us so, 57 with twice as many, 65 with two thirds (41 us for the bytes);
-// more blocks also mean more partial sums of dw.  (Two values at a time, as forwards: 51
-// to 50 us, but 51 to 61 at 4096 rows of 8192, where registers run out.)  512 threads where each holds two
-// vectors, so that all blocks run at once: 8192 rows of 4096 take 70 us with 768.
+// took 53 us so (50 since the inputs leave the caches early), 57 with twice as many,
+// 65 with two thirds (41 us for the bytes); more blocks also mean more partial sums of
+// dw.  512 threads where each holds two vectors, so that all blocks run at once: 8192
+// rows of 4096 take 70 us with 768, 67 so.  Two values an instruction, as forwards,
+// take 50 us, but 61 instead of 51 at 4096 rows of 8192, where registers run out.
 int rms_norm_backward_blocks(int64_t rows, int width) {
   const Shape s = shape_of(rows, width, 32);
   const int threads = s.nv == 1 ? 768 : 512;
