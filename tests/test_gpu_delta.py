@@ -468,3 +468,42 @@ def test_states_off_the_grid_and_inputs_that_are_one_tensor(dtype):
         dS.double())
     for name, x, y in zip(("q and k", "v", "g", "S0"), got, want):
         assert rel(x, y) <= (TOL["state", dtype] * 2 if name == "S0" else TOL["grad", dtype]), name
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values a tensor.  The last 128 tokens start from a wiped state, so they, and
+    their gradients, are those of a call on them alone."""
+    T, H, d, tail = 2 ** 20 + 128, 16, 128, 128
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v, do = (torch.randn(1, T, H, d, generator=gen, device="cuda", dtype=torch.bfloat16)
+                   for _ in range(4))
+    q.mul_(d ** -0.5), k.mul_(d ** -0.5)
+    g = torch.full((1, T, H), -0.05, device="cuda")
+    g[:, T - tail] = -math.inf
+    beta = torch.full((1, T, H), 0.5, device="cuda")
+    results = []
+    for part in (slice(0, T), slice(T - tail, T)):
+        leaves = [t[:, part].detach().requires_grad_() for t in (q, k, v, beta)]
+        o, S = gsa.gated_delta_rule(*leaves[:3], g[:, part], leaves[3], output_final_state=True)
+        grads = torch.autograd.grad(o, leaves, do[:, part])
+        results.append([o[:, -tail:].clone(), S.clone()] + [t[:, -tail:].clone() for t in grads])
+        del o, S, grads, leaves
+    for name, a, b in zip(("o", "S", "q", "k", "v", "beta"), *results):
+        assert torch.isfinite(a).all()
+        assert rel(a, b) <= TOL["o" if name == "o" else "state" if name == "S" else "grad", "bf16"]
+    del q, k, v, do, results
+    torch.cuda.empty_cache()
+
+
+def test_slots_past_32_bits():
+    *a, r = make(3, 2, 16, 16, 128, 128, seed=11)
+    pool = torch.zeros(8195, 16, 128, 128, device="cuda")  # 2^31 values and 3 states
+    few = r(3, 16, 128, 128)
+    slots = torch.tensor([8194, 0, 8192], dtype=torch.int32, device="cuda")
+    pool[slots.long()] = few
+    o = gsa.gated_delta_step(*a, pool, state_indices=slots)
+    want = gsa.gated_delta_step(*a, few)
+    assert torch.equal(o, want) and torch.equal(pool[slots.long()], few)
+    assert not pool[1].any() and not pool[8193].any() and not pool[8191].any()
+    del pool
+    torch.cuda.empty_cache()

@@ -272,3 +272,30 @@ def test_residual_that_is_the_input_and_a_broadcast_gradient(dtype):
     # x gets two equal gradients, added up in its type
     assert rel(got[0], want[0]) <= 2 * TOL[dtype]
     assert rel(got[1], want[1]) <= (1e-5 if dtype == "fp32" else 2.0 ** -8)
+
+
+@pytest.mark.parametrize("width", [32768, 32767])
+def test_offsets_past_32_bits(width):
+    """More than 2^31 values a tensor: the last rows are those of a call on them alone."""
+    rows, tail = 65552, 8
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x, dy = (torch.randn(rows, width, generator=gen, device="cuda", dtype=torch.bfloat16)
+             for _ in range(2))
+    w = (1 + 0.2 * rnd(width, seed=5)).bfloat16()
+    leaf = x.requires_grad_()
+    y = gsa.rms_norm(leaf, w)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    last = x[-tail:].detach().clone().requires_grad_()
+    part = gsa.rms_norm(last, w)
+    want, = torch.autograd.grad(part, last, dy[-tail:])
+    assert rel(y[-tail:], part) <= TOL["bf16"] and rel(dx[-tail:], want) <= TOL["bf16"]
+    with torch.no_grad():
+        del dx, dy, y
+        y8, s = gsa.rms_norm_fp8(x, w)
+        want8, want_s = gsa.rms_norm_fp8(last, w)
+        assert rel(s[-tail:], want_s) <= 4e-6
+        # values at a rounding boundary may fall to either side: a step of e4m3, 2^-3
+        err = (y8[-tail:].float() - want8.float()).abs()
+        assert (err <= want8.float().abs() * 2.0 ** -3 + 2.0 ** -9).all()
+        del y8, x, leaf
+    torch.cuda.empty_cache()
