@@ -136,8 +136,6 @@ class _GatedDeltaRule(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, do, dfinal):
         q, k, v, g, beta, cu, ws = ctx.saved_tensors
-        B, T, Hk, dk = q.shape
-        Hv, dv_ = v.shape[2], v.shape[3]
         if do is not None:
             do = do.to(q.dtype).contiguous()
             if do.data_ptr() % 16:
@@ -147,20 +145,17 @@ class _GatedDeltaRule(torch.autograd.Function):
         with _on(q.device):
             a = _args(q, k, v, g, beta, ctx.scale, ctx.N, cu, None)
             scratch = _workspace(a, _lib.GSA_DELTA_BACKWARD, q.device)
-            dq = torch.empty(B, T, Hk, dk, dtype=q.dtype, device=q.device)
-            dk_ = torch.empty_like(dq)
-            dv = torch.empty(B, T, Hv, dv_, dtype=q.dtype, device=q.device)
-            dg = torch.empty(B, T, Hv, dtype=g.dtype, device=q.device)
-            dbeta = torch.empty_like(dg)
-            dinitial = (torch.empty(ctx.N, Hv, dk, dv_, dtype=torch.float32, device=q.device)
+            dq, dk, dv, dg, dbeta = _like(q), _like(k), _like(v), _like(g), _like(beta)
+            dinitial = (torch.empty(ctx.N, v.shape[2], q.shape[3], v.shape[3],
+                                    dtype=torch.float32, device=q.device)
                         if ctx.has_initial and ctx.needs_input_grad[5] else None)
             rc = _lib.load().gsa_delta_rule_backward(
                 a, _ptr(do), _ptr(dfinal), ws.data_ptr(), ws.numel(),
-                scratch.data_ptr(), scratch.numel(), dq.data_ptr(), dk_.data_ptr(), dv.data_ptr(),
+                scratch.data_ptr(), scratch.numel(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                 dg.data_ptr(), dbeta.data_ptr(), _ptr(dinitial),
                 _raw_stream(q.device.index))
         _lib.check(rc, "gsa_delta_rule_backward")
-        return dq, dk_, dv, dg, dbeta, dinitial, None, None, None, None
+        return dq, dk, dv, dg, dbeta, dinitial, None, None, None, None
 
 
 def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor,

@@ -92,12 +92,12 @@ class _RmsNorm(torch.autograd.Function):
         if dy is None:  # only the sum h was used
             return dh, None, dh, None
         h, weight, rstd = ctx.saved_tensors
-        h, dy = _unit(h), _unit(dy)
+        h, dy = _unit(h), _unit(dy.to(h.dtype))
         rows, width = h.shape
         dh_ptr = dw = dw_ptr = ws = ws_ptr = None
         dh_stride = need = 0
         if dh is not None:
-            dh = _unit(dh)
+            dh = _unit(dh.to(h.dtype))
             dh_ptr, dh_stride = dh.data_ptr(), _row_stride(dh)
         lib, device = _lib.load(), h.device
         dx = torch.empty_like(h) if h.is_contiguous() else torch.empty(
@@ -105,7 +105,7 @@ class _RmsNorm(torch.autograd.Function):
         if want_w:
             dw = torch.empty_like(weight)
             need = lib.gsa_rms_norm_backward_workspace_size(rows, width)
-            ws = torch.empty(need, dtype=torch.uint8, device=device)
+            ws = rstd.new_empty(need // 4)  # floats
             dw_ptr, ws_ptr = dw.data_ptr(), ws.data_ptr()
         with _on(device):
             rc = lib.gsa_rms_norm_backward(

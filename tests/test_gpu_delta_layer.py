@@ -154,3 +154,23 @@ def test_training_step():
         grads.append(torch.autograd.grad(run(*leaves), leaves, [dy.to(to), dh.to(to)]))
     for name, a, b in zip(("x", "residual", "w_in", "unit", "w_out"), *grads):
         assert rel(a, b) <= 2.4e-4, (name, rel(a, b))
+
+
+def test_gradients_of_another_type():
+    """Gradients of the outputs in fp32 for operators in bf16, and the other way round."""
+    for dtype, other in ((torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)):
+        x, res = rows(5, 96, dtype=dtype, seed=1), rows(5, 96, dtype=dtype, seed=2)
+        w = weights(dtype)[2]
+        up = rows(5, 96, dtype=torch.bfloat16, seed=3)  # the same values in either type
+        leaves = [t.requires_grad_() for t in (x, w, res)]
+        outs = gsa.rms_norm(leaves[0], leaves[1], residual=leaves[2])
+        a = torch.autograd.grad(outs, leaves, [up.to(other)] * 2, retain_graph=True)
+        b = torch.autograd.grad(outs, leaves, [up.to(dtype)] * 2)
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+        mixed = [t.detach().requires_grad_() for t in inputs(
+            rows(1, 70, WIDTH, dtype=dtype, seed=4), weights(dtype)[1], gsa.rms_norm)]
+        o = gsa.gated_delta_rule(*mixed)[0]
+        up = rows(1, 70, HV, DV, dtype=torch.bfloat16, seed=5)
+        a = torch.autograd.grad(o, mixed, up.to(other), retain_graph=True)
+        b = torch.autograd.grad(o, mixed, up.to(dtype))
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
