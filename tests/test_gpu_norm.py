@@ -299,3 +299,14 @@ def test_offsets_past_32_bits(width):
         assert (err <= want8.float().abs() * 2.0 ** -3 + 2.0 ** -9).all()
         del y8, x, leaf
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("wdtype", ["fp32", "bf16"])
+def test_no_rows(wdtype):
+    x = torch.empty(0, 48, device="cuda", requires_grad=True)
+    w = rnd(48, seed=33).to(DT[wdtype]).requires_grad_()
+    y, h = gsa.rms_norm(x, w, residual=x)
+    dx, dw = torch.autograd.grad([y, h], [x, w], [torch.empty_like(y), torch.empty_like(h)])
+    assert dx.shape == (0, 48) and not dw.any() and dw.dtype == w.dtype
+    y8, s = gsa.rms_norm_fp8(x.detach(), w.detach())
+    assert y8.shape == (0, 48) and s.shape == (0, 1)
