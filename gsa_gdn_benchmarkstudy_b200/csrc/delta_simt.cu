@@ -89,7 +89,7 @@ __device__ __forceinline__ void multiply(float (&acc)[4][NJ], const float (&a)[4
 // acc += a b over k = first .. last - 1 (multiples of 4).
 template <int NJ, typename A, typename B>
 __device__ __forceinline__ void product(float (&acc)[4][NJ], int first, int last, A a, B b) {
-#pragma unroll 4
+#pragma unroll(NJ > 2 ? 2 : 4)
   for (int k = first; k < last; k += 4) {
     float av[4][4], bv[4][NJ];
     a.load(av, row0(), k);
@@ -101,7 +101,7 @@ __device__ __forceinline__ void product(float (&acc)[4][NJ], int first, int last
 template <int NJ, typename A, typename B>
 __device__ __forceinline__ void product2(float (&acc)[4][NJ], float (&more)[4][NJ], int last, A a,
                                          A a2, B b) {
-#pragma unroll 4
+#pragma unroll(NJ > 2 ? 2 : 4)
   for (int k = 0; k < last; k += 4) {
     float av[4][4], bv[4][NJ];
     b.load(bv, k, col0_of());
