@@ -43,6 +43,15 @@ def _gates_ok(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _int32(t: torch.Tensor, least: int) -> torch.Tensor:
+    """Whole numbers as contiguous int32.  What int32 does not hold becomes ``least`` or 2^31 - 1,
+    which the kernels refuse as they would the number itself: no pool has 2^31 states (the smallest
+    is 256 bytes) and no call so many tokens."""
+    if t.dtype is not torch.int32:
+        t = t.clamp(least, 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
+
+
 def _check(q, k, v, g, beta, *others) -> None:
     if not q.is_cuda:
         _cuda(q, k, v, g, beta, *others)
@@ -188,7 +197,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
             raise ValueError("cu_seqlens must be int32 or int64 [N + 1] with N >= 1")
         if B != 1:
             raise ValueError("cu_seqlens needs a batch of 1")
-        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+        cu_seqlens = _int32(cu_seqlens, -1)
         N = cu_seqlens.numel() - 1
     if initial_state is not None:
         if initial_state.shape != (N, Hv, dk, dv) or initial_state.dtype != torch.float32:
@@ -233,7 +242,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         if state_indices.shape != (B,) or state_indices.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"state_indices must be int32 or int64 [{B}]")
         if state_indices.dtype is not torch.int32 or not state_indices.is_contiguous():
-            state_indices = state_indices.to(torch.int32).contiguous()
+            state_indices = _int32(state_indices, -2)
     elif slots < B:
         raise ValueError(f"{B} rows need as many states, got {slots}")
     scale = dk ** -0.5 if scale is None else float(scale)
