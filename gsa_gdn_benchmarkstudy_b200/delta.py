@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .ops import _DTYPES, _cuda, _dtype_code, _on, _ptr, _raw_stream
@@ -255,4 +256,6 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
             _raw_stream(q.device.index))
     if rc:
         _lib.check(rc, "gsa_delta_step")
+    if not state.is_inference():
+        increment_version(state)  # graphs that saved it notice
     return o

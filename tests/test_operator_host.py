@@ -81,3 +81,29 @@ def test_wide_cu_seqlens_stay_wrong(library, cu):
     got = library.cu_seqlens
     assert [x for x, y in zip(got, cu) if 0 <= y <= T] == [y for y in cu if 0 <= y <= T]
     assert all(x < 0 or x > T for x, y in zip(got, cu) if not 0 <= y <= T)
+
+
+def test_step_counts_as_a_change_of_the_state(library):
+    """A graph that saved the states must notice that the step has overwritten them."""
+    pool = torch.zeros(3, 2, 16, 16)
+    w = torch.ones_like(pool, requires_grad=True)
+    loss = (pool * w).sum()
+    gsa.gated_delta_step(*inputs(T=1), pool)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+    base = torch.zeros(2, 3, 2, 16, 16)  # a view's base and its other views share the count
+    loss = (base[1] * w).sum()
+    gsa.gated_delta_step(*inputs(T=1), base[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+
+
+def test_step_in_inference_mode(library):
+    """States made in inference mode carry no count."""
+    with torch.inference_mode():
+        pool = torch.zeros(3, 2, 16, 16)
+        gsa.gated_delta_step(*inputs(T=1), pool)
+    outside = torch.zeros(3, 2, 16, 16)
+    with torch.inference_mode():
+        gsa.gated_delta_step(*inputs(T=1), outside)
+    gsa.gated_delta_step(*inputs(T=1), outside)
