@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from .ops import _DTYPES, _cuda, _dtype_code, _on, _ptr, _raw_stream
+from .ops import _DTYPES, _cuda, _dtype_code, _no_tangents, _on, _ptr, _raw_stream
 
 
 def _rows_ok(t: torch.Tensor) -> torch.Tensor:
@@ -54,6 +54,7 @@ def _int32(t: torch.Tensor, least: int) -> torch.Tensor:
 
 
 def _check(q, k, v, g, beta, *others) -> None:
+    _no_tangents(q, k, v, g, beta, *others)
     if not q.is_cuda:
         _cuda(q, k, v, g, beta, *others)
     device = q.get_device()
@@ -183,7 +184,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     other; rows of no sequence come out, and in the gradients, as zeros.
 
     Returns (o [B, T, Hv, dv] in q's dtype, final state [N, Hv, dk, dv] fp32 or
-    None).  Differentiable once in q, k, v, g, beta and the initial state; the
+    None).  Differentiable once, in reverse mode, in q, k, v, g, beta and the initial state; the
     gradients have the inputs' dtypes and add up in a fixed order.  States, decays
     and sums are fp32; bf16 gradients are formed from factors rounded to bf16.
     Keys are expected near unit length (``rms_norm`` with weight dk ** -0.5 makes

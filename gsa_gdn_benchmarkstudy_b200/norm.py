@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _DTYPES, _cuda, _dtype_code, _on, _ptr, _raw_stream
+from .ops import _DTYPES, _cuda, _dtype_code, _no_tangents, _on, _ptr, _raw_stream
 
 
 def _unit(t: torch.Tensor) -> torch.Tensor:
@@ -26,6 +26,7 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _check(x, weight, residual) -> None:
+    _no_tangents(x, weight, residual)
     if not x.is_cuda:
         _cuda(x, weight, residual)
     device = x.get_device()
@@ -124,7 +125,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     x [..., D] (bf16 or fp32), weight [D] (bf16 or fp32).  Returns y in x's dtype, or
     (y, h) with ``residual`` (x's shape and dtype): h = x + residual rounded to
     that dtype, which is what the norm reads and the next residual is.
-    Differentiable once in x, weight and the residual; the weight's gradient
+    Differentiable once, in reverse mode, in x, weight and the residual; the weight's gradient
     adds the rows up in a fixed order."""
     _check(x, weight, residual)
     weight = weight.contiguous()

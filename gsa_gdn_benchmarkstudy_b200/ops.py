@@ -16,6 +16,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -46,6 +47,16 @@ def _cuda(*ts: torch.Tensor) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError("gsa_b200 runs only on CUDA tensors (no CPU fallback)")
+
+
+def _no_tangents(*ts: torch.Tensor) -> None:
+    """Raises for a tensor that carries a forward-mode derivative: it has no requires_grad, and
+    the result would come out as a constant."""
+    if forward_ad._current_level < 0:  # what unpack_dual looks at first, for every tensor
+        return
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("no forward-mode derivatives")
 
 
 def _rows(t: torch.Tensor, width: int, name: str) -> int:

@@ -107,3 +107,33 @@ def test_step_in_inference_mode(library):
     with torch.inference_mode():
         gsa.gated_delta_step(*inputs(T=1), outside)
     gsa.gated_delta_step(*inputs(T=1), outside)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("at", range(6))
+def test_forward_mode_derivatives_are_refused(library, grad, at):
+    """A tangent must not be dropped, whether reverse mode is on or not."""
+    from torch.autograd import forward_ad
+    x = [*inputs(T=1), torch.zeros(1, 2, 16, 16)]
+    rows = [torch.ones(4, 128), torch.ones(128), torch.ones(4, 128)]
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        x[at] = forward_ad.make_dual(x[at], torch.ones_like(x[at]))
+        for call in (lambda: gsa.gated_delta_rule(*x[:5], initial_state=x[5]),
+                     lambda: gsa.gated_delta_step(*x)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        if at < 3:
+            rows[at] = forward_ad.make_dual(rows[at], torch.ones_like(rows[at]))
+            for norm_of in (gsa.rms_norm, gsa.rms_norm_fp8):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    norm_of(rows[0], rows[1], residual=rows[2])
+    with torch.no_grad(), forward_ad.dual_level():  # no tangents: an ordinary call
+        gsa.gated_delta_step(*inputs(T=1), torch.zeros(1, 2, 16, 16))
+
+
+def test_function_transforms_are_refused(library):
+    x = [*inputs(T=1), torch.zeros(1, 2, 16, 16)]
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda q: gsa.gated_delta_rule(q, *x[1:5])[0], (x[0],), (x[0],))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda v: gsa.rms_norm(v, torch.ones(16)), (x[2],), (x[2],))
