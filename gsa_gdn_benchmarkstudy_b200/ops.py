@@ -35,7 +35,8 @@ def _stream() -> int:
 
 
 _HERE = contextlib.nullcontext()
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device index
+# the current stream of a device index (a torch without CUDA has none, and no call gets as far)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _on(device: torch.device):

@@ -2,6 +2,9 @@
 reach the library, and what autograd is told.  CPU tensors against a stand-in for the library."""
 import contextlib
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -137,3 +140,20 @@ def test_function_transforms_are_refused(library):
         torch.func.jvp(lambda q: gsa.gated_delta_rule(q, *x[1:5])[0], (x[0],), (x[0],))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda v: gsa.rms_norm(v, torch.ones(16)), (x[2],), (x[2],))
+
+
+def test_import_without_cuda_in_torch():
+    """A torch built without CUDA has no raw streams; the package's host parts still import."""
+    code = ("import torch\n"
+            "if hasattr(torch._C, '_cuda_getCurrentRawStream'):\n"
+            "    del torch._C._cuda_getCurrentRawStream\n"
+            "import gsa_gdn_benchmarkstudy_b200 as gsa\n"
+            "try:\n"
+            "    gsa.rms_norm(torch.zeros(2, 8), torch.zeros(8))\n"
+            "except RuntimeError as e:\n"
+            "    assert 'only on CUDA' in str(e)\n"
+            "else:\n"
+            "    raise SystemExit('no error')\n")
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
+                         cwd=Path(__file__).resolve().parent.parent)
+    assert got.returncode == 0, got.stderr
