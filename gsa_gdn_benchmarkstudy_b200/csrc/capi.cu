@@ -195,6 +195,13 @@ struct ProjLayout {
 };
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Whether the (maybe NULL) pointers lie on whole elements of `size` bytes, a power of two.
+template <typename... P>
+bool on_elements(size_t size, const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & (size - 1)) == 0;
+}
+size_t size_of(int dtype) { return dtype == GSA_DTYPE_BF16 ? 2 : 4; }
+int off_elements() { return set_error(GSA_ERR_ALIGNMENT, "pointer between two elements"); }
 
 int finish(cudaError_t e) { return e == cudaSuccess ? GSA_OK : set_cuda_error(e); }
 
@@ -947,6 +954,9 @@ bool delta_rows_ok(const void* q, const int64_t* stride, const gsa_delta_t& p, i
 }
 
 int check_delta_inputs(const gsa_delta_t* p) {
+  if (!on_elements(size_of(p->dtype), p->q, p->k, p->v) ||
+      !on_elements(size_of(p->gate_dtype), p->g, p->beta))
+    return off_elements();
   if (static_cast<int64_t>(p->B) * p->T == 0) return GSA_OK;
   if (!p->q || !p->k || !p->v || !p->g || !p->beta)
     return set_error(GSA_ERR_INVALID_ARG, "q / k / v / g / beta is NULL");
@@ -1038,6 +1048,9 @@ int gsa_delta_rule_forward(const gsa_delta_t* p, void* o, float* final_state, in
   if (p->B == 0 || p->N == 0) return GSA_OK;
   if ((rc = check_delta_inputs(p))) return rc;
   if (!o && p->T > 0) return set_error(GSA_ERR_INVALID_ARG, "o is NULL");
+  if (!on_elements(4, p->cu_seqlens, p->initial_state, final_state) ||
+      !on_elements(size_of(p->dtype), o))
+    return off_elements();
   if (p->dtype == GSA_DTYPE_BF16 && !aligned16(o))
     return set_error(GSA_ERR_ALIGNMENT, "o must be 16-byte aligned");
   const int64_t need = gsa_delta_rule_workspace_size(p, use);
@@ -1070,6 +1083,10 @@ int gsa_delta_rule_backward(const gsa_delta_t* p, const void* dout, const float*
   if ((rc = check_delta_inputs(p))) return rc;
   if (p->T > 0 && (!dq || !dk || !dv || !dg || !dbeta))
     return set_error(GSA_ERR_INVALID_ARG, "dq / dk / dv / dg / dbeta is NULL");
+  if (!on_elements(4, p->cu_seqlens, dfinal, dinitial) ||
+      !on_elements(size_of(p->dtype), dout, dq, dk, dv) ||
+      !on_elements(size_of(p->gate_dtype), dg, dbeta))
+    return off_elements();
   if (p->dtype == GSA_DTYPE_BF16 &&
       (!aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv)))
     return set_error(GSA_ERR_ALIGNMENT, "bf16 gradients must be 16-byte aligned");
@@ -1110,6 +1127,7 @@ int gsa_delta_step(const gsa_delta_t* p, float* state, int64_t slots, const int3
   if (p->B == 0 || p->T == 0) return GSA_OK;
   if ((rc = check_delta_inputs(p))) return rc;
   if (!o || (!state && slots > 0)) return set_error(GSA_ERR_INVALID_ARG, "o / state is NULL");
+  if (!on_elements(4, indices) || !on_elements(size_of(p->dtype), o)) return off_elements();
   if (!aligned16(state)) return set_error(GSA_ERR_ALIGNMENT, "state must be 16-byte aligned");
   DeviceState* st = nullptr;
   if ((rc = device_state(&st))) return rc;
@@ -1135,6 +1153,9 @@ int rms_norm_impl(gsa::RmsNormArgs a, int dtype, int weight_dtype, void* stream)
   if (a.rows == 0) return GSA_OK;
   if (!a.x || !a.weight || !a.y) return set_error(GSA_ERR_INVALID_ARG, "x / weight / y is NULL");
   if (a.residual && !a.h) return set_error(GSA_ERR_INVALID_ARG, "a residual needs h");
+  if (!on_elements(size_of(dtype), a.x, a.residual, a.h, a.scale ? nullptr : a.y) ||
+      !on_elements(size_of(weight_dtype), a.weight) || !on_elements(4, a.rstd, a.scale))
+    return off_elements();
   if (a.x_stride < 0 || a.y_stride < a.width || (a.residual && a.residual_stride < 0) ||
       (a.residual && a.h_stride < a.width))
     return set_error(GSA_ERR_INVALID_ARG, "bad row stride");
@@ -1184,6 +1205,9 @@ int gsa_rms_norm_backward(const void* dy, int64_t dy_stride, const void* dh, int
   if (rows == 0 && !dweight) return GSA_OK;
   if (rows > 0 && (!dy || !h || !weight || !rstd || !dx))
     return set_error(GSA_ERR_INVALID_ARG, "dy / h / weight / rstd / dx is NULL");
+  if (!on_elements(size_of(dtype), dy, dh, h, dx) ||
+      !on_elements(size_of(weight_dtype), weight, dweight) || !on_elements(4, rstd))
+    return off_elements();
   if (rows > 0 && (dy_stride < 0 || h_stride < 0 || (dh && dh_stride < 0) || dx_stride < width))
     return set_error(GSA_ERR_INVALID_ARG, "bad row stride");
   const int64_t need = dweight ? gsa_rms_norm_backward_workspace_size(rows, width) : 0;

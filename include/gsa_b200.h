@@ -41,7 +41,7 @@ extern "C" {
 typedef enum {
   GSA_OK = 0,
   GSA_ERR_INVALID_ARG = 1,     /* null pointer, non-positive or inconsistent size */
-  GSA_ERR_ALIGNMENT = 2,       /* pointer or stride breaks a 16-byte rule */
+  GSA_ERR_ALIGNMENT = 2,       /* pointer or stride breaks a 16-byte rule, or an element's */
   GSA_ERR_UNSUPPORTED = 3,     /* shape/dtype this build does not implement */
   GSA_ERR_CUDA = 4,            /* a CUDA runtime/driver call failed */
   GSA_ERR_DEVICE_TIMEOUT = 5,  /* a bounded device-side wait expired */

@@ -191,3 +191,69 @@ def test_norm_shapes(no_device_check):
         gsa.rms_norm_fp8(x, w, group_size=128)
     with pytest.raises(RuntimeError, match="no gradients"):
         gsa.rms_norm_fp8(x.requires_grad_(), w)
+
+
+# Addresses between two elements, which a kernel could only fault on: refused before any device
+# work.  4096 stands for a good address; nothing reads it, because each call has one bad one.
+def test_delta_addresses_between_elements(lib):
+    for dtype, gates in ((0, 0), (0, 1), (1, 0), (1, 1)):
+        def make(**over):
+            a = args(dtype=dtype, gate_dtype=gates)
+            for n in ("q", "k", "v"):
+                setattr(a, n, 4096)
+                getattr(a, n + "_stride")[:] = [1 << 20, 1 << 10, 128]
+            a.g = a.beta = 4096
+            for n, v in over.items():
+                setattr(a, n, v)
+            return a
+
+        word, gate = (2 if dtype == 0 else 4), (2 if gates == 0 else 4)
+        inputs = {"q": word, "k": word, "v": word, "g": gate, "beta": gate}
+
+        def forward(a, o=4096, final=4096):
+            return lib.gsa_delta_rule_forward(ctypes.byref(a), o, final, 0, 4096, 1 << 40, None)
+
+        def backward(a, at=None):
+            p = [4096] * 10
+            if at is not None:
+                p[at[0]] = at[1]
+            dout, dfinal, dq, dk, dv, dg, dbeta, dinitial = p[:8]
+            return lib.gsa_delta_rule_backward(
+                ctypes.byref(a), dout, dfinal, 4096, 1 << 40, 4096, 1 << 40, dq, dk, dv, dg,
+                dbeta, dinitial, None)
+
+        def step(a, indices=4096, o=4096):
+            return lib.gsa_delta_step(ctypes.byref(a), 4096, 9, indices, o, None)
+
+        for name, size in inputs.items():
+            bad = make(**{name: 4096 + size // 2})
+            assert forward(bad) == 2 and backward(bad) == 2 and step(bad) == 2, name
+        assert forward(make(initial_state=4098)) == 2
+        assert forward(make(initial_state=4098, T=0)) == 2
+        assert forward(make(cu_seqlens=4098, B=1)) == 2
+        assert backward(make(cu_seqlens=4098, B=1)) == 2
+        assert forward(make(), o=4096 + word // 2) == 2
+        assert forward(make(), final=4098) == 2 and forward(make(T=0), final=4098) == 2
+        for i, size in enumerate((word, 4, word, word, word, gate, gate, 4)):
+            assert backward(make(), (i, 4096 + size // 2)) == 2, i
+        assert backward(make(T=0), (1, 4098)) == 2 and backward(make(T=0), (7, 4098)) == 2
+        assert step(make(), indices=4098) == 2 and step(make(), o=4096 + word // 2) == 2
+
+
+def test_norm_addresses_between_elements(lib):
+    for dtype, wdtype in ((0, 0), (0, 1), (1, 0), (1, 1)):
+        word, weight = (2 if dtype == 0 else 4), (2 if wdtype == 0 else 4)
+
+        def off(sizes, call):
+            good = [4096] * len(sizes)
+            for i, size in enumerate(sizes):
+                if size > 1:
+                    assert call(*(good[:i] + [4096 + size // 2] + good[i + 1:])) == 2, i
+
+        off([word, word, weight, word, word, 4], lambda x, r, w, y, h, rstd: lib.gsa_rms_norm(
+            x, 8, r, 8, w, wdtype, 1e-6, dtype, 2, 8, y, 8, h, 8, rstd, None))
+        off([word, word, weight, 1, 4, word], lambda x, r, w, y, s, h: lib.gsa_rms_norm_fp8(
+            x, 8, r, 8, w, wdtype, 1e-6, dtype, 2, 8, y, 8, s, 0, h, 8, None))
+        off([word, word, word, weight, 4, word, weight],
+            lambda dy, dh, h, w, rstd, dx, dw: lib.gsa_rms_norm_backward(
+                dy, 8, dh, 8, h, 8, w, wdtype, rstd, dtype, 2, 8, dx, 8, dw, 4096, 1 << 40, None))
