@@ -70,14 +70,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
-// ... and 8.
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-      : "memory");
-}
-
 // Tiles of `step` bytes for 64 columns.  Rows are the outer dimension (M or N) and
 // columns contracted: columns 16 ks .. 16 ks + 15.
 __device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int ks, uint32_t step = kTile) {

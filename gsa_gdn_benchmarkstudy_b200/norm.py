@@ -89,7 +89,7 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        want_x, want_w, want_r, _ = ctx.needs_input_grad
+        _, want_w, want_r, _ = ctx.needs_input_grad
         if dy is None:  # only the sum h was used
             return dh, None, dh, None
         h, weight, rstd = ctx.saved_tensors
