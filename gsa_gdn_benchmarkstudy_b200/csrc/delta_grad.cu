@@ -16,11 +16,12 @@
 // key head one after the other, so that their gradients add up in one order.  All
 // products have 128 rows: channels (dO S0^T and its like, transposed: S0's image is
 // the left operand), or N's and dY's tokens on top of one another.  The factors
-// are bf16, rounded once: the results are bf16 too.  About 210 KB a chunk and head
-// of 128 x 128 come and go, the next head's while this one's elements are worked on:
-// 64 heads of 4096 tokens take 285 us, 130 for the bytes.  Bound by the chain of copies,
-// products and passes within a head (a block an SM: its operands fill shared memory;
-// 33% of the cycles issue, 14% multiply).
+// are bf16, rounded once, as dQ and dK are in the end (off by about 3e-3 together).  dg
+// and dbeta are sums of products of the same factors, also where the gates are fp32 (about
+// 2e-3 then).  About 210 KB a chunk and head of 128 x 128 come and go, the next
+// head's while this one's elements are worked on: 64 heads of 4096 tokens take 285 us, 130 for the bytes.  Bound by the chain of copies,
+// products and passes within a head (a block an SM: its operands take 202 KB of shared
+// memory; 33% of the cycles issue, 14% multiply; 248 bytes of registers spill).
 #include "delta_tc.cuh"
 
 namespace gsa {

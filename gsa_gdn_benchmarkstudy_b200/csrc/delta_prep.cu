@@ -9,7 +9,7 @@
 // the sequential pass copies whole, so bulk copies store them.  Bound by latency:
 // loads, the product, a triangular inverse and 34 KB of stores one after the
 // other; six blocks an SM overlap theirs.  256 chunks of 16 heads of 128 channels take
-// 65 us (32 for the bytes); products by mma.sync, copies and stores by the threads, four
+// 65 us (42 for the bytes); products by mma.sync, copies and stores by the threads, four
 // blocks an SM: 94.
 #include "delta_tc.cuh"
 

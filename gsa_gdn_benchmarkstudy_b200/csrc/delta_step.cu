@@ -6,11 +6,12 @@
 //   S <- a S + k u^T,
 // so the state is read once, stays in registers over all tokens of the call,
 // and is written once.  Bound by HBM: 8 * dk * dv bytes a head and sequence, and by
-// how many of them are on their way: 128 sequences of 16 heads of 128 x 128 take 48 us
-// with six blocks of 16 KB an SM (80 registers a thread, two columns an instruction)
-// and states that leave the caches early, 53 with the four that 109 registers allow,
-// 51 with eight, which spill (a plain copy of the bytes takes 41).  Blocks of 64 and
-// 128 columns took 61 and 83: more warps meet at each barrier.
+// how many of them are on their way: a batch of 128 rows, 117 of them with a state of
+// 16 heads of 128 x 128, takes 48 us (5.1 TB/s; 38 at a plain copy's rate) with six
+// blocks of 16 KB an SM (80 registers a thread, two columns an instruction) and states
+// that leave the caches early, 53 with the four that 109 registers allow, 51 with
+// eight, which spill.  Blocks of 64 and 128 columns took 61 and 83: more warps meet at
+// each barrier.
 #include "delta_common.cuh"
 
 namespace gsa {

@@ -563,7 +563,9 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, int dtype, cudaStream_t stream
 // 65 with two thirds (41 us for the bytes); more blocks also mean more partial sums of
 // dw.  512 threads where each holds two vectors, so that all blocks run at once: 8192
 // rows of 4096 take 70 us with 768, 67 so.  Two values an instruction, as forwards,
-// take 50 us, but 61 instead of 51 at 4096 rows of 8192, where registers run out.
+// take 50 us, but 61 instead of 51 at 4096 rows of 8192, where registers run out.  Past
+// 8192 values a row's 1024 threads have at most 64 registers each and spill (bf16 0.5 to 4
+// KB a thread); in fp32 the 512 threads of rows past 4096 do too (0.2 to 0.4 KB).
 int rms_norm_backward_blocks(int64_t rows, int width) {
   const Shape s = shape_of(rows, width, 32);
   const int threads = s.nv == 1 ? 768 : 512;

@@ -179,14 +179,17 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     (value head h reads key head h // (Hv // Hk)), dk <= 128 and dv <= 256,
     multiples of 8; g (log decay, at most 0) and beta [B, T, Hv], both bf16 or
     both fp32; scale defaults to dk ** -0.5.  ``initial_state`` [N, Hv, dk, dv]
-    fp32 (default zeros).  With ``cu_seqlens`` (int32 [N + 1] on the device, as
+    fp32 (default zeros).  With ``cu_seqlens`` (int32 or int64 [N + 1] on the device, as
     ``[0, n_0, n_0 + n_1, ...]``) B is 1 and the N sequences lie one behind the
     other; rows of no sequence come out, and in the gradients, as zeros.
 
     Returns (o [B, T, Hv, dv] in q's dtype, final state [N, Hv, dk, dv] fp32 or
     None).  Differentiable once, in reverse mode, in q, k, v, g, beta and the initial state; the
     gradients have the inputs' dtypes and add up in a fixed order.  States, decays
-    and sums are fp32; bf16 gradients are formed from factors rounded to bf16.
+    and sums are held in fp32.  From bf16 inputs the products take pairs of bf16 for
+    the state, which comes out within about 5e-6 of exact, and single ones for the
+    gradients: dq and dk are within about 3e-3, dg and dbeta within about 2e-3 where
+    the gates, and so they, are fp32.  fp32 inputs keep fp32 throughout.
     Keys are expected near unit length (``rms_norm`` with weight dk ** -0.5 makes
     them), values finite."""
     _check(q, k, v, g, beta, initial_state, cu_seqlens)
@@ -223,10 +226,11 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
 
     Inputs as ``gated_delta_rule`` with T the tokens of the step (usually 1).
     ``state`` [slots, Hv, dk, dv] fp32, contiguous: sequence b has the slot
-    ``state_indices[b]`` (int32 [B] on the device; default b); -1 marks an empty
+    ``state_indices[b]`` (int32 or int64 [B] on the device; default b); -1 marks an empty
     row of the batch, whose output is zero.  An index outside [-1, slots) or one
     that an earlier row has already is refused on the device: that row comes out
     as NaN, no state changes for it, and ``_lib.device_error()`` reports it.
+    Autograd counts the call as a change of ``state`` in place.
     Returns o [B, T, Hv, dv].  No gradients."""
     _check(q, k, v, g, beta, state, state_indices)
     B, T, _, dk = q.shape

@@ -426,9 +426,11 @@ GSA_API int gsa_fused_projection_pack(const void* w_q, const void* w_k,
  *   Sequences that overlap or leave [0, T] are cut to their order and to T,
  *   and the device error word (gsa_device_error) is set.
  *   initial_state float32 [N, Hv, dk, dv] contiguous, or NULL for zeros.
- * bf16: tensor cores with 16-bit pairs for the state, so the state keeps
- * about fp32's accuracy; q, k, v rows 16-byte aligned and strides positive
- * (gsa_delta_rule_*).  f32: CUDA cores.
+ * bf16: tensor cores with pairs of bf16 for the state's products, so states come
+ * out within about 5e-6 of exact (2-norm); gradients are formed from factors
+ * rounded to bf16 (dq, dk within about 3e-3; dg, dbeta within about 2e-3 where the
+ * gates, and so they, are float32).  q, k, v rows 16-byte aligned and strides
+ * positive (gsa_delta_rule_*).  f32: CUDA cores, fp32 throughout (about 5e-7).
  */
 typedef struct {
   const void* q;
